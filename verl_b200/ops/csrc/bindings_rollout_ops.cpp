@@ -1,0 +1,236 @@
+// torch.ops.verl_b200.* bindings of the page bookkeeping, the 4-bit cache and the scores of logits.
+#include <ATen/ATen.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/library.h>
+
+#include <tuple>
+
+#include "rollout_ops.h"
+
+namespace {
+
+using at::Tensor;
+using OptTensor = c10::optional<at::Tensor>;
+
+inline cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
+inline long long* lptr(const Tensor& t) { return reinterpret_cast<long long*>(t.data_ptr<int64_t>()); }
+#define CHECK_RC(rc, what) TORCH_CHECK((rc) == 0, what " failed with code ", (rc))
+
+// A vector of n whole numbers on the device of `like`.
+void check_vec(const Tensor& t, at::ScalarType type, int64_t n, const Tensor& like, const char* what) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.scalar_type() == type && t.dim() == 1 && t.size(0) == n && t.is_contiguous(), what,
+              ": expected a contiguous ", type, " vector of ", n, " on ", like.device(), ", got ", t.scalar_type(), " ", t.sizes(), " on ", t.device());
+}
+void check_table(const Tensor& t, const char* what) {
+  TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kInt && t.dim() == 2 && t.stride(1) == 1 && t.size(0) <= INT_MAX && t.size(1) <= INT_MAX, what,
+              ": block_table must be a CUDA int32 matrix with contiguous rows");
+}
+int type_of(const Tensor& t, bool f32, const char* what) {
+  TORCH_CHECK(t.is_cuda(), what, ": expected a CUDA tensor");
+  if (t.scalar_type() == at::kBFloat16) return 0;
+  if (t.scalar_type() == at::kHalf) return 1;
+  TORCH_CHECK(f32 && t.scalar_type() == at::kFloat, what, f32 ? ": expected bf16, fp16 or fp32" : ": expected bf16 or fp16", ", got ", t.scalar_type());
+  return 2;
+}
+
+std::tuple<Tensor, Tensor, Tensor> decode_slot_map(const Tensor& table, const Tensor& pos, const Tensor& ctx, const Tensor& active, int64_t bs) {
+  check_table(table, "decode_slot_map");
+  const int64_t S = table.size(0);
+  check_vec(pos, at::kInt, S, table, "decode_slot_map: pos");
+  check_vec(ctx, at::kInt, S, table, "decode_slot_map: ctx");
+  check_vec(active, at::kBool, S, table, "decode_slot_map: active");
+  TORCH_CHECK(bs > 0 && bs <= (1 << 20), "decode_slot_map: block_size");
+  const c10::cuda::CUDAGuard guard(table.device());
+  Tensor slots = at::empty({S}, table.options().dtype(at::kLong)), ctx_out = at::empty({S}, table.options()), plan = at::empty({S + 1}, table.options());
+  verl_count_launches(1);
+  CHECK_RC(vb_decode_slot_map(table.data_ptr<int>(), table.stride(0), (int)table.size(1), pos.data_ptr<int>(), ctx.data_ptr<int>(),
+                              active.data_ptr<bool>(), (int)S, (int)bs, lptr(slots), ctx_out.data_ptr<int>(), plan.data_ptr<int>(), cur_stream()),
+           "vb_decode_slot_map");
+  return {slots, ctx_out, plan};
+}
+
+Tensor extend_block_tables_(Tensor table, const Tensor& rows, const Tensor& have, const Tensor& lengths, const Tensor& pool, int64_t bs) {
+  check_table(table, "extend_block_tables_");
+  const int64_t B = rows.size(0);
+  check_vec(rows, at::kInt, B, table, "extend_block_tables_: rows");
+  check_vec(have, at::kInt, B, table, "extend_block_tables_: have");
+  check_vec(lengths, at::kInt, B, table, "extend_block_tables_: lengths");
+  check_vec(pool, at::kInt, pool.size(0), table, "extend_block_tables_: pool");
+  TORCH_CHECK(bs > 0 && bs <= (1 << 20) && table.size(1) <= (1 << 20) && B <= (1 << 20) && pool.size(0) <= INT_MAX,
+              "extend_block_tables_: at most 2^20 rows of at most 2^20 blocks");
+  const c10::cuda::CUDAGuard guard(table.device());
+  Tensor used = at::empty({1}, table.options());
+  if (B == 0) return used.zero_();
+  verl_count_launches(1);
+  CHECK_RC(vb_extend_block_tables(table.data_ptr<int>(), table.stride(0), (int)table.size(0), (int)table.size(1), rows.data_ptr<int>(),
+                                  have.data_ptr<int>(), lengths.data_ptr<int>(), (int)B, pool.data_ptr<int>(), (int)pool.size(0), (int)bs,
+                                  used.data_ptr<int>(), cur_stream()),
+           "vb_extend_block_tables");
+  return used;
+}
+
+std::tuple<Tensor, Tensor, Tensor> build_slot_map(const Tensor& table, const Tensor& rows, const Tensor& starts, const Tensor& ends, int64_t bs,
+                                                  int64_t total) {
+  check_table(table, "build_slot_map");
+  const int64_t B = rows.size(0);
+  check_vec(rows, at::kInt, B, table, "build_slot_map: rows");
+  check_vec(starts, at::kInt, B, table, "build_slot_map: starts");
+  check_vec(ends, at::kInt, B, table, "build_slot_map: ends");
+  TORCH_CHECK(bs > 0 && bs <= (1 << 20), "build_slot_map: block_size");
+  TORCH_CHECK(total >= 0 && total <= (1 << 22) && B <= 8192, "build_slot_map: at most 2^22 tokens of at most 8192 sequences, got ", total, " of ", B);
+  const c10::cuda::CUDAGuard guard(table.device());
+  Tensor cu = at::empty({B + 1}, table.options()), positions = at::empty({total}, table.options()),
+         slots = at::empty({total}, table.options().dtype(at::kLong));
+  verl_count_launches(1);
+  CHECK_RC(vb_build_slot_map(table.data_ptr<int>(), table.stride(0), (int)table.size(0), (int)table.size(1), rows.data_ptr<int>(),
+                             starts.data_ptr<int>(), ends.data_ptr<int>(), (int)B, (int)bs, (int)total, cu.data_ptr<int>(),
+                             positions.data_ptr<int>(), lptr(slots), cur_stream()),
+           "vb_build_slot_map");
+  return {cu, positions, slots};
+}
+
+// Block size of a 4-bit pool [blocks, heads, bytes of a page] for heads of hd channels.
+int64_t kv4_block(const Tensor& pages, int64_t hd, const char* what) {
+  TORCH_CHECK(pages.is_cuda() && pages.scalar_type() == at::kByte && pages.dim() == 3 && pages.is_contiguous() &&
+              reinterpret_cast<uintptr_t>(pages.data_ptr()) % 16 == 0, what, ": pages must be a contiguous CUDA uint8 tensor [blocks, heads, page bytes]");
+  TORCH_CHECK(hd > 0 && hd % 32 == 0 && hd <= 1024, what, ": heads of a multiple of 32 channels, got ", hd);
+  const int64_t bs = pages.size(2) * 4 / (5 * hd);
+  TORCH_CHECK(bs > 0 && bs * hd * 5 == pages.size(2) * 4 && bs % 16 == 0, what, ": pages of ", pages.size(2),
+              " bytes hold no multiple of 16 tokens of a head of ", hd);
+  TORCH_CHECK(bs <= 1024, what, ": blocks of at most 1024 tokens");
+  return bs;
+}
+
+void kv4_append_(const Tensor& k, const Tensor& v, const Tensor& slots, Tensor pages) {
+  const int type = type_of(k, false, "kv4_append_");
+  TORCH_CHECK(v.scalar_type() == k.scalar_type() && v.device() == k.device() && k.device() == pages.device() && k.dim() == 3 && v.sizes() == k.sizes(),
+              "kv4_append_: k and v [tokens, heads, channels] of one type on the device of the pages");
+  const int64_t T = k.size(0), nkv = k.size(1), hd = k.size(2);
+  const int64_t bs = kv4_block(pages, hd, "kv4_append_");
+  TORCH_CHECK(pages.size(1) == nkv, "kv4_append_: the pages hold ", pages.size(1), " heads, k has ", nkv);
+  check_vec(slots, at::kLong, T, k, "kv4_append_: slots");
+  if (T == 0 || nkv == 0 || pages.size(0) == 0) return;
+  for (const Tensor* t : {&k, &v})
+    TORCH_CHECK(t->stride(2) == 1 && (nkv == 1 || t->stride(1) == hd) && (T == 1 || t->stride(0) % 8 == 0) &&
+                reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, "kv4_append_: heads of a token side by side, tokens on 16-byte boundaries");
+  const c10::cuda::CUDAGuard guard(k.device());
+  verl_count_launches(1);
+  CHECK_RC(vb_kv4_append(type, k.data_ptr(), v.data_ptr(), T == 1 ? 0 : k.stride(0), T == 1 ? 0 : v.stride(0), lptr(slots), pages.data_ptr(), (int)T,
+                         (int)nkv, (int)hd, (int)bs, pages.size(0) * bs, cur_stream()),
+           "vb_kv4_append");
+}
+
+std::tuple<Tensor, Tensor> kv4_gather(const Tensor& pages, const Tensor& slots, int64_t hd, at::ScalarType dtype) {
+  const int64_t bs = kv4_block(pages, hd, "kv4_gather"), T = slots.size(0), nkv = pages.size(1);
+  TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kHalf, "kv4_gather: bf16 or fp16");
+  check_vec(slots, at::kLong, T, pages, "kv4_gather: slots");
+  const c10::cuda::CUDAGuard guard(pages.device());
+  Tensor k = at::empty({T, nkv, hd}, pages.options().dtype(dtype)), v = at::empty_like(k);
+  if (T == 0 || nkv == 0) return {k, v};
+  verl_count_launches(1);
+  CHECK_RC(vb_kv4_gather(dtype == at::kHalf, pages.data_ptr(), lptr(slots), k.data_ptr(), v.data_ptr(), (int)T, (int)nkv, (int)hd, (int)bs,
+                         pages.size(0) * bs, cur_stream()),
+           "vb_kv4_gather");
+  return {k, v};
+}
+
+Tensor paged_decode_kv4(const Tensor& q, const Tensor& pages, const Tensor& table, const Tensor& ctx, const OptTensor& plan, double scale) {
+  VbKv4Decode a{};
+  a.type = type_of(q, false, "paged_decode_kv4");
+  TORCH_CHECK(q.dim() == 3 && (q.size(2) == 64 || q.size(2) == 128), "paged_decode_kv4: q [sequences, heads, 64 or 128 channels]");
+  const int64_t B = q.size(0), nh = q.size(1), hd = q.size(2), bs = kv4_block(pages, hd, "paged_decode_kv4"), nkv = pages.size(1);
+  TORCH_CHECK(pages.device() == q.device() && table.device() == q.device(), "paged_decode_kv4: tensors on several devices");
+  TORCH_CHECK(nkv > 0 && nh > 0 && nh % nkv == 0 && nh / nkv <= 16, "paged_decode_kv4: at most 16 query heads to a key head, got ", nh, " / ", nkv);
+  TORCH_CHECK((bs & (bs - 1)) == 0 && bs <= 256, "paged_decode_kv4: blocks of 16, 32, 64, 128 or 256 tokens, got ", bs);
+  check_table(table, "paged_decode_kv4");
+  TORCH_CHECK(table.size(0) == B && pages.size(0) <= INT_MAX && B <= 65535, "paged_decode_kv4: one table row for each of at most 65535 sequences");
+  check_vec(ctx, at::kInt, B, q, "paged_decode_kv4: ctx_len");
+  if (plan.has_value()) check_vec(*plan, at::kInt, B + 1, q, "paged_decode_kv4: plan");
+  const c10::cuda::CUDAGuard guard(q.device());
+  Tensor out = at::empty({B, nh, hd}, q.options());
+  if (B == 0) return out;
+  if (pages.size(0) == 0 || table.size(1) == 0) return out.zero_();
+  TORCH_CHECK(q.stride(2) == 1 && q.stride(1) == hd && (B == 1 || q.stride(0) % 8 == 0) && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
+              "paged_decode_kv4: heads of a sequence side by side, sequences on 16-byte boundaries");
+  a.q = q.data_ptr(); a.ldq = B == 1 ? 0 : q.stride(0);
+  a.pages = pages.data_ptr<uint8_t>(); a.num_blocks = (int)pages.size(0); a.block_size = (int)bs;
+  a.table = table.data_ptr<int>(); a.width = (int)table.size(1); a.ldt = table.stride(0);
+  a.ctx = ctx.data_ptr<int>(); a.out = out.data_ptr();
+  a.B = (int)B; a.nh = (int)nh; a.nkv = (int)nkv; a.hd = (int)hd; a.scale = (float)scale;
+  Tensor made, part;
+  if (plan.has_value()) {
+    a.plan = plan->data_ptr<int>();
+  } else {
+    made = at::empty({B + 1}, ctx.options());
+    a.plan_ws = made.data_ptr<int>();
+  }
+  const long long n = vb_kv4_decode_scratch(a.B, a.nh, a.nkv, a.hd);
+  if (n > 0) {
+    part = at::empty({n}, q.options().dtype(at::kFloat));
+    a.part = part.data_ptr<float>();
+  }
+  CHECK_RC(vb_kv4_decode(&a, cur_stream()), "vb_kv4_decode");
+  return out;
+}
+
+VbScores scores_of(const Tensor& x, const Tensor& ids, double temperature, int64_t valid, const char* what) {
+  VbScores a{};
+  a.type = type_of(x, true, what);
+  TORCH_CHECK(x.dim() == 2 && (x.stride(1) == 1 || x.size(1) <= 1) && x.size(1) > 0 && x.size(1) < INT_MAX && x.size(0) <= INT_MAX, what,
+              ": logits [rows, vocabulary] with contiguous rows");
+  TORCH_CHECK(valid > 0 && valid <= x.size(1), what, ": valid_vocab must lie in 1 .. ", x.size(1), ", got ", valid);
+  TORCH_CHECK(temperature > 0, what, ": temperature must be positive");
+  TORCH_CHECK(ids.device() == x.device() && ids.scalar_type() == at::kLong && ids.dim() == 2 && ids.size(0) == x.size(0) && ids.is_contiguous(), what,
+              ": ids must be a contiguous int64 matrix with a row for each row of logits");
+  TORCH_CHECK(ids.size(1) <= 4096, what, ": at most 4096 given tokens a row");
+  a.x = x.data_ptr(); a.ldx = x.size(0) <= 1 ? 0 : x.stride(0); a.T = (int)x.size(0); a.V = (int)valid;
+  a.inv_temp = (float)(1.0 / temperature);
+  a.ids = lptr(ids); a.K = (int)ids.size(1);
+  return a;
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_scores(const Tensor& x, const Tensor& ids, int64_t top, double temperature, int64_t valid) {
+  VbScores a = scores_of(x, ids, temperature, valid, "token_scores");
+  TORCH_CHECK(top >= 0 && top <= 128 && top <= valid, "token_scores: top_k must lie in 0 .. min(128, valid_vocab), got ", top);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const auto f32 = x.options().dtype(at::kFloat);
+  Tensor lp = at::empty(ids.sizes(), f32), ent = at::empty({x.size(0)}, f32), lse = at::empty({x.size(0)}, f32);
+  Tensor top_ids = at::empty({x.size(0), top}, ids.options()), top_lp = at::empty({x.size(0), top}, f32);
+  a.top = (int)top;
+  a.logprob = lp.data_ptr<float>(); a.entropy = ent.data_ptr<float>(); a.lse = lse.data_ptr<float>();
+  a.top_ids = lptr(top_ids); a.top_lp = top_lp.data_ptr<float>();
+  CHECK_RC(vb_token_scores(&a, cur_stream()), "vb_token_scores");
+  return {lp, ent, lse, top_ids, top_lp};
+}
+
+Tensor token_scores_bwd(const Tensor& x, const Tensor& ids, const Tensor& lse, const Tensor& ent, const Tensor& g_lp, const OptTensor& g_ent,
+                        double temperature, int64_t valid) {
+  VbScores a = scores_of(x, ids, temperature, valid, "token_scores_bwd");
+  const int64_t T = x.size(0);
+  check_vec(lse, at::kFloat, T, x, "token_scores_bwd: lse");
+  check_vec(ent, at::kFloat, T, x, "token_scores_bwd: entropy");
+  TORCH_CHECK(g_lp.device() == x.device() && g_lp.scalar_type() == at::kFloat && g_lp.sizes() == ids.sizes() && g_lp.is_contiguous(),
+              "token_scores_bwd: g_logprob must be a contiguous fp32 tensor of the shape of ids");
+  if (g_ent.has_value()) check_vec(*g_ent, at::kFloat, T, x, "token_scores_bwd: g_entropy");
+  const c10::cuda::CUDAGuard guard(x.device());
+  Tensor dx = at::empty({T, x.size(1)}, x.options());
+  a.lse = lse.data_ptr<float>(); a.entropy = ent.data_ptr<float>();
+  CHECK_RC(vb_token_scores_bwd(&a, g_lp.data_ptr<float>(), g_ent.has_value() ? g_ent->data_ptr<float>() : nullptr, dx.data_ptr(), dx.stride(0),
+                               (int)x.size(1), cur_stream()),
+           "vb_token_scores_bwd");
+  return dx;
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(verl_b200, m) {
+  m.def("decode_slot_map", &decode_slot_map);
+  m.def("extend_block_tables_", &extend_block_tables_);
+  m.def("build_slot_map", &build_slot_map);
+  m.def("kv4_append_", &kv4_append_);
+  m.def("kv4_gather", &kv4_gather);
+  m.def("paged_decode_kv4", &paged_decode_kv4);
+  m.def("token_scores", &token_scores);
+  m.def("token_scores_bwd", &token_scores_bwd);
+}

@@ -1,0 +1,188 @@
+// Page bookkeeping of the rollout engine on the device: block tables grown from a list of free pages, the cache slots and positions of the
+// tokens of a prefill batch, and the slots, contexts and attention plan of a decode step, all from the lengths of the requests.
+//
+// need_i = ceil(length_i / block), new_i = max(need_i - have_i, 0), and sequence i takes pool[sum of new_j over j < i ...]; token t of a packed
+// batch belongs to the sequence i with cu_i <= t < cu_{i+1} and lies at position starts_i + t - cu_i. Both are exclusive sums over the batch,
+// which every block of a launch takes for itself (a batch is at most some thousand sequences, read from L2): one launch, no block waits
+// for another. Nothing out of range is read or written whatever the tensors hold: a token whose row, position or page is none gets slot -1.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "rollout_ops.h"
+
+namespace vb {
+
+constexpr int PM_THREADS = 1024;
+
+// inclusive sum over the block; `red` holds 32 ints. Every thread also gets the block's total.
+__device__ __forceinline__ int pm_scan(int v, int* red, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  __syncthreads();
+  if (lane == 31) red[warp] = v;
+  __syncthreads();
+  int w = lane < nw ? red[lane] : 0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += u;
+  }
+  total = __shfl_sync(0xffffffffu, w, 31);
+  const int before = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
+  return v + (warp > 0 ? before : 0);
+}
+
+// One block over all slots. The plan counts the 64-token pieces of the contexts in front of every sequence: what the attention over the
+// 4-bit cache deals to its CTAs.
+__global__ void __launch_bounds__(PM_THREADS)
+decode_slot_map_kernel(const int* __restrict__ table, long long ldt, int width, const int* __restrict__ pos, const int* __restrict__ ctx,
+                       const bool* __restrict__ active, int S, int bs, long long* __restrict__ slots, int* __restrict__ ctx_out,
+                       int* __restrict__ plan) {
+  __shared__ int red[32];
+  int carry = 0;
+  if (threadIdx.x == 0) plan[0] = 0;
+  for (int base = 0; base < S; base += blockDim.x) {
+    const int s = base + threadIdx.x;
+    int n = 0;
+    if (s < S) {
+      const bool on = active[s];
+      const int p = pos[s], c = on ? max(ctx[s], 0) : 0;
+      long long slot = -1;
+      if (on && p >= 0 && p / bs < width) {
+        const int blk = table[s * ldt + p / bs];
+        if (blk >= 0) slot = static_cast<long long>(blk) * bs + p % bs;
+      }
+      slots[s] = slot;
+      ctx_out[s] = c;
+      const int seen = static_cast<int>(min(static_cast<long long>(c), static_cast<long long>(width) * bs));
+      n = seen / 64 + (seen % 64 != 0);
+    }
+    int total;
+    const int inc = pm_scan(n, red, total);
+    if (s < S) plan[s + 1] = carry + inc;
+    carry += total;
+  }
+}
+
+// A warp per row, 32 rows a block; every block sums the whole batch (for the verdict) and what stands in front of its rows.
+__global__ void __launch_bounds__(PM_THREADS)
+extend_block_tables_kernel(int* __restrict__ table, long long ldt, int S, int width, const int* __restrict__ rows, const int* __restrict__ have,
+                           const int* __restrict__ lengths, int B, const int* __restrict__ pool, int pool_size, int bs, int* __restrict__ used) {
+  __shared__ int red[32], off[32], fresh[32];
+  __shared__ int bad;
+  if (threadIdx.x == 0) bad = 0;
+  __syncthreads();
+  const int first = blockIdx.x * 32;
+  long long all = 0;
+  for (int base = 0; base < B; base += blockDim.x) {
+    const int i = base + threadIdx.x;
+    int n = 0;
+    if (i < B) {
+      const int len = max(lengths[i], 0), need = len / bs + (len % bs != 0);
+      n = max(need - have[i], 0);
+      if (rows[i] < 0 || rows[i] >= S || have[i] < 0 || have[i] > width || need > width) { bad = 1; n = 0; }
+    }
+    int total;
+    const int inc = pm_scan(n, red, total);
+    if (i >= first && i < first + 32) {   // sums fit an int where the verdict lets the rows be written: pool_size does
+      off[i - first] = static_cast<int>(all) + inc - n;
+      fresh[i - first] = n;
+    }
+    all += total;
+  }
+  __syncthreads();
+  const bool fits = !bad && all <= pool_size;
+  if (blockIdx.x == 0 && threadIdx.x == 0) used[0] = fits ? static_cast<int>(all) : -1;
+  const int w = threadIdx.x >> 5, i = first + w;
+  if (!fits || i >= B) return;
+  int* row = table + rows[i] * ldt + have[i];
+  for (int j = threadIdx.x & 31; j < fresh[w]; j += 32) row[j] = pool[off[w] + j];
+}
+
+constexpr int SM_THREADS = 256;
+constexpr int SM_TOKENS = 4;  // consecutive tokens of a thread: 16 and 32 bytes of output
+
+__global__ void __launch_bounds__(SM_THREADS)
+build_slot_map_kernel(const int* __restrict__ table, long long ldt, int S, int width, const int* __restrict__ rows, const int* __restrict__ starts,
+                      const int* __restrict__ ends, int B, int bs, int total, int* __restrict__ cu_out, int* __restrict__ positions,
+                      long long* __restrict__ slots) {
+  extern __shared__ int cu[];  // [B + 1]
+  __shared__ int red[32];
+  int carry = 0;
+  if (threadIdx.x == 0) cu[0] = 0;
+  for (int base = 0; base < B; base += blockDim.x) {
+    const int i = base + threadIdx.x;
+    const int n = i < B ? min(max(ends[i] - max(starts[i], 0), 0), total) : 0;
+    int sum;  // at most 256 x 2^22 (SM_MAX_TOTAL)
+    const int inc = pm_scan(n, red, sum);
+    if (i < B) cu[i + 1] = min(carry + inc, total);
+    carry = min(carry + sum, total);
+  }
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i <= B; i += blockDim.x) cu_out[i] = cu[i];
+  const int end = cu[B];
+  const int t0 = (blockIdx.x * SM_THREADS + threadIdx.x) * SM_TOKENS;
+  if (t0 >= total) return;
+  int lo = 0, hi = B;  // the sequence of t0: the last i with cu[i] <= t0, as far as there is one
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cu[mid] <= t0) lo = mid; else hi = mid;
+  }
+  int at[SM_TOKENS];
+  long long slot[SM_TOKENS];
+#pragma unroll
+  for (int u = 0; u < SM_TOKENS; ++u) {
+    const int t = t0 + u;
+    at[u] = 0;
+    slot[u] = -1;
+    if (t >= end) continue;
+    while (cu[lo + 1] <= t) ++lo;
+    const int p = max(starts[lo], 0) + t - cu[lo], r = rows[lo], j = p / bs;
+    at[u] = p;
+    if (p >= 0 && r >= 0 && r < S && j < width) {
+      const int blk = table[r * ldt + j];
+      if (blk >= 0) slot[u] = static_cast<long long>(blk) * bs + (p - j * bs);
+    }
+  }
+  if (t0 + SM_TOKENS <= total) {
+    *reinterpret_cast<int4*>(positions + t0) = make_int4(at[0], at[1], at[2], at[3]);
+    *reinterpret_cast<longlong2*>(slots + t0) = make_longlong2(slot[0], slot[1]);
+    *reinterpret_cast<longlong2*>(slots + t0 + 2) = make_longlong2(slot[2], slot[3]);
+  } else {
+    for (int u = 0; u < SM_TOKENS && t0 + u < total; ++u) {
+      positions[t0 + u] = at[u];
+      slots[t0 + u] = slot[u];
+    }
+  }
+}
+
+}  // namespace vb
+
+using namespace vb;
+
+extern "C" int vb_decode_slot_map(const int* table, long long ldt, int width, const int* pos, const int* ctx, const bool* active, int S, int block_size,
+                                  long long* slots, int* ctx_out, int* plan, cudaStream_t s) {
+  const int threads = S >= PM_THREADS ? PM_THREADS : max(32, (S + 31) / 32 * 32);
+  decode_slot_map_kernel<<<1, threads, 0, s>>>(table, ldt, width, pos, ctx, active, S, block_size, slots, ctx_out, plan);
+  return static_cast<int>(cudaGetLastError());
+}
+
+extern "C" int vb_extend_block_tables(int* table, long long ldt, int S, int width, const int* rows, const int* have, const int* lengths, int B,
+                                      const int* pool, int pool_size, int block_size, int* used, cudaStream_t s) {
+  extend_block_tables_kernel<<<(B + 31) / 32, PM_THREADS, 0, s>>>(table, ldt, S, width, rows, have, lengths, B, pool, pool_size, block_size, used);
+  return static_cast<int>(cudaGetLastError());
+}
+
+extern "C" int vb_build_slot_map(const int* table, long long ldt, int S, int width, const int* rows, const int* starts, const int* ends, int B,
+                                 int block_size, int total, int* cu, int* positions, long long* slots, cudaStream_t s) {
+  const int per = SM_THREADS * SM_TOKENS;
+  const int blocks = total > 0 ? (total + per - 1) / per : 1;
+  build_slot_map_kernel<<<blocks, SM_THREADS, (B + 1) * sizeof(int), s>>>(table, ldt, S, width, rows, starts, ends, B, block_size, total, cu, positions,
+                                                                         slots);
+  return static_cast<int>(cudaGetLastError());
+}

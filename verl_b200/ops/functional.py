@@ -12,7 +12,7 @@ autograd sees ``None`` for that parameter.
 from __future__ import annotations
 
 import math
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import os
 
@@ -38,6 +38,16 @@ __all__ = [
     "attention_varlen_bwd",
     "paged_decode_attention",
     "kv_append_",
+    "extend_block_tables_",
+    "build_slot_map",
+    "decode_slot_map",
+    "kv4_page_bytes",
+    "kv4_append_",
+    "kv4_gather",
+    "paged_decode_attention_kv4",
+    "TokenScores",
+    "token_scores",
+    "token_scores_bwd",
     "sample_tokens",
     "grpo_advantage",
     "gae_advantage",
@@ -684,6 +694,297 @@ def paged_decode_attention(q, k_cache, v_cache, block_table, ctx_len, scale: Opt
         s = torch.einsum("hd,thd->ht", q[b].float(), kk) * scale
         p = torch.softmax(s, -1)
         out[b] = torch.einsum("ht,thd->hd", p, vv).to(q.dtype)
+    return out
+
+
+# ----------------------------------------------------------------------------------------------- page bookkeeping
+def _check_i32(op: str, table: torch.Tensor, **vectors) -> None:
+    if table.dim() != 2 or table.dtype != torch.int32:
+        raise ValueError(f"{op}: block_table must be an int32 matrix [rows, blocks], got {table.dtype} {tuple(table.shape)}")
+    n = None
+    for name, t in vectors.items():
+        n = t.shape[0] if n is None and t.dim() == 1 else n
+        if t.dim() != 1 or t.dtype != torch.int32 or t.shape[0] != n:
+            raise ValueError(f"{op}: {name} must be an int32 vector of {n}, got {t.dtype} {tuple(t.shape)}")
+
+
+def extend_block_tables_(block_table: torch.Tensor, rows: torch.Tensor, have: torch.Tensor, lengths: torch.Tensor, pool: torch.Tensor,
+                         block_size: int) -> torch.Tensor:
+    """Grow the block tables of some sequences to their new lengths, from the front of a list of free blocks.
+
+    Sequence ``i`` (row ``rows[i]`` of ``block_table`` [R, blocks]; every row at most once) holds ``have[i]`` blocks and is to hold
+    ``ceil(lengths[i] / block_size)``; the blocks that it lacks are taken from ``pool`` in the order of the sequences. All int32. Returns
+    how many blocks of ``pool`` were taken, an int32 tensor [1]; -1 where the pool or a row is too small or a row is out of range: nothing
+    was written then."""
+    _check_i32("extend_block_tables_", block_table, rows=rows, have=have, lengths=lengths)
+    _check_i32("extend_block_tables_", block_table, pool=pool)
+    if block_table.is_cuda:
+        return _ops().extend_block_tables_(block_table, rows, have, lengths, pool, int(block_size))
+    R, width = block_table.shape
+    need = (lengths.clamp(min=0).long() + block_size - 1) // block_size
+    new = (need - have).clamp(min=0)
+    if bool(((rows < 0) | (rows >= R) | (have < 0) | (have > width) | (need > width)).any()) or int(new.sum()) > pool.numel():
+        return torch.full((1,), -1, dtype=torch.int32)
+    at = 0
+    for r, h, n in zip(rows.tolist(), have.tolist(), new.tolist()):
+        block_table[r, h : h + n] = pool[at : at + n]
+        at += n
+    return torch.tensor([at], dtype=torch.int32)
+
+
+def build_slot_map(block_table: torch.Tensor, rows: torch.Tensor, starts: torch.Tensor, ends: torch.Tensor, block_size: int, total: int):
+    """Where the tokens of a packed batch go: tokens ``starts[i] .. ends[i]`` of the sequences in rows ``rows[i]`` of ``block_table``, one
+    sequence behind the other. Returns ``(cu_seqlens int32 [n + 1], positions int32 [total], slots int64 [total])``, a slot being
+    ``block * block_size + offset``. ``total`` is the number of tokens (the sum of the lengths, known to the host); places behind the
+    last token, and tokens without a valid row or block, get slot -1."""
+    _check_i32("build_slot_map", block_table, rows=rows, starts=starts, ends=ends)
+    if total < 0:
+        raise ValueError(f"build_slot_map: total must not be negative, got {total}")
+    if block_table.is_cuda:
+        return _ops().build_slot_map(block_table, rows, starts, ends, int(block_size), int(total))
+    R, width = block_table.shape
+    a = starts.clamp(min=0).long()
+    cu = torch.cat([a.new_zeros(1), (ends - a).clamp(min=0).cumsum(0)]).clamp(max=total)
+    t = torch.arange(int(total))
+    seq = torch.searchsorted(cu[1:], t, right=True)
+    on = seq < len(rows)
+    seq = seq.clamp(max=max(len(rows) - 1, 0))
+    if not len(rows):
+        return cu.to(torch.int32), torch.zeros(int(total), dtype=torch.int32), torch.full((int(total),), -1, dtype=torch.int64)
+    p = torch.where(on, a[seq] + t - cu[seq], 0)
+    r, j = rows[seq].long(), p // block_size
+    ok = on & (r >= 0) & (r < R) & (j < width)
+    blk = block_table[r.clamp(0, max(R - 1, 0)), j.clamp(max=max(width - 1, 0))].long() if R and width else torch.full_like(p, -1)
+    slots = torch.where(ok & (blk >= 0), blk * block_size + p % block_size, -1)
+    return cu.to(torch.int32), p.to(torch.int32), slots
+
+
+def decode_slot_map(block_table: torch.Tensor, pos: torch.Tensor, ctx: torch.Tensor, active: torch.Tensor, block_size: int):
+    """A decode step's bookkeeping over all sequence slots (rows of ``block_table``): the cache slot of every active row's token at ``pos``
+    (-1: inactive, or no block there), the context lengths with those of inactive rows zeroed, and the plan of
+    :func:`paged_decode_attention_kv4`: the 64-token pieces of the contexts summed up in front of every row (int32 [S + 1]). Returns
+    ``(slots int64 [S], ctx int32 [S], plan)``. One launch."""
+    _check_i32("decode_slot_map", block_table, pos=pos, ctx=ctx)
+    S, width = block_table.shape
+    if pos.shape[0] != S or active.shape != (S,) or active.dtype != torch.bool:
+        raise ValueError(f"decode_slot_map: pos, ctx (int32) and active (bool) must have an entry for each of the {S} rows")
+    if block_table.is_cuda:
+        return _ops().decode_slot_map(block_table, pos, ctx, active, int(block_size))
+    p = pos.long()
+    ok = active & (p >= 0) & (p // block_size < width)
+    blk = block_table.gather(1, (p // block_size).clamp(0, max(width - 1, 0))[:, None])[:, 0].long() if width and S else torch.full_like(p, -1)
+    slots = torch.where(ok & (blk >= 0), blk * block_size + p % block_size, -1)
+    ctx = torch.where(active, ctx.clamp(min=0), 0)
+    return slots, ctx, _kv4_plan(ctx, width * block_size)
+
+
+def _kv4_plan(ctx: torch.Tensor, most: int) -> torch.Tensor:
+    pieces = (ctx.clamp(0, most).long() + 63) // 64
+    return torch.cat([pieces.new_zeros(1), pieces.cumsum(0)]).to(torch.int32)
+
+
+# ----------------------------------------------------------------------------------------------- 4-bit cache
+KV4_GROUP = 32   # channels of a head of a token that share a scale and a least value
+
+
+def kv4_page_bytes(block_size: int, head_dim: int) -> int:
+    """Bytes of a page of the 4-bit cache: ``block_size`` tokens of one KV head, keys and values. A pool is a uint8 tensor
+    [blocks, kv_heads, kv4_page_bytes]; a page holds the codes of the keys [block_size, head_dim / 2], those of the values, then
+    (scale, least value) in fp16 for each group of 32 channels of the keys and of the values: 0.625 bytes an element."""
+    if head_dim <= 0 or head_dim % KV4_GROUP:
+        raise ValueError(f"kv4: heads of a multiple of {KV4_GROUP} channels, got {head_dim}")
+    if block_size <= 0 or block_size % 16 or block_size > 1024:
+        raise ValueError(f"kv4: blocks of a multiple of 16 tokens, at most 1024, got {block_size}")
+    return block_size * head_dim + block_size * head_dim // 4
+
+
+def _kv4_block_size(op: str, pages: torch.Tensor, head_dim: int) -> int:
+    if pages.dtype != torch.uint8 or pages.dim() != 3 or not pages.is_contiguous():
+        raise ValueError(f"{op}: pages must be a contiguous uint8 tensor [blocks, kv_heads, page bytes], got {pages.dtype} {tuple(pages.shape)}")
+    bs = pages.shape[2] * 4 // (5 * max(head_dim, 1))
+    if bs <= 0 or kv4_page_bytes(bs, head_dim) != pages.shape[2]:
+        raise ValueError(f"{op}: pages of {pages.shape[2]} bytes hold no whole block of a head of {head_dim} channels")
+    return bs
+
+
+def _kv4_views(pages: torch.Tensor, bs: int, hd: int):
+    """Per keys and values: (codes [blocks, heads, bs, hd / 2], parameters [blocks, heads, bs, hd / 32, 2] fp16) as views of the pool."""
+    n = bs * hd // 2
+    out = []
+    for i in range(2):
+        codes = pages[..., i * n : (i + 1) * n].unflatten(-1, (bs, hd // 2))
+        params = pages[..., 2 * n + i * n // 4 : 2 * n + (i + 1) * n // 4].unflatten(-1, (bs, hd // KV4_GROUP, 4))
+        out.append((codes, params.view(torch.float16)))
+    return out
+
+
+def _kv4_dequantise(codes: torch.Tensor, params: torch.Tensor) -> torch.Tensor:
+    q = torch.stack([codes & 15, codes >> 4], -1).flatten(-2).float().unflatten(-1, (-1, KV4_GROUP))
+    return (q * params[..., :1].float() + params[..., 1:].float()).flatten(-2)
+
+
+def kv4_append_(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, pages: torch.Tensor) -> None:
+    """Quantise keys and values [T, kv_heads, head_dim] into a 4-bit pool (:func:`kv4_page_bytes`) at ``slots`` int64 [T]; negative slots
+    are skipped, and a slot may occur once. A group of 32 channels is held as ``least + code * scale``, ``code`` in 0 .. 15 between its
+    least and largest value. Values beyond the range of fp16 are held as its largest, a NaN makes its group NaN. bf16 or fp16 on a GPU."""
+    if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype or not k.is_floating_point():
+        raise ValueError(f"kv4_append_: k and v must be [tokens, heads, channels] of one floating type, got {k.dtype} {tuple(k.shape)}, "
+                         f"{v.dtype} {tuple(v.shape)}")
+    bs = _kv4_block_size("kv4_append_", pages, k.shape[2])
+    if pages.shape[1] != k.shape[1]:
+        raise ValueError(f"kv4_append_: the pool holds {pages.shape[1]} heads, k has {k.shape[1]}")
+    if slots.dtype != torch.int64 or slots.shape != (k.shape[0],):
+        raise ValueError(f"kv4_append_: slots must be int64 [{k.shape[0]}], got {slots.dtype} {tuple(slots.shape)}")
+    audit.check_index("kv4_append_", "slots", slots, pages.shape[0] * bs, skip_negative=True)
+    if k.is_cuda:
+        _ops().kv4_append_(k, v, slots, pages)
+        return
+    ok = (slots >= 0) & (slots < pages.shape[0] * bs)
+    block, off = slots[ok] // bs, slots[ok] % bs
+    for x, (codes, params) in zip((k, v), _kv4_views(pages, bs, k.shape[2])):
+        g = x[ok].float().clamp(-65504.0, 65504.0).unflatten(-1, (-1, KV4_GROUP))
+        least = g.amin(-1, keepdim=True)
+        scale = ((g.amax(-1, keepdim=True) - least) / 15.0).half()
+        least = least.half()
+        q = torch.where(scale > 0, (g - least.float()) / scale.float(), 0.0).round().clamp(0, 15).to(torch.uint8).flatten(-2)
+        codes[block, :, off] = q[..., 0::2] | (q[..., 1::2] << 4)
+        params[block, :, off] = torch.cat([scale, least], -1)
+
+
+def kv4_gather(pages: torch.Tensor, slots: torch.Tensor, head_dim: int, dtype: torch.dtype = torch.bfloat16):
+    """Keys and values [T, kv_heads, head_dim] of the tokens at ``slots`` int64 [T] of a 4-bit pool, rounded once to ``dtype`` (bf16 or fp16
+    on a GPU); zeros for negative slots."""
+    bs = _kv4_block_size("kv4_gather", pages, head_dim)
+    if slots.dtype != torch.int64 or slots.dim() != 1:
+        raise ValueError(f"kv4_gather: slots must be an int64 vector, got {slots.dtype} {tuple(slots.shape)}")
+    audit.check_index("kv4_gather", "slots", slots, pages.shape[0] * bs, skip_negative=True)
+    if pages.is_cuda:
+        return _ops().kv4_gather(pages, slots, int(head_dim), dtype)
+    ok = (slots >= 0) & (slots < pages.shape[0] * bs)
+    block, off = slots[ok] // bs, slots[ok] % bs
+    out = []
+    for codes, params in _kv4_views(pages, bs, head_dim):
+        x = torch.zeros(len(slots), pages.shape[1], head_dim, dtype=dtype)
+        x[ok] = _kv4_dequantise(codes[block, :, off], params[block, :, off]).to(dtype)
+        out.append(x)
+    return tuple(out)
+
+
+def paged_decode_attention_kv4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, ctx_len: torch.Tensor,
+                               scale: Optional[float] = None, plan: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One query token per sequence, ``q`` [B, heads, head_dim], against the first ``ctx_len[b]`` tokens of its row of ``block_table`` [B, blocks]
+    in a 4-bit pool: as :func:`paged_decode_attention` over the values that the pool holds; zeros for a context of zero tokens. On a GPU: bf16
+    or fp16, heads of 64 or 128 channels, blocks of 16 to 256 tokens (a power of two), at most 16 query heads to a KV head.
+
+    ``plan`` (third result of :func:`decode_slot_map` for the same contexts) saves a launch when it is made once for all layers of a step."""
+    if q.dim() != 3 or not q.is_floating_point():
+        raise ValueError(f"paged_decode_attention_kv4: q must be [sequences, heads, channels], got {q.dtype} {tuple(q.shape)}")
+    B, nh, hd = q.shape
+    bs, nkv = _kv4_block_size("paged_decode_attention_kv4", pages, hd), pages.shape[1]
+    _check_i32("paged_decode_attention_kv4", block_table, ctx_len=ctx_len)
+    if block_table.shape[0] != B or ctx_len.shape[0] != B or nkv == 0 or nh % nkv:
+        raise ValueError(f"paged_decode_attention_kv4: {B} sequences of {nh} heads against tables of {block_table.shape[0]} rows, "
+                         f"{ctx_len.shape[0]} contexts and {nkv} KV heads")
+    if plan is not None and (plan.dtype != torch.int32 or plan.shape != (B + 1,)):
+        raise ValueError(f"paged_decode_attention_kv4: plan must be int32 [{B + 1}], got {plan.dtype} {tuple(plan.shape)}")
+    scale = scale if scale is not None else 1.0 / math.sqrt(hd)
+    audit.check_paged_cache("paged_decode_attention_kv4", block_table, ctx_len, pages.shape[0], bs)
+    if q.is_cuda:
+        return _ops().paged_decode_kv4(q, pages, block_table, ctx_len, plan, float(scale))
+    out = torch.zeros_like(q)
+    (kc, kp), (vc, vp) = _kv4_views(pages, bs, hd)
+    for b in range(B):
+        n = min(int(ctx_len[b]), block_table.shape[1] * bs)
+        if n <= 0:
+            continue
+        blk = block_table[b, : -(-n // bs)].long()
+        rows = lambda codes, params: _kv4_dequantise(codes[blk], params[blk]).transpose(0, 1).flatten(1, 2)[:, :n]   # [nkv, n, hd]
+        kk, vv = rows(kc, kp), rows(vc, vp)
+        s = torch.einsum("ghd,gtd->ght", q[b].float().view(nkv, nh // nkv, hd), kk) * scale
+        out[b] = torch.einsum("ght,gtd->ghd", torch.softmax(s, -1), vv).reshape(nh, hd).to(q.dtype)
+    return out
+
+
+# ----------------------------------------------------------------------------------------------- scores of logits
+class TokenScores(NamedTuple):
+    logprob: torch.Tensor      # of the given tokens, fp32, the shape of ids
+    entropy: torch.Tensor      # fp32 [T]
+    lse: torch.Tensor          # log-sum-exp of the scaled logits, fp32 [T]
+    top_ids: torch.Tensor      # most likely tokens, int64 [T, top_k], equal ones by their number
+    top_logprob: torch.Tensor  # fp32 [T, top_k]
+
+
+TOP_K_LIMIT = 128
+
+
+def _scores_args(op: str, logits: torch.Tensor, ids: torch.Tensor, temperature: float, valid_vocab: int) -> int:
+    if logits.dim() != 2 or logits.shape[1] == 0 or not logits.is_floating_point():
+        raise ValueError(f"{op}: logits must be [rows, vocabulary], got {logits.dtype} {tuple(logits.shape)}")
+    if ids.dim() not in (1, 2) or ids.shape[0] != logits.shape[0] or ids.dtype != torch.int64:
+        raise ValueError(f"{op}: ids must be int64 [{logits.shape[0]}] or [{logits.shape[0]}, n], got {ids.dtype} {tuple(ids.shape)}")
+    if ids.dim() == 2 and ids.shape[1] > 4096:
+        raise ValueError(f"{op}: at most 4096 given tokens a row, got {ids.shape[1]}")
+    if not temperature > 0:
+        raise ValueError(f"{op}: temperature must be positive, got {temperature}")
+    if valid_vocab < 0 or valid_vocab > logits.shape[1]:
+        raise ValueError(f"{op}: valid_vocab must lie in 0 .. {logits.shape[1]}, got {valid_vocab}")
+    return valid_vocab or logits.shape[1]
+
+
+def token_scores(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0, temperature: float = 1.0, valid_vocab: int = 0) -> TokenScores:
+    """Log-probs of given tokens, entropy and the most likely tokens of ``softmax(logits / temperature)`` for rows of logits [T, V] (bf16, fp16 or
+    fp32), in one pass over them. ``ids`` [T] or [T, n]; an id outside the vocabulary (padding) has log-prob 0. The first ``valid_vocab``
+    columns count (0: all). ``top_k`` at most 128.
+
+    A logit of -inf has probability 0; a row that has nothing else scores -inf, with entropy 0. A NaN or +inf makes its row's scores NaN;
+    among the most likely tokens a NaN counts as the largest value."""
+    V = _scores_args("token_scores", logits, ids, temperature, valid_vocab)
+    if not 0 <= top_k <= min(TOP_K_LIMIT, V):
+        raise ValueError(f"token_scores: top_k must lie in 0 .. {min(TOP_K_LIMIT, V)}, got {top_k}")
+    flat = ids if ids.dim() == 2 else ids[:, None]
+    if logits.is_cuda:
+        x = logits if logits.stride(1) == 1 else logits.contiguous()
+        out = _ops().token_scores(x, flat.contiguous(), int(top_k), float(temperature), V)
+        return TokenScores(out[0].view(ids.shape), *out[1:])
+    x = logits[:, :V].float()
+    z = x * (1.0 / float(temperature))
+    m = z.amax(-1, keepdim=True)
+    empty = m == float("-inf")
+    e = torch.exp(z - torch.where(empty, 0.0, m))
+    s = e.sum(-1, keepdim=True)
+    lse = m + torch.log(s)
+    ent = torch.where(empty, 0.0, torch.log(s) - torch.where(e == 0, 0.0, e * (z - m)).sum(-1, keepdim=True) / s)
+    score = lambda at: torch.where(empty, float("-inf"), z.gather(1, at) - lse)
+    ok = (flat >= 0) & (flat < V)
+    lp = torch.where(ok, score(flat.clamp(0, V - 1)), 0.0)
+    top = torch.sort(x, dim=-1, descending=True, stable=True).indices[:, : int(top_k)]
+    return TokenScores(lp.view(ids.shape), ent[:, 0], lse[:, 0], top, score(top))
+
+
+def token_scores_bwd(logits: torch.Tensor, ids: torch.Tensor, lse: torch.Tensor, entropy: torch.Tensor, g_logprob: torch.Tensor,
+                     g_entropy: Optional[torch.Tensor], temperature: float = 1.0, valid_vocab: int = 0) -> torch.Tensor:
+    """Gradient of the logits, in their type, from those of ``logprob`` and ``entropy`` (None: none) of :func:`token_scores`. A token that is given
+    several times gathers all its gradients; ids outside the vocabulary and columns behind ``valid_vocab`` have none."""
+    V = _scores_args("token_scores_bwd", logits, ids, temperature, valid_vocab)
+    T = logits.shape[0]
+    if g_logprob.shape != ids.shape or (g_entropy is not None and g_entropy.shape != (T,)) or lse.shape != (T,) or entropy.shape != (T,):
+        raise ValueError("token_scores_bwd: g_logprob has the shape of ids; lse, entropy and g_entropy have an entry for each row")
+    flat, g = (t if t.dim() == 2 else t[:, None] for t in (ids, g_logprob.float()))
+    if logits.is_cuda:
+        x = logits if logits.stride(1) == 1 else logits.contiguous()
+        return _ops().token_scores_bwd(x, flat.contiguous(), lse.contiguous(), entropy.contiguous(), g.contiguous(),
+                                       g_entropy.float().contiguous() if g_entropy is not None else None, float(temperature), V)
+    inv = 1.0 / float(temperature)
+    logp = logits[:, :V].float() * inv - lse[:, None]
+    p = torch.exp(logp)
+    g = torch.where((flat >= 0) & (flat < V), g, 0.0)
+    slope = g.sum(-1, keepdim=True)
+    if g_entropy is not None:
+        slope = slope + g_entropy.float()[:, None] * (logp + entropy[:, None])
+    d = torch.where(p == 0, 0.0, -p * slope)
+    d.scatter_add_(1, flat.clamp(0, V - 1), g)
+    out = torch.zeros_like(logits, memory_format=torch.contiguous_format)
+    out[:, :V] = torch.where(lse[:, None] == float("-inf"), 0.0, d * inv).to(logits.dtype)
     return out
 
 
