@@ -309,7 +309,8 @@ def test_blocks_that_do_not_exist_are_skipped(dev):
         if dev == "cuda":
             out = F.paged_decode_attention_kv4(q, pages, t, ctx)
             assert torch.equal(out[1], good[1])
-            assert torch.equal(out[0], F.paged_decode_attention_kv4(q, pages, table, i32([192, 64], dev))[0])
+            want, off = attention_64(q, pages, table, [192, 64], 64, 0.125)
+            assert (np.abs(out.double().cpu().numpy() - want) <= off + 2.0**-8 * np.abs(want) + 2.0**-24).all()
     with audit.scope(), pytest.raises(audit.AuditError):
         F.paged_decode_attention_kv4(q, pages, table, i32([257, 64], dev))
 
