@@ -118,7 +118,7 @@ def test_refusals_of_the_bookkeeping(dev):
 def quantised(x):
     """Codes and parameters of x [..., channels] (numpy fp32), every step one rounded fp32 operation."""
     with np.errstate(invalid="ignore", divide="ignore"):
-        g = np.clip(x.astype(np.float32), -65504, 65504).reshape(*x.shape[:-1], -1, 32)
+        g = np.clip(x.astype(np.float32), -7600, 7600).reshape(*x.shape[:-1], -1, 32)
         low = g.min(-1, keepdims=True)
         scale = ((g.max(-1, keepdims=True) - low) / np.float32(15)).astype(np.float16)
         low = low.astype(np.float16)
@@ -188,7 +188,7 @@ def test_values_outside_the_range_of_the_cache(dev):
     F.kv4_append_(x, x, slots, pages)
     k, v = (t.float().cpu() for t in F.kv4_gather(pages, slots, 64))
     assert torch.equal(k.isnan(), v.isnan()) and k[0, 0, :32].isnan().all() and (k[0, 0, 32:] == 0).all() and not k[1:].isnan().any()
-    top = float(torch.tensor(65504.0).bfloat16())
+    top = float(torch.tensor(7600.0).bfloat16())
     assert k[1, 0, 40] == pytest.approx(top, rel=2.0**-7) and k[2, 0, 0] == -top and k[3].abs().max() <= 2e-6
 
 
@@ -237,7 +237,8 @@ def make_pool(rs, lens, nkv, hd, bs, width, dev):
 def attention_64(q, pages, table, lens, bs, scale):
     """(output, largest |output| that the roundings of the kernel may change each value by), in 64 bits."""
     B, nh, hd = q.shape
-    k, v = rows_of(pages, bs, hd)
+    (codes, step, _), (k, v) = unpacked(pages, bs, hd), rows_of(pages, bs, hd)
+    part = (codes.astype(np.float64) * step.astype(np.float64)).reshape(*codes.shape[:-2], hd)     # what a code adds to its group's least value
     nkv = k.shape[1]
     q = q.double().cpu().numpy().reshape(B, nkv, nh // nkv, hd)
     out, off = np.zeros((B, nkv, nh // nkv, hd)), np.zeros((B, nkv, nh // nkv, hd))
@@ -245,16 +246,22 @@ def attention_64(q, pages, table, lens, bs, scale):
         if n == 0:
             continue
         blk = table[b, : -(-n // bs)].cpu().numpy()
-        kk, vv = (x[blk].transpose(1, 0, 2, 3).reshape(nkv, -1, hd)[:, :n] for x in (k, v))
+        kk, vv, kp, vp = (x[blk].transpose(1, 0, 2, 3).reshape(nkv, -1, hd)[:, :n] for x in (k, v, part[0], part[1]))
         s = np.einsum("hgd,htd->hgt", q[b], kk) * scale
         w = np.exp(s - s.max(-1, keepdims=True))
         w /= w.sum(-1, keepdims=True)
         out[b] = np.einsum("hgt,htd->hgd", w, vv)
-        # keys and values are rounded to fp16 (U16 of each), sums of products to fp32 (their length times U32): a score is off by at most
-        # ds, a weight by 2 ds and the rounding of e^s to fp16 (U16, and 2^-25 of the largest where it is small)
-        ds = ((U16 + (hd + 8) * U32) * scale * np.einsum("hgd,htd->hgt", np.abs(q[b]), np.abs(kk))).max(-1, keepdims=True)
-        size = np.einsum("hgt,htd->hgd", w, np.abs(vv))
-        off[b] = (2 * ds + 3 * U16 + (n + 64) * U32) * size + 2.0**-24 * n * w.max(-1, keepdims=True) * np.abs(vv).max(1)[:, None]
+        # The kernel rounds code * scale to fp16 (U16 of it, or half of 16 times the least fp16 number: 2^-21) and nothing else of a key or value:
+        # the least values are fp16 already, their factor is held in two halves (2^-22). Sums of products are fp32 (their length times U32). A
+        # score is off by at most ds, a weight by 2 ds and by the rounding of e^s to fp16 (U16, and 2^-25 of the largest where it is small),
+        # which acts on the whole value.
+        size_q = np.abs(q[b]).sum(-1, keepdims=True)
+        ds = scale * (U16 * np.einsum("hgd,htd->hgt", np.abs(q[b]), np.abs(kp)) + (2.0**-21 * size_q)
+                      + (2.0**-22 + (hd + 8) * U32) * np.einsum("hgd,htd->hgt", np.abs(q[b]), np.abs(kk) + 2 * np.abs(kp)))
+        ds = ds.max(-1, keepdims=True)
+        size, codes_size = (np.einsum("hgt,htd->hgd", w, np.abs(x)) for x in (vv, vp))
+        off[b] = ((2 * ds + 2 * U16) * size + U16 * codes_size + 2.0**-21 + (n + 64) * U32 * (size + 2 * codes_size)
+                  + 2.0**-24 * n * w.max(-1, keepdims=True) * np.abs(vv).max(1)[:, None])
     return out.reshape(B, nh, hd), off.reshape(B, nh, hd)
 
 

@@ -2,8 +2,9 @@
 //
 // A group of 32 channels of one head of one token is quantised between its least and its largest value:
 //   least = f16(min), scale = f16((max - min) / 15), q = clamp(rint((x - least) / scale), 0, 15), 0 where the scale is 0.
-// Every step is one correctly rounded fp32 operation, so that the codes are those of the same formula anywhere. Values beyond fp16's range
-// are taken as its largest; a NaN makes the parameters of its group NaN, so that what is read back is NaN, as from a 16-bit cache.
+// Every step is one correctly rounded fp32 operation, so that the codes are those of the same formula anywhere. Values beyond
+// +- 7600 are taken as that: scales stay below 1024, on which the attention counts. A NaN makes the parameters of its group NaN, so that what
+// is read back is NaN, as from a 16-bit cache.
 //
 // Both kernels move bytes: 8 channels a thread (16 bytes of input, 4 of codes), four threads a group, the group's extremes by two shuffles.
 #include "kv4_common.cuh"
@@ -48,10 +49,10 @@ kv4_append_kernel(const T2* __restrict__ k, const T2* __restrict__ v, long long 
     x[2 * j] = f.x;
     x[2 * j + 1] = f.y;
   }
-  float lo = 65504.f, hi = -65504.f;
+  float lo = KV4_LIMIT, hi = -KV4_LIMIT;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    x[j] = min_nan(max_nan(x[j], -65504.f), 65504.f);
+    x[j] = min_nan(max_nan(x[j], -KV4_LIMIT), KV4_LIMIT);
     lo = min_nan(lo, x[j]);
     hi = max_nan(hi, x[j]);
   }

@@ -14,6 +14,7 @@
 namespace vb {
 
 constexpr int KV4_GROUP = 32;
+constexpr float KV4_LIMIT = 7600.f;  // largest magnitude that is kept: scales are at most 15200 / 15
 
 __host__ __device__ constexpr long long kv4_page_bytes(int block, int hd) { return static_cast<long long>(block) * hd + block * hd / 4; }
 __host__ __device__ constexpr int kv4_codes_at(int block, int hd, int value) { return value ? block * hd / 2 : 0; }

@@ -784,7 +784,8 @@ def _kv4_plan(ctx: torch.Tensor, most: int) -> torch.Tensor:
 
 
 # ----------------------------------------------------------------------------------------------- 4-bit cache
-KV4_GROUP = 32   # channels of a head of a token that share a scale and a least value
+KV4_GROUP = 32        # channels of a head of a token that share a scale and a least value
+KV4_LIMIT = 7600.0    # largest magnitude that is kept
 
 
 def kv4_page_bytes(block_size: int, head_dim: int) -> int:
@@ -826,7 +827,7 @@ def _kv4_dequantise(codes: torch.Tensor, params: torch.Tensor) -> torch.Tensor:
 def kv4_append_(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, pages: torch.Tensor) -> None:
     """Quantise keys and values [T, kv_heads, head_dim] into a 4-bit pool (:func:`kv4_page_bytes`) at ``slots`` int64 [T]; negative slots
     are skipped, and a slot may occur once. A group of 32 channels is held as ``least + code * scale``, ``code`` in 0 .. 15 between its
-    least and largest value. Values beyond the range of fp16 are held as its largest, a NaN makes its group NaN. bf16 or fp16 on a GPU."""
+    least and largest value. Values beyond +-7600 are held as that, a NaN makes its group NaN. bf16 or fp16 on a GPU."""
     if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype or not k.is_floating_point():
         raise ValueError(f"kv4_append_: k and v must be [tokens, heads, channels] of one floating type, got {k.dtype} {tuple(k.shape)}, "
                          f"{v.dtype} {tuple(v.shape)}")
@@ -842,7 +843,7 @@ def kv4_append_(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, pages: to
     ok = (slots >= 0) & (slots < pages.shape[0] * bs)
     block, off = slots[ok] // bs, slots[ok] % bs
     for x, (codes, params) in zip((k, v), _kv4_views(pages, bs, k.shape[2])):
-        g = x[ok].float().clamp(-65504.0, 65504.0).unflatten(-1, (-1, KV4_GROUP))
+        g = x[ok].float().clamp(-KV4_LIMIT, KV4_LIMIT).unflatten(-1, (-1, KV4_GROUP))
         least = g.amin(-1, keepdim=True)
         scale = ((g.amax(-1, keepdim=True) - least) / 15.0).half()
         least = least.half()
