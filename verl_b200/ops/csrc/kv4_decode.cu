@@ -5,10 +5,11 @@
 // (sequence, head) leaves its sums in a slot of its own, and a second small launch, started early by programmatic dependence, joins them
 // by their maxima, in the order of the runs: no atomics, the same bits every time.
 //
-// A CTA: one warp brings pieces into a ring of shared memory by bulk copies (a piece is at most 16 contiguous runs; four for blocks of 64 and
-// more); four warps take one piece after the other, each by itself, and meet at the end of a segment.
-//   S^T[64 tokens, 8 heads] = K[64, hd] Q^T        keys are the A operand of m16n8k16: a thread's share of a token's row is one contiguous run
-//   O^T[hd, 8 heads]       += V^T[hd, 64] P^T      values are the A operand as well; P^T is S^T's accumulator through movmatrix
+// A CTA: its four warps take chunks of 32 tokens in turn, each with two stages of shared memory of its own that it fills by bulk copies (a chunk is
+// at most 8 contiguous runs; four for blocks of 32 and more) while it works on the other: no warp waits for another until the end of a segment,
+// where their sums meet in pairs, fragment by fragment.
+//   S^T[32 tokens, 8 heads] = K[32, hd] Q^T        keys are the A operand of m16n8k16: a thread's share of a token's row is one contiguous run
+//   O^T[hd, 8 heads]       += V^T[hd, 32] P^T      values are the A operand as well; P^T is S^T's accumulator through movmatrix
 // so that with up to 8 heads to a KV head a matrix instruction takes 256 cache elements (query heads as the 16 rows would take 128).
 //
 // A code becomes a number without a conversion: (w & 0x000f000f) | 0x5400.. is 64 + q / 16 in fp16 and (w & 0x00f000f0) | 0x4400.. is 4 + q / 16, so
@@ -27,11 +28,14 @@ namespace vb {
 
 int num_sms();
 
-constexpr int KD_PIECE = 64;
-constexpr int KD_WARPS = 4;                      // warps that compute
-constexpr int KD_THREADS = (KD_WARPS + 1) * 32;
-constexpr int KD_STAGES = 2 * KD_WARPS;           // a stage belongs to one warp: its barrier's phases are then met one by one
-constexpr int KD_CTAS = 2;                       // CTAs of an SM
+constexpr int KD_PIECE = 64;                     // tokens that the plan counts in
+constexpr int KD_CHUNK = 32;                     // tokens of a stage
+constexpr int KD_PER_PIECE = KD_PIECE / KD_CHUNK;
+constexpr int KD_WARPS = 4;
+constexpr int KD_THREADS = KD_WARPS * 32;
+constexpr int KD_STAGES = 2;                     // of a warp
+constexpr int KD_TILES = KD_CHUNK / 16;
+__host__ __device__ constexpr int kd_ctas(int nt) { return nt == 1 ? 4 : 3; }  // CTAs of an SM: what registers and shared memory hold
 constexpr int KD_MIN_PIECES = 4;                 // shortest run of a CTA
 
 __device__ int g_kv4_status[4];
@@ -46,6 +50,11 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16_16816_from_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t movmatrix_t(uint32_t a) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
@@ -56,39 +65,62 @@ __device__ __forceinline__ float fast_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t h2_bits(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
-__device__ __forceinline__ __half2 h2_of(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
+// fp16 pairs as the 32 bits that they are
+__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
 // Factors of a pair of codes: their scales, and what 64 and 4 become under them.
 struct Scales {
-  __half2 s, n64, n4;
-  __device__ __forceinline__ explicit Scales(__half2 v) : s(v), n64(__hmul2(v, __float2half2_rn(-64.f))), n4(__hmul2(v, __float2half2_rn(-4.f))) {}
+  uint32_t s, n64, n4;
+  __device__ __forceinline__ explicit Scales(uint32_t v) : s(v), n64(mul2(v, 0xd400d400u)), n4(mul2(v, 0xc400c400u)) {}
+};
+// The exponents that codes are put under. An instruction takes one constant: these stay in registers, where the compiler would otherwise make
+// them again for each of the 256 uses in a piece.
+struct Magic {
+  uint32_t even, odd;
+  __device__ __forceinline__ Magic() {
+    asm volatile("mov.b32 %0, 0x54005400;" : "=r"(even));
+    asm volatile("mov.b32 %0, 0x44004400;" : "=r"(odd));
+  }
 };
 // q s / 16 for pairs 0 / 1 of the four that a word of codes holds: its nibbles (0, 4) and (1, 5); the other two after a shift by 8
-__device__ __forceinline__ uint32_t codes_even(uint32_t w, const Scales& f) {
+__device__ __forceinline__ uint32_t codes_even(uint32_t w, const Scales& f, const Magic& k) {
   uint32_t x;
-  asm("lop3.b32 %0, %1, 0x000f000f, 0x54005400, 0xea;" : "=r"(x) : "r"(w));
-  return h2_bits(__hfma2(h2_of(x), f.s, f.n64));
+  asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xea;" : "=r"(x) : "r"(w), "r"(k.even));
+  return fma2(x, f.s, f.n64);
 }
-__device__ __forceinline__ uint32_t codes_odd(uint32_t w, const Scales& f) {
+__device__ __forceinline__ uint32_t codes_odd(uint32_t w, const Scales& f, const Magic& k) {
   uint32_t x;
-  asm("lop3.b32 %0, %1, 0x00f000f0, 0x44004400, 0xea;" : "=r"(x) : "r"(w));
-  return h2_bits(__hfma2(h2_of(x), f.s, f.n4));
+  asm("lop3.b32 %0, %1, 0x00f000f0, %2, 0xea;" : "=r"(x) : "r"(w), "r"(k.odd));
+  return fma2(x, f.s, f.n4);
 }
 
 template <int HD, int NT>
 struct KDSmem {
-  static constexpr int CODES = KD_PIECE * HD / 2;             // of keys, or of values
-  static constexpr int PARAMS = KD_PIECE * (HD / KV4_GROUP) * 4;
+  static constexpr int CODES = KD_CHUNK * HD / 2;             // of keys, or of values
+  static constexpr int PARAMS = KD_CHUNK * (HD / KV4_GROUP) * 4;
   static constexpr int OFF_PK = 2 * CODES;
   static constexpr int STAGE = 2 * CODES + 2 * PARAMS;        // a multiple of 128 bytes
-  static constexpr int MROW = HD + 4;                         // a head's sums and (maximum, sum of weights)
-  static constexpr int OFF_MERGE = KD_STAGES * STAGE;
-  static constexpr int OFF_BAR = OFF_MERGE + KD_WARPS * 8 * MROW * 4;
-  static constexpr int TOTAL = OFF_BAR + KD_STAGES * (8 + 8 + 4) + 128;
+  static constexpr int MEET = HD / 4 + 4;                     // floats of a lane: O of 8 heads, maxima and sums of weights of two
+  static constexpr int OFF_MEET = KD_WARPS * KD_STAGES * STAGE;
+  static constexpr int OFF_BAR = OFF_MEET + 2 * 32 * MEET * 4;
+  static constexpr int TOTAL = OFF_BAR + KD_WARPS * KD_STAGES * 8;
 };
 
 // The sequence that piece u (over all heads) belongs to: the last one with plan[b] * nkv <= u. The whole warp searches, 32 places a round.
-__device__ __forceinline__ int kd_locate(const int* plan, int B, int nkv, long long u) {
+__device__ __forceinline__ int kd_locate(const int* plan, int B, int nkv, int u) {
   const int lane = threadIdx.x & 31;
   int lo = 0, n = B;
   while (n > 1) {
@@ -102,119 +134,106 @@ __device__ __forceinline__ int kd_locate(const int* plan, int B, int nkv, long l
   return lo;
 }
 
-struct KDRun {
-  long long first, end;  // this CTA's pieces
-};
-__device__ __forceinline__ long long kd_total(const VbKv4Decode& p) {
-  const long long most = static_cast<long long>(p.B) * ((static_cast<long long>(p.width) * p.block_size + KD_PIECE - 1) / KD_PIECE);
-  return min(max(static_cast<long long>(p.plan[p.B]), 0LL), most) * p.nkv;
+// Pieces of everything and of a CTA's run. The launcher sees that chunks, and tokens of a table row, are counted in 31 bits.
+__device__ __forceinline__ int kd_total(const VbKv4Decode& p) {
+  return min(max(p.plan[p.B], 0), p.B * ((p.width * p.block_size + KD_PIECE - 1) / KD_PIECE)) * p.nkv;
 }
-__device__ __forceinline__ long long kd_per(long long total, int ctas) { return max(static_cast<long long>(KD_MIN_PIECES), (total + ctas - 1) / ctas); }
-__device__ __forceinline__ long long kd_len(const VbKv4Decode& p, int b) {
-  return min(static_cast<long long>(max(p.ctx[b], 0)), static_cast<long long>(p.width) * p.block_size);
-}
+__device__ __forceinline__ int kd_per(int total, int ctas) { return max(KD_MIN_PIECES, (total + ctas - 1) / ctas); }
+__device__ __forceinline__ int kd_len(const VbKv4Decode& p, int b) { return min(max(p.ctx[b], 0), p.width * p.block_size); }
 
-// One (sequence, head) of a run.
+// One (sequence, head), in chunks: two to a piece, the second one of a context's last piece may be empty.
 struct KDSegment {
-  int b, kvh;
-  long long base, n;  // its first piece and how many it has, in the numbering over everything
-  __device__ __forceinline__ void find(const VbKv4Decode& p, int b_, long long u) {
-    b = b_;
-    while (b + 1 < p.B && static_cast<long long>(p.plan[b + 1]) * p.nkv <= u) ++b;
-    const long long at = static_cast<long long>(p.plan[b]) * p.nkv;
-    n = max(static_cast<long long>(p.plan[b + 1]) - p.plan[b], 1LL);
-    kvh = static_cast<int>(min(max((u - at) / n, 0LL), static_cast<long long>(p.nkv - 1)));
+  int b, kvh, base, end, len;  // its chunks in the numbering over everything, its tokens
+  __device__ __forceinline__ void find(const VbKv4Decode& p, int u) {
+    const int f = p.nkv * KD_PER_PIECE;
+    while (b + 1 < p.B && p.plan[b + 1] * f <= u) ++b;
+    const int at = p.plan[b] * f, n = max(p.plan[b + 1] - p.plan[b], 1) * KD_PER_PIECE;
+    kvh = min(max(u - at, 0) / n, p.nkv - 1);
     base = at + kvh * n;
+    end = max(base + n, u + 1);
+    len = kd_len(p, b);
   }
 };
+
+__device__ __forceinline__ bool kd_wait(uint64_t* bar, uint32_t parity) {  // as mbar_wait, asleep up to 2 us at a time
+  const uint64_t t0 = global_timer_ns();
+  for (;;) {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 2000;\nselp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    if (ok) return true;
+    if (global_timer_ns() - t0 > VB_WAIT_LIMIT_NS) return false;
+  }
+}
 
 template <int HD, int NT, typename T>
-__global__ void __launch_bounds__(KD_THREADS, KD_CTAS)
-kv4_decode_kernel(const VbKv4Decode p, int* status) {
+__global__ void __launch_bounds__(KD_THREADS, kd_ctas(NT))
+kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
   using L = KDSmem<HD, NT>;
-  constexpr int STEP = NT == 1 ? 4 : 2;  // 16-token tiles between two looks at the maximum: what the registers hold
   constexpr int CPR = HD / 4, VPR = HD / 8, KW = CPR / 8, VW = VPR / 8;  // channels of a thread's run, and words of them
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
-  uint64_t* empty = full + KD_STAGES;
-  uint32_t* absent = reinterpret_cast<uint32_t*>(empty + KD_STAGES);  // per stage: the pages of its piece that do not exist
+  extern __shared__ __align__(16) uint8_t smem[];  // 16 bytes are what bulk copies ask for
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.nh / p.nkv, bs = p.block_size;
+  uint8_t* ring = smem + warp * KD_STAGES * L::STAGE;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR) + warp * KD_STAGES;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const long long total = kd_total(p), per = kd_per(total, gridDim.x);
-  const long long u0 = blockIdx.x * per, u1 = min(total, u0 + per);
-  if (u0 >= u1) return;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < KD_STAGES; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-    }
+  const int total = kd_total(p), per = kd_per(total, gridDim.x);
+  if (static_cast<long long>(blockIdx.x) * per >= total) return;
+  const int u0 = blockIdx.x * per * KD_PER_PIECE, u1 = min(total, static_cast<int>(blockIdx.x + 1) * per) * KD_PER_PIECE;  // this CTA's chunks
+  if (lane == 0) {
+    for (int s = 0; s < KD_STAGES; ++s) mbar_init(&full[s], 1);
     mbar_fence_init();
   }
-  __syncthreads();
+  __syncwarp();
 
-  if (warp == KD_WARPS) {
-    // ---- the warp that loads: 4 lanes per page of a piece (keys' codes, values' codes, keys' parameters, values' parameters)
-    const int pages = bs < KD_PIECE ? KD_PIECE / bs : 1, lanes = 4 * pages, batch = 32 / lanes;
-    const int page = (lane % lanes) >> 2, what = lane & 3, tokens = min(bs, KD_PIECE);
-    const uint32_t bytes = what < 2 ? tokens * HD / 2 : tokens * (HD / KV4_GROUP) * 4;
-    const int dst_off = (what < 2 ? what * L::CODES : L::OFF_PK + (what - 2) * L::PARAMS) + page * bytes;
-    const int src_off = what < 2 ? kv4_codes_at(bs, HD, what) : kv4_params_at(bs, HD, what - 2);
-    KDSegment g;
-    g.b = kd_locate(p.plan, p.B, p.nkv, u0);
-    bool ok = true;
-    long long done = 0;
-    for (long long u = u0; u < u1 && ok; u += batch) {
-      const long long mine = min(u + lane / lanes, u1 - 1);
-      g.find(p, g.b, mine);
-      const long long piece = max(mine - g.base, 0LL);
-      const long long tok = piece * KD_PIECE + page * bs;  // first token of this lane's page (of its 64, for larger blocks)
-      const bool inside = tok < kd_len(p, g.b);            // pages behind the context are not looked up
-      int blk = -1;
-      if (inside) blk = p.table[g.b * p.ldt + tok / bs];
-      const bool there = blk >= 0 && blk < p.num_blocks;
-      const uint8_t* src = p.pages + (static_cast<long long>(max(blk, 0)) * p.nkv + g.kvh) * kv4_page_bytes(bs, HD) + src_off +
-                           static_cast<int>(tok % bs) * (what < 2 ? HD / 2 : (HD / KV4_GROUP) * 4);
-      const uint32_t copies = __ballot_sync(0xffffffffu, there && what == 0), lost = __ballot_sync(0xffffffffu, inside && !there && what == 0);
-      for (int i = 0; i < batch && u + i < u1; ++i) {
-        const long long k = u + i - u0;
-        const int s = static_cast<int>(k % KD_STAGES);
-        if (k >= KD_STAGES) ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], static_cast<uint32_t>((k / KD_STAGES - 1) & 1)));
-        if (!ok) break;
-        uint8_t* stage = smem + s * L::STAGE;
-        if (lane == i * lanes) {
-          const uint32_t group = lanes == 32 ? 0xffffffffu : ((1u << lanes) - 1) << lane;
-          uint32_t gone = 0;
-          for (int j = 0; j < pages; ++j) gone |= ((lost >> (lane + 4 * j)) & 1u) << j;
-          absent[s] = gone;
-          mbar_expect_tx(&full[s], __popc(copies & group) * tokens * (HD + HD / 4));
-        }
-        __syncwarp();
-        if (lane / lanes == i && there) bulk_load(stage + dst_off, src, bytes, &full[s]);
-        done = k + 1;
-      }
-      g.b = __shfl_sync(0xffffffffu, g.b, min(batch, static_cast<int>(min(u1 - u, 32LL))) * lanes - 1);
+  // ---- loading: 4 lanes per page of a chunk (keys' codes, values' codes, keys' parameters, values' parameters)
+  const int tokens = min(bs, KD_CHUNK), pages = KD_CHUNK / tokens, page = lane >> 2, what = lane & 3;
+  const uint32_t row = what < 2 ? HD / 2 : (HD / KV4_GROUP) * 4, bytes = tokens * row;
+  const int dst_off = (what < 2 ? what * L::CODES : L::OFF_PK + (what - 2) * L::PARAMS) + page * bytes;
+  const int src_off = what < 2 ? kv4_codes_at(bs, HD, what) : kv4_params_at(bs, HD, what - 2);
+  KDSegment ahead;  // of the chunk that is looked up
+  ahead.b = kd_locate(p.plan, p.B, p.nkv, u0 / KD_PER_PIECE);
+  KDSegment g;
+  g.b = ahead.b;
+  g.end = u0;
+  ahead.end = u0;
+  int look_tok = 0, look_blk = -1;
+  bool look_in = false;
+  const auto look = [&](int u) {  // the page of this lane in chunk u; the answer is used a chunk later
+    if (u >= ahead.end) ahead.find(p, u);
+    look_tok = (u - ahead.base) * KD_CHUNK + page * tokens;
+    look_in = page < pages && look_tok >= 0 && look_tok < ahead.len;
+    look_blk = look_in ? p.table[ahead.b * p.ldt + (look_tok >> block_shift)] : -1;
+  };
+  const auto load = [&](int s) {  // what was looked up into stage s; returns the pages of it that do not exist
+    const bool there = look_blk >= 0 && look_blk < p.num_blocks;
+    const uint32_t copies = __ballot_sync(0xffffffffu, there && what == 0), lost = __ballot_sync(0xffffffffu, look_in && !there && what == 0);
+    if (lane == 0) mbar_expect_tx(&full[s], __popc(copies) * tokens * (HD + HD / 4));
+    __syncwarp();
+    if (there)
+      bulk_load(ring + s * L::STAGE + dst_off, p.pages + (static_cast<long long>(look_blk) * p.nkv + ahead.kvh) * kv4_page_bytes(bs, HD) + src_off + (look_tok & (bs - 1)) * row,
+                bytes, &full[s]);
+    return lost;
+  };
+  uint32_t lost[KD_STAGES] = {};
+#pragma unroll
+  for (int s = 0; s < KD_STAGES; ++s)
+    if (u0 + warp + s * KD_WARPS < u1) {
+      look(u0 + warp + s * KD_WARPS);
+      lost[s] = load(s);
     }
-    if (!ok && lane == 0) atomicExch(status, ST_TIMEOUT_PRODUCER);
-    // no copy is in flight when the CTA ends, not even where a wait ran out
-    for (long long k = max(done - KD_STAGES, 0LL); k < done; ++k) mbar_wait(&full[k % KD_STAGES], static_cast<uint32_t>((k / KD_STAGES) & 1));
-    return;
-  }
 
-  // ---- the warps that compute
+  // ---- computing
   const int r = lane >> 2, c = lane & 3;
   const int krow = (r & 1) * 4 + (r >> 1);  // row r of S^T is this token of the first 8 of 16, row r + 8 the same of the others: a thread's
                                             // share of V^T (rows 2c, 2c + 1, 2c + 8, 2c + 9) is then tokens c, c + 4, c + 8, c + 12
-  float* merge = reinterpret_cast<float*>(smem + L::OFF_MERGE);
-  int at = warp, stage_at = warp, round = 0;  // this warp's next piece, its stage (stages s, s + 4 .. are warp s's) and how often it was here
-  KDSegment g;
-  g.b = kd_locate(p.plan, p.B, p.nkv, u0);
+  float* meet = reinterpret_cast<float*>(smem + L::OFF_MEET);
+  const Magic magic;
+  int u = u0 + warp, stage_at = 0;  // this warp's next chunk and its stage
+  uint32_t round = 0;
   bool ok = true;
-  for (long long seg = u0; seg < u1;) {
-    g.find(p, g.b, seg);
-    const long long seg_end = min(u1, max(g.base + g.n, seg + 1));
-    const int stop = static_cast<int>(seg_end - u0);
-    const long long len = kd_len(p, g.b), ahead = (u0 - g.base) * KD_PIECE;  // token of piece i: ahead + 64 i
+  for (int seg = u0; seg < u1;) {
+    g.find(p, seg);
+    const int seg_end = min(u1, g.end);
     uint32_t qf[NT][KW][4], qs[NT];  // a word's four pairs of channels (0, 4), (1, 5), (2, 6), (3, 7); the run's sum / 16 in two halves
     float o[NT][HD / 16][4], z[NT][4], m[NT][2], l[NT][2], sc[NT][2];
 #pragma unroll
@@ -222,7 +241,7 @@ kv4_decode_kernel(const VbKv4Decode p, int* status) {
       const int head = t * 8 + r;
       float x[CPR], big = 0.f, sum = 0.f;
       if (head < G) {
-        const uint4* q = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + g.b * p.ldq + (static_cast<long long>(g.kvh) * G + head) * HD + c * CPR);
+        const uint4* q = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + g.b * p.ldq + (g.kvh * G + head) * HD + c * CPR);
 #pragma unroll
         for (int j = 0; j < CPR / 8; ++j) {
           const uint4 v = q[j];
@@ -238,21 +257,23 @@ kv4_decode_kernel(const VbKv4Decode p, int* status) {
       for (int j = 0; j < CPR; ++j) big = fmaxf(big, fabsf(x[j]));
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-      // largest value into [2^10, 2^11): fp16 then holds all 11 bits of what is at least 2^-24 of it, and the sum of 32 channels
+      // largest magnitude into [2^10, 2^11): fp16 then holds all 11 bits of what is at least 2^-24 of it, and the sum of 32 channels
       const int e = max(static_cast<int>(__float_as_uint(big) >> 23) - 127, -100);
-      const float f = __uint_as_float(static_cast<uint32_t>(10 - e + 127) << 23);
+      const float f = copysignf(__uint_as_float(static_cast<uint32_t>(10 - e + 127) << 23), p.scale);
 #pragma unroll
       for (int j = 0; j < CPR; ++j) {
         x[j] *= f;
-        sum += x[j] * 0.0625f;
+        sum += x[j];
       }
+      sum *= 0.0625f;
 #pragma unroll
       for (int w = 0; w < KW; ++w)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) qf[t][w][j] = h2_bits(__floats2half2_rn(x[w * 8 + j], x[w * 8 + j + 4]));
+        for (int j = 0; j < 4; ++j) qf[t][w][j] = pack2(x[w * 8 + j], x[w * 8 + j + 4]);
       const float hi = __half2float(__float2half_rn(sum));
-      qs[t] = h2_bits(__floats2half2_rn(hi, sum - hi));
-      const float back = p.scale * (16.f * 1.4426950408889634f) * __uint_as_float(static_cast<uint32_t>(e - 10 + 127) << 23);
+      qs[t] = pack2(hi, sum - hi);
+      // not zero, so that -inf stays what it is under it
+      const float back = fmaxf(fabsf(p.scale) * (16.f * 1.4426950408889634f) * __uint_as_float(static_cast<uint32_t>(e - 10 + 127) << 23), 1e-37f);
       sc[t][0] = __shfl_sync(0xffffffffu, back, 8 * c);
       sc[t][1] = __shfl_sync(0xffffffffu, back, 8 * c + 4);
       m[t][0] = m[t][1] = -INFINITY;
@@ -261,23 +282,28 @@ kv4_decode_kernel(const VbKv4Decode p, int* status) {
 #pragma unroll
       for (int i = 0; i < HD / 16; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
     }
-    for (; at < stop; at += KD_WARPS) {
-      const uint8_t* stage = smem + stage_at * L::STAGE;
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[stage_at], round & 1));  // else: no more work, the barriers only
-      const uint32_t gone = absent[stage_at];
-      const int left = static_cast<int>(min(len - (ahead + static_cast<long long>(at) * KD_PIECE), static_cast<long long>(KD_PIECE)));  // tokens that count
-#pragma unroll 1
-      for (int i0 = 0; ok && i0 < left; i0 += STEP * 16) {
-        const bool ragged = left < i0 + STEP * 16 || gone != 0;
-        // does token i of the step count?
-        const auto counts = [&](int i) { return i0 + i < left && !((gone >> (bs < KD_PIECE ? (i0 + i) / bs : 0)) & 1u); };
-        const uint8_t* kc = stage + (i0 + krow) * (HD / 2) + c * (CPR / 2);
-        const uint8_t* kp = stage + L::OFF_PK + ((i0 + krow) * (HD / KV4_GROUP) + c * CPR / KV4_GROUP) * 4;
-        float st[NT][STEP][4];
+    for (; u < seg_end; u += KD_WARPS) {
+      const uint8_t* stage = ring + stage_at * L::STAGE;
+      const int next = u + KD_STAGES * KD_WARPS;
+      if (next < u1) look(next);
+      if (ok) {
+        ok = __all_sync(0xffffffffu, kd_wait(&full[stage_at], round & 1));
+        if (!ok)  // no more work, the barriers only; what is in flight gets another while to land
+          for (int s = 0; s < KD_STAGES; ++s) kd_wait(&full[s], (round + (s < stage_at)) & 1);
+      }
+      const int left = min(g.len - (u - g.base) * KD_CHUNK, KD_CHUNK);  // tokens that count
+      if (ok && left > 0) {
+        const uint32_t gone = lost[0];
+        const bool ragged = left < KD_CHUNK || gone != 0;
+        // does token i of the chunk count?
+        const auto counts = [&](int i) { return i < left && !((gone >> (4 * (i / tokens))) & 1u); };
+        const uint8_t* kc = stage + krow * (HD / 2) + c * (CPR / 2);
+        const uint8_t* kp = stage + L::OFF_PK + (krow * (HD / KV4_GROUP) + c * CPR / KV4_GROUP) * 4;
+        float st[NT][KD_TILES][4];
 #pragma unroll
-        for (int i = 0; i < STEP; ++i) {
+        for (int i = 0; i < KD_TILES; ++i) {
           uint32_t wk[2][KW];
-          __half2 par[2];
+          uint32_t par[2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint8_t* at_k = kc + (i * 16 + h * 8) * (HD / 2);
@@ -288,19 +314,18 @@ kv4_decode_kernel(const VbKv4Decode p, int* status) {
               const uint2 v = *reinterpret_cast<const uint2*>(at_k);
               wk[h][0] = v.x; wk[h][1] = v.y;
             }
-            par[h] = *reinterpret_cast<const __half2*>(kp + (i * 16 + h * 8) * (HD / KV4_GROUP) * 4);
+            par[h] = *reinterpret_cast<const uint32_t*>(kp + (i * 16 + h * 8) * (HD / KV4_GROUP) * 4);
           }
-          const Scales f0(__low2half2(par[0])), f1(__low2half2(par[1]));
+          const Scales f0(__byte_perm(par[0], 0u, 0x1010)), f1(__byte_perm(par[1], 0u, 0x1010));
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            st[t][i][0] = st[t][i][1] = st[t][i][2] = st[t][i][3] = 0.f;
-            mma_f16_16816(st[t][i], h2_bits(__high2half2(par[0])), h2_bits(__high2half2(par[1])), 0u, 0u, qs[t], 0u);
+            mma_f16_16816_from_zero(st[t][i], __byte_perm(par[0], 0u, 0x3232), __byte_perm(par[1], 0u, 0x3232), 0u, 0u, qs[t], 0u);
           }
 #pragma unroll
           for (int w = 0; w < KW; ++w) {
             const uint32_t a = wk[0][w], b = wk[1][w], a8 = a >> 8, b8 = b >> 8;
-            const uint32_t a0 = codes_even(a, f0), a1 = codes_even(b, f1), a2 = codes_odd(a, f0), a3 = codes_odd(b, f1);
-            const uint32_t b0 = codes_even(a8, f0), b1 = codes_even(b8, f1), b2 = codes_odd(a8, f0), b3 = codes_odd(b8, f1);
+            const uint32_t a0 = codes_even(a, f0, magic), a1 = codes_even(b, f1, magic), a2 = codes_odd(a, f0, magic), a3 = codes_odd(b, f1, magic);
+            const uint32_t b0 = codes_even(a8, f0, magic), b1 = codes_even(b8, f1, magic), b2 = codes_odd(a8, f0, magic), b3 = codes_odd(b8, f1, magic);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
               mma_f16_16816(st[t][i], a0, a1, a2, a3, qf[t][w][0], qf[t][w][1]);
@@ -308,48 +333,44 @@ kv4_decode_kernel(const VbKv4Decode p, int* status) {
             }
           }
         }
-        uint32_t pb[NT][STEP][2];
+        uint32_t pb[NT][KD_TILES][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           float alpha[2];
           bool grew = false;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int i = 0; i < STEP; ++i) {
-              st[t][i][h] *= sc[t][h];
-              st[t][i][2 + h] *= sc[t][h];
-            }
             if (ragged) {  // what does not count may be anything
 #pragma unroll
-              for (int i = 0; i < STEP; ++i) {
+              for (int i = 0; i < KD_TILES; ++i) {
                 if (!counts(i * 16 + krow)) st[t][i][h] = -INFINITY;
                 if (!counts(i * 16 + krow + 8)) st[t][i][2 + h] = -INFINITY;
               }
             }
-            float mx = m[t][h];
+            float mx = fmaxf(st[t][0][h], st[t][0][2 + h]);
 #pragma unroll
-            for (int i = 0; i < STEP; ++i) mx = fmaxf(mx, fmaxf(st[t][i][h], st[t][i][2 + h]));
+            for (int i = 1; i < KD_TILES; ++i) mx = fmaxf(mx, fmaxf(st[t][i][h], st[t][i][2 + h]));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            mx = fmaxf(m[t][h], mx * sc[t][h]);  // the factor is not negative: its sign is the query's
             grew |= mx > m[t][h];
-            alpha[h] = m[t][h] == -INFINITY ? 0.f : fast_exp2(m[t][h] - mx);
-            m[t][h] = mx;
             const float mu = mx == -INFINITY ? 0.f : mx;
+            alpha[h] = fast_exp2(m[t][h] - mu);
+            m[t][h] = mx;
             float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < STEP; ++i) {
-              st[t][i][h] = fast_exp2(st[t][i][h] - mu);
-              st[t][i][2 + h] = fast_exp2(st[t][i][2 + h] - mu);
+            for (int i = 0; i < KD_TILES; ++i) {
+              st[t][i][h] = fast_exp2(fmaf(st[t][i][h], sc[t][h], -mu));
+              st[t][i][2 + h] = fast_exp2(fmaf(st[t][i][2 + h], sc[t][h], -mu));
               sum += st[t][i][h] + st[t][i][2 + h];
             }
             l[t][h] = l[t][h] * alpha[h] + sum;
           }
 #pragma unroll
-          for (int i = 0; i < STEP; ++i) {
-            pb[t][i][0] = movmatrix_t(h2_bits(__floats2half2_rn(st[t][i][0], st[t][i][1])));
-            pb[t][i][1] = movmatrix_t(h2_bits(__floats2half2_rn(st[t][i][2], st[t][i][3])));
+          for (int i = 0; i < KD_TILES; ++i) {
+            pb[t][i][0] = movmatrix_t(pack2(st[t][i][0], st[t][i][1]));
+            pb[t][i][1] = movmatrix_t(pack2(st[t][i][2], st[t][i][3]));
           }
           if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
@@ -361,10 +382,10 @@ kv4_decode_kernel(const VbKv4Decode p, int* status) {
           }
         }
         // values: this thread's run of channels of four tokens at a time
-        const uint8_t* vc = stage + L::CODES + (i0 + c) * (HD / 2) + r * (VPR / 2);
-        const uint8_t* vp = stage + L::OFF_PK + L::PARAMS + ((i0 + c) * (HD / KV4_GROUP) + r * VPR / KV4_GROUP) * 4;
+        const uint8_t* vc = stage + L::CODES + c * (HD / 2) + r * (VPR / 2);
+        const uint8_t* vp = stage + L::OFF_PK + L::PARAMS + (c * (HD / KV4_GROUP) + r * VPR / KV4_GROUP) * 4;
 #pragma unroll
-        for (int i = 0; i < STEP; ++i) {
+        for (int i = 0; i < KD_TILES; ++i) {
           uint32_t wv[4][VW], pv[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -382,7 +403,7 @@ kv4_decode_kernel(const VbKv4Decode p, int* status) {
             for (int j = 0; j < 4; ++j)
               if (!counts(i * 16 + j * 4 + c)) pv[j] = 0u;  // values of zero
           }
-          const Scales f01(h2_of(__byte_perm(pv[0], pv[1], 0x5410))), f23(h2_of(__byte_perm(pv[2], pv[3], 0x5410)));
+          const Scales f01(__byte_perm(pv[0], pv[1], 0x5410)), f23(__byte_perm(pv[2], pv[3], 0x5410));
           const uint32_t m01 = __byte_perm(pv[0], pv[1], 0x7632), m23 = __byte_perm(pv[2], pv[3], 0x7632);
 #pragma unroll
           for (int t = 0; t < NT; ++t) mma_f16_16816(z[t], m01, 0u, m23, 0u, pb[t][i][0], pb[t][i][1]);
@@ -392,8 +413,8 @@ kv4_decode_kernel(const VbKv4Decode p, int* status) {
             for (int half = 0; half < 2; ++half) {  // channels 0..3 and 4..7 of the word: a pair of tokens side by side
               const uint32_t sel = half == 0 ? 0x5410 : 0x7632;
               const uint32_t x = __byte_perm(wv[0][w], wv[1][w], sel), y = __byte_perm(wv[2][w], wv[3][w], sel), x8 = x >> 8, y8 = y >> 8;
-              const uint32_t a0 = codes_even(x, f01), a1 = codes_odd(x, f01), a2 = codes_even(y, f23), a3 = codes_odd(y, f23);
-              const uint32_t b0 = codes_even(x8, f01), b1 = codes_odd(x8, f01), b2 = codes_even(y8, f23), b3 = codes_odd(y8, f23);
+              const uint32_t a0 = codes_even(x, f01, magic), a1 = codes_odd(x, f01, magic), a2 = codes_even(y, f23, magic), a3 = codes_odd(y, f23, magic);
+              const uint32_t b0 = codes_even(x8, f01, magic), b1 = codes_odd(x8, f01, magic), b2 = codes_even(y8, f23, magic), b3 = codes_odd(y8, f23, magic);
 #pragma unroll
               for (int t = 0; t < NT; ++t) {
                 mma_f16_16816(o[t][w * 4 + half * 2], a0, a1, a2, a3, pb[t][i][0], pb[t][i][1]);
@@ -403,60 +424,93 @@ kv4_decode_kernel(const VbKv4Decode p, int* status) {
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[stage_at]);
-      stage_at += KD_WARPS;
-      if (stage_at >= KD_STAGES) {
-        stage_at -= KD_STAGES;
+      lost[0] = lost[1];
+      if (ok && next < u1) lost[1] = load(stage_at);
+      if (++stage_at == KD_STAGES) {
+        stage_at = 0;
         ++round;
       }
     }
 
-    // ---- end of a segment: the four warps' sums meet, 8 heads at a time. O^T[channel r VPR + 2 i (+ 1), head] = 16 o + z
-    const bool whole = seg == g.base && seg_end == g.base + g.n;
-    float* part = p.part + (2LL * blockIdx.x + (seg == u0 ? 0 : 1)) * G * (HD + 2);
+    // ---- end of a segment: warps 1 and 3 hand their sums to 0 and 2, then 2 to 0, lane by lane. O^T[channel r VPR + 2 i (+ 1), head] = 16 o + z
+    const bool whole = seg == g.base && seg_end == g.end;
+    float* part = p.part + (2LL * blockIdx.x + (seg == u0 ? 0 : 1)) * G * (HD + 4);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
+      float sum[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float sum = l[t][h];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-        float* row = merge + (warp * 8 + 2 * c + h) * L::MROW;
+        sum[h] = l[t][h];
+        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 4);
+        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 8);
+        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 16);
 #pragma unroll
-        for (int i = 0; i < HD / 16; ++i)
-          *reinterpret_cast<float2*>(row + r * VPR + 2 * i) = make_float2(fmaf(16.f, o[t][i][h], z[t][h]), fmaf(16.f, o[t][i][2 + h], z[t][h]));
-        if (r == 0) {
-          row[HD] = m[t][h];
-          row[HD + 1] = sum;
+        for (int i = 0; i < HD / 16; ++i) {
+          o[t][i][h] = fmaf(16.f, o[t][i][h], z[t][h]);
+          o[t][i][2 + h] = fmaf(16.f, o[t][i][2 + h], z[t][h]);
         }
       }
-      asm volatile("bar.sync 1, %0;" ::"n"(KD_WARPS * 32) : "memory");
-      for (int i = threadIdx.x; i < min(G - t * 8, 8) * HD; i += KD_WARPS * 32) {
-        const int d = i % HD, head = t * 8 + i / HD;
-        const float* row = merge + (i / HD) * L::MROW;
-        float M = -INFINITY, sum = 0.f, acc = 0.f;
 #pragma unroll
-        for (int w = 0; w < KD_WARPS; ++w) M = fmaxf(M, row[w * 8 * L::MROW + HD]);
+      for (int step = 1; step < KD_WARPS; step *= 2) {
+        float4* mine = reinterpret_cast<float4*>(meet + (step == 1 ? warp >> 1 : 0) * 32 * L::MEET) + lane;  // float4 i of lane: 32 i + lane
+        if ((warp & (2 * step - 1)) == step) {
 #pragma unroll
-        for (int w = 0; w < KD_WARPS; ++w) {
-          const float* rw = row + w * 8 * L::MROW;
-          const float f = rw[HD] == -INFINITY ? 0.f : fast_exp2(rw[HD] - M);
-          sum += rw[HD + 1] * f;
-          acc += rw[d] * f;
+          for (int i = 0; i < HD / 16; ++i) mine[32 * i] = make_float4(o[t][i][0], o[t][i][1], o[t][i][2], o[t][i][3]);
+          mine[32 * (HD / 16)] = make_float4(m[t][0], m[t][1], sum[0], sum[1]);
         }
-        if (whole) {
-          static_cast<T*>(p.out)[(static_cast<long long>(g.b) * p.nh + g.kvh * G + head) * HD + d] = static_cast<T>(sum == 0.f ? 0.f : acc / sum);
-        } else {
-          part[head * (HD + 2) + d] = acc;
-          if (d == 0) {
-            part[head * (HD + 2) + HD] = M;
-            part[head * (HD + 2) + HD + 1] = sum;
+        __syncthreads();
+        if ((warp & (2 * step - 1)) == 0) {
+          const float4 other = mine[32 * (HD / 16)];
+          float fa[2], fb[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float mo = h == 0 ? other.x : other.y, M = fmaxf(m[t][h], mo), mu = M == -INFINITY ? 0.f : M;
+            fa[h] = fast_exp2(m[t][h] - mu);
+            fb[h] = fast_exp2(mo - mu);
+            m[t][h] = M;
+            sum[h] = sum[h] * fa[h] + (h == 0 ? other.z : other.w) * fb[h];
+          }
+#pragma unroll
+          for (int i = 0; i < HD / 16; ++i) {
+            const float4 v = mine[32 * i];
+            o[t][i][0] = o[t][i][0] * fa[0] + v.x * fb[0];
+            o[t][i][1] = o[t][i][1] * fa[1] + v.y * fb[1];
+            o[t][i][2] = o[t][i][2] * fa[0] + v.z * fb[0];
+            o[t][i][3] = o[t][i][3] * fa[1] + v.w * fb[1];
+          }
+        }
+        if (step * 2 < KD_WARPS || NT > 1) __syncthreads();  // what was handed over is read
+      }
+      if (warp == 0) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int head = t * 8 + 2 * c + h;
+          if (head >= G) continue;
+          if (whole) {
+            const float inv = sum[h] == 0.f ? 0.f : 1.f / sum[h];
+            T* out = static_cast<T*>(p.out) + (static_cast<long long>(g.b) * p.nh + g.kvh * G + head) * HD + r * VPR;
+#pragma unroll
+            for (int i = 0; i < HD / 16; i += 4) {
+              uint4 v;
+              T* e = reinterpret_cast<T*>(&v);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                e[2 * j] = static_cast<T>(o[t][i + j][h] * inv);
+                e[2 * j + 1] = static_cast<T>(o[t][i + j][2 + h] * inv);
+              }
+              *reinterpret_cast<uint4*>(out + 2 * i) = v;
+            }
+          } else {
+            float* to = part + head * (HD + 4);
+#pragma unroll
+            for (int i = 0; i < HD / 16; i += 2)
+              *reinterpret_cast<float4*>(to + r * VPR + 2 * i) = make_float4(o[t][i][h], o[t][i][2 + h], o[t][i + 1][h], o[t][i + 1][2 + h]);
+            if (r == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(m[t][h], sum[h]);
           }
         }
       }
-      asm volatile("bar.sync 1, %0;" ::"n"(KD_WARPS * 32) : "memory");
     }
+    if (NT == 1) __syncthreads();
     seg = seg_end;
   }
   if (!ok && lane == 0) atomicExch(status, ST_TIMEOUT_EPILOGUE);
@@ -469,20 +523,18 @@ kv4_join_kernel(const VbKv4Decode p, int ctas) {
   __shared__ float red[HD / 32];
   __shared__ float wgt[HD];
   const int b = blockIdx.y, h = blockIdx.x, G = p.nh / p.nkv, kvh = h / G, head = h % G;
-  const long long total = kd_total(p), per = kd_per(total, ctas);
-  const long long n = static_cast<long long>(p.plan[b + 1]) - p.plan[b];
+  const int total = kd_total(p), per = kd_per(total, ctas), n = p.plan[b + 1] - p.plan[b];
   T* out = static_cast<T*>(p.out) + (static_cast<long long>(b) * p.nh + h) * HD + threadIdx.x;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the runs' sums, and what came before them
   if (n <= 0 || kd_len(p, b) == 0) {
     *out = static_cast<T>(0.f);
     return;
   }
-  const long long base = static_cast<long long>(p.plan[b]) * p.nkv + kvh * n;
-  const long long i0 = base / per, i1 = min((base + n - 1) / per, static_cast<long long>(ctas - 1));
+  const int base = p.plan[b] * p.nkv + kvh * n, i0 = max(base, 0) / per, i1 = min((base + n - 1) / per, ctas - 1);
   if (i0 >= i1) return;
-  const auto slot = [&](long long i) { return p.part + ((2 * i + (i * per >= base ? 0 : 1)) * G + head) * (HD + 2); };
+  const auto slot = [&](int i) { return p.part + ((2LL * i + (i * per >= base ? 0 : 1)) * G + head) * (HD + 4); };
   float M = -INFINITY;
-  for (long long i = i0 + threadIdx.x; i <= i1; i += HD) M = fmaxf(M, slot(i)[HD]);
+  for (int i = i0 + threadIdx.x; i <= i1; i += HD) M = fmaxf(M, slot(i)[HD]);
 #pragma unroll
   for (int k = 16; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = M;
@@ -491,8 +543,8 @@ kv4_join_kernel(const VbKv4Decode p, int ctas) {
 #pragma unroll
   for (int w = 1; w < HD / 32; ++w) M = fmaxf(M, red[w]);
   float acc = 0.f, sum = 0.f;
-  for (long long at = i0; at <= i1; at += HD) {
-    const int k = static_cast<int>(min(static_cast<long long>(HD), i1 - at + 1));
+  for (int at = i0; at <= i1; at += HD) {
+    const int k = min(HD, i1 - at + 1);
     __syncthreads();
     if (threadIdx.x < k) {
       const float mi = slot(at + threadIdx.x)[HD];
@@ -544,8 +596,8 @@ static cudaError_t kd_launch(const VbKv4Decode& p, int* status, cudaStream_t s) 
   constexpr int smem = KDSmem<HD, NT>::TOTAL;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  const int ctas = num_sms() * KD_CTAS;
-  kern<<<ctas, KD_THREADS, smem, s>>>(p, status);
+  const int ctas = num_sms() * kd_ctas(NT);
+  kern<<<ctas, KD_THREADS, smem, s>>>(p, __builtin_ctz(static_cast<unsigned>(p.block_size)), status);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[1];
@@ -573,7 +625,7 @@ using namespace vb;
 
 extern "C" long long vb_kv4_decode_scratch(int B, int nh, int nkv, int hd) {
   const int G = nh / nkv;
-  return 2LL * num_sms() * KD_CTAS * G * (hd + 2);
+  return 2LL * num_sms() * kd_ctas(G <= 8 ? 1 : 2) * G * (hd + 4);
 }
 
 extern "C" int vb_kv4_status() {
@@ -588,7 +640,9 @@ extern "C" int vb_kv4_status() {
 
 extern "C" int vb_kv4_decode(const VbKv4Decode* a, cudaStream_t s) {
   if (a->B == 0) return 0;
-  if ((a->hd != 64 && a->hd != 128) || a->nh % a->nkv || a->nh / a->nkv > 16 || a->B > 65535) return -2;
+  if ((a->hd != 64 && a->hd != 128) || a->nh % a->nkv || a->nh / a->nkv > 16 || a->B > 65535 || (a->block_size & (a->block_size - 1)) || a->block_size < 16) return -2;
+  const long long tokens = static_cast<long long>(a->width) * a->block_size;
+  if (tokens > 1LL << 30 || ((tokens + KD_PIECE - 1) / KD_PIECE) * KD_PER_PIECE * a->B * a->nkv > 0x7fffffffLL) return -4;  // counted in 31 bits
   VbKv4Decode p = *a;
   int* status = nullptr;
   cudaError_t e = cudaGetSymbolAddress(reinterpret_cast<void**>(&status), g_kv4_status);
