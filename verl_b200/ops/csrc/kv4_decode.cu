@@ -17,7 +17,7 @@
 // The least values m of the groups go through the matrix unit apart from the codes:
 //   S gains m (sum of q over the thread's channels), one more k step of an instruction that has m twice against that sum's two fp16 halves;
 //   O gains sum_t p_t m_t, the same for all channels of a thread: one accumulator more, added at the end.
-// 1.2 instructions an element. Queries are scaled by a power of two per head so that fp16 holds them exactly; weights are e^(s - max) <= 1 in fp16.
+// 1.2 instructions an element. Queries are scaled by a power of two per head so that fp16 holds them exactly; weights are e^(s - reference) <= 64 in fp16.
 #include <math.h>
 
 #include "kv4_common.cuh"
@@ -155,15 +155,20 @@ struct KDSegment {
   }
 };
 
-__device__ __forceinline__ bool kd_wait(uint64_t* bar, uint32_t parity) {  // as mbar_wait, asleep up to 2 us at a time
+// as mbar_wait, asleep up to 2 us at a time
+__device__ __forceinline__ bool kd_try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 2000;\nselp.u32 %0, 1, 0, p;\n}\n"
+               : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool kd_wait(uint64_t* full, uint32_t parity) {
+  const uint32_t bar = smem_u32(full);
+  if (kd_try_wait(bar, parity)) return true;
   const uint64_t t0 = global_timer_ns();
-  for (;;) {
-    uint32_t ok;
-    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 2000;\nselp.u32 %0, 1, 0, p;\n}\n"
-                 : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-    if (ok) return true;
+  while (!kd_try_wait(bar, parity))
     if (global_timer_ns() - t0 > VB_WAIT_LIMIT_NS) return false;
-  }
+  return true;
 }
 
 template <int HD, int NT, typename T>
@@ -185,42 +190,48 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
   }
   __syncwarp();
 
-  // ---- loading: 4 lanes per page of a chunk (keys' codes, values' codes, keys' parameters, values' parameters)
-  const int tokens = min(bs, KD_CHUNK), pages = KD_CHUNK / tokens, page = lane >> 2, what = lane & 3;
+  // ---- loading. Lanes 8 j .. 8 j + 7 look up and fetch the j-th of the warp's next four chunks: four lanes a page (keys' codes, values' codes,
+  // keys' parameters, values' parameters), one page or two a chunk
+  const int tokens = min(bs, KD_CHUNK), page = (lane >> 2) & 1, what = lane & 3;
   const uint32_t row = what < 2 ? HD / 2 : (HD / KV4_GROUP) * 4, bytes = tokens * row;
   const int dst_off = (what < 2 ? what * L::CODES : L::OFF_PK + (what - 2) * L::PARAMS) + page * bytes;
   const int src_off = what < 2 ? kv4_codes_at(bs, HD, what) : kv4_params_at(bs, HD, what - 2);
-  KDSegment ahead;  // of the chunk that is looked up
+  KDSegment ahead;  // of the chunk that this lane looks up
   ahead.b = kd_locate(p.plan, p.B, p.nkv, u0 / KD_PER_PIECE);
   KDSegment g;
   g.b = ahead.b;
   g.end = u0;
   ahead.end = u0;
-  int look_tok = 0, look_blk = -1;
-  bool look_in = false;
-  const auto look = [&](int u) {  // the page of this lane in chunk u; the answer is used a chunk later
+  const uint8_t* src = nullptr;  // what this lane fetches (null: nothing)
+  bool missing = false;          // of a page that does not exist
+  const auto look = [&](int u) {  // chunk u is the first of the four; the answer is used a chunk later
+    u += (lane >> 3) * KD_WARPS;
+    src = nullptr;
+    missing = false;
+    if (u >= u1 || page * tokens >= KD_CHUNK) return;
     if (u >= ahead.end) ahead.find(p, u);
-    look_tok = (u - ahead.base) * KD_CHUNK + page * tokens;
-    look_in = page < pages && look_tok >= 0 && look_tok < ahead.len;
-    look_blk = look_in ? p.table[ahead.b * p.ldt + (look_tok >> block_shift)] : -1;
+    const int tok = (u - ahead.base) * KD_CHUNK + page * tokens;
+    if (tok < 0 || tok >= ahead.len) return;
+    const int blk = p.table[ahead.b * p.ldt + (tok >> block_shift)];
+    missing = blk < 0 || blk >= p.num_blocks;
+    if (!missing)
+      src = p.pages + (static_cast<long long>(blk) * p.nkv + ahead.kvh) * kv4_page_bytes(bs, HD) + src_off + (tok & (bs - 1)) * row;
   };
-  const auto load = [&](int s) {  // what was looked up into stage s; returns the pages of it that do not exist
-    const bool there = look_blk >= 0 && look_blk < p.num_blocks;
-    const uint32_t copies = __ballot_sync(0xffffffffu, there && what == 0), lost = __ballot_sync(0xffffffffu, look_in && !there && what == 0);
+  const auto load = [&](int j, int s) {  // the j-th of the four into stage s; returns the pages of it that do not exist (bits 0 and 4)
+    const bool mine = (lane >> 3) == j;
+    const uint32_t copies = __ballot_sync(0xffffffffu, mine && src != nullptr && what == 0);
+    const uint32_t gone = __ballot_sync(0xffffffffu, mine && missing && what == 0);
     if (lane == 0) mbar_expect_tx(&full[s], __popc(copies) * tokens * (HD + HD / 4));
     __syncwarp();
-    if (there)
-      bulk_load(ring + s * L::STAGE + dst_off, p.pages + (static_cast<long long>(look_blk) * p.nkv + ahead.kvh) * kv4_page_bytes(bs, HD) + src_off + (look_tok & (bs - 1)) * row,
-                bytes, &full[s]);
-    return lost;
+    if (mine && src != nullptr) bulk_load(ring + s * L::STAGE + dst_off, src, bytes, &full[s]);
+    return gone >> (8 * j);
   };
   uint32_t lost[KD_STAGES] = {};
+  look(u0 + warp);
 #pragma unroll
   for (int s = 0; s < KD_STAGES; ++s)
-    if (u0 + warp + s * KD_WARPS < u1) {
-      look(u0 + warp + s * KD_WARPS);
-      lost[s] = load(s);
-    }
+    if (u0 + warp + s * KD_WARPS < u1) lost[s] = load(s, s);
+  int looked = KD_STAGES;  // the next of the four
 
   // ---- computing
   const int r = lane >> 2, c = lane & 3;
@@ -285,7 +296,10 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
     for (; u < seg_end; u += KD_WARPS) {
       const uint8_t* stage = ring + stage_at * L::STAGE;
       const int next = u + KD_STAGES * KD_WARPS;
-      if (next < u1) look(next);
+      if (looked == 4) {
+        looked = 0;
+        if (next < u1) look(next);
+      }
       if (ok) {
         ok = __all_sync(0xffffffffu, kd_wait(&full[stage_at], round & 1));
         if (!ok)  // no more work, the barriers only; what is in flight gets another while to land
@@ -336,8 +350,7 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
         uint32_t pb[NT][KD_TILES][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          float alpha[2];
-          bool grew = false;
+          float top[2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             if (ragged) {  // what does not count may be anything
@@ -347,38 +360,44 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
                 if (!counts(i * 16 + krow + 8)) st[t][i][2 + h] = -INFINITY;
               }
             }
-            float mx = fmaxf(st[t][0][h], st[t][0][2 + h]);
+            top[h] = fmaxf(st[t][0][h], st[t][0][2 + h]);
 #pragma unroll
-            for (int i = 1; i < KD_TILES; ++i) mx = fmaxf(mx, fmaxf(st[t][i][h], st[t][i][2 + h]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            mx = fmaxf(m[t][h], mx * sc[t][h]);  // the factor is not negative: its sign is the query's
-            grew |= mx > m[t][h];
-            const float mu = mx == -INFINITY ? 0.f : mx;
-            alpha[h] = fast_exp2(m[t][h] - mu);
-            m[t][h] = mx;
-            float sum = 0.f;
+            for (int i = 1; i < KD_TILES; ++i) top[h] = fmaxf(top[h], fmaxf(st[t][i][h], st[t][i][2 + h]));
+            top[h] *= sc[t][h];  // the factor is not negative: its sign is the query's
+          }
+          // the reference stays until a score is 2^6 above it: weights up to 64 are as exact in fp16 as those up to 1
+          if (__any_sync(0xffffffffu, top[0] > m[t][0] + 6.f || top[1] > m[t][1] + 6.f)) {
+            float alpha[2];
 #pragma unroll
-            for (int i = 0; i < KD_TILES; ++i) {
-              st[t][i][h] = fast_exp2(fmaf(st[t][i][h], sc[t][h], -mu));
-              st[t][i][2 + h] = fast_exp2(fmaf(st[t][i][2 + h], sc[t][h], -mu));
-              sum += st[t][i][h] + st[t][i][2 + h];
+            for (int h = 0; h < 2; ++h) {
+              float mx = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 4));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+              mx = fmaxf(fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16)), m[t][h]);
+              alpha[h] = fast_exp2(m[t][h] - (mx == -INFINITY ? 0.f : mx));
+              m[t][h] = mx;
+              l[t][h] *= alpha[h];
+              z[t][h] *= alpha[h];
             }
-            l[t][h] = l[t][h] * alpha[h] + sum;
-          }
-#pragma unroll
-          for (int i = 0; i < KD_TILES; ++i) {
-            pb[t][i][0] = movmatrix_t(pack2(st[t][i][0], st[t][i][1]));
-            pb[t][i][1] = movmatrix_t(pack2(st[t][i][2], st[t][i][3]));
-          }
-          if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
             for (int i = 0; i < HD / 16; ++i) {
               o[t][i][0] *= alpha[0]; o[t][i][1] *= alpha[1];
               o[t][i][2] *= alpha[0]; o[t][i][3] *= alpha[1];
             }
-            z[t][0] *= alpha[0]; z[t][1] *= alpha[1];
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float mu = m[t][h] == -INFINITY ? 0.f : m[t][h];
+#pragma unroll
+            for (int i = 0; i < KD_TILES; ++i) {
+              st[t][i][h] = fast_exp2(fmaf(st[t][i][h], sc[t][h], -mu));
+              st[t][i][2 + h] = fast_exp2(fmaf(st[t][i][2 + h], sc[t][h], -mu));
+              l[t][h] += st[t][i][h] + st[t][i][2 + h];
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < KD_TILES; ++i) {
+            pb[t][i][0] = movmatrix_t(pack2(st[t][i][0], st[t][i][1]));
+            pb[t][i][1] = movmatrix_t(pack2(st[t][i][2], st[t][i][3]));
           }
         }
         // values: this thread's run of channels of four tokens at a time
@@ -425,7 +444,8 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
       }
       __syncwarp();
       lost[0] = lost[1];
-      if (ok && next < u1) lost[1] = load(stage_at);
+      if (ok && next < u1) lost[1] = load(looked, stage_at);
+      ++looked;
       if (++stage_at == KD_STAGES) {
         stage_at = 0;
         ++round;
