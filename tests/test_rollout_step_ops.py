@@ -238,7 +238,8 @@ def attention_64(q, pages, table, lens, bs, scale):
     """(output, largest |output| that the roundings of the kernel may change each value by), in 64 bits."""
     B, nh, hd = q.shape
     (codes, step, _), (k, v) = unpacked(pages, bs, hd), rows_of(pages, bs, hd)
-    part = (codes.astype(np.float64) * step.astype(np.float64)).reshape(*codes.shape[:-2], hd)     # what a code adds to its group's least value
+    step = np.broadcast_to(step.astype(np.float64), codes.shape).reshape(*codes.shape[:-2], hd)
+    part = codes.reshape(*codes.shape[:-2], hd) * step         # what a code adds to its group's least value
     nkv = k.shape[1]
     q = q.double().cpu().numpy().reshape(B, nkv, nh // nkv, hd)
     out, off = np.zeros((B, nkv, nh // nkv, hd)), np.zeros((B, nkv, nh // nkv, hd))
@@ -246,21 +247,22 @@ def attention_64(q, pages, table, lens, bs, scale):
         if n == 0:
             continue
         blk = table[b, : -(-n // bs)].cpu().numpy()
-        kk, vv, kp, vp = (x[blk].transpose(1, 0, 2, 3).reshape(nkv, -1, hd)[:, :n] for x in (k, v, part[0], part[1]))
+        kk, vv, kp, vp, ks, vs = (x[blk].transpose(1, 0, 2, 3).reshape(nkv, -1, hd)[:, :n] for x in (k, v, part[0], part[1], step[0], step[1]))
         s = np.einsum("hgd,htd->hgt", q[b], kk) * scale
         w = np.exp(s - s.max(-1, keepdims=True))
         w /= w.sum(-1, keepdims=True)
         out[b] = np.einsum("hgt,htd->hgd", w, vv)
-        # The kernel rounds code * scale to fp16 (U16 of it, or half of 16 times the least fp16 number: 2^-21) and nothing else of a key or value:
-        # the least values are fp16 already, their factor is held in two halves (2^-22). Sums of products are fp32 (their length times U32). A
-        # score is off by at most ds, a weight by 2 ds and by the rounding of e^s to fp16 (U16, and 2^-25 of the largest where it is small),
-        # which acts on the whole value.
-        size_q = np.abs(q[b]).sum(-1, keepdims=True)
-        ds = scale * (U16 * np.einsum("hgd,htd->hgt", np.abs(q[b]), np.abs(kp)) + (2.0**-21 * size_q)
-                      + (2.0**-22 + (hd + 8) * U32) * np.einsum("hgd,htd->hgt", np.abs(q[b]), np.abs(kk) + 2 * np.abs(kp)))
+        # The kernel rounds to fp16, for neighbours a, b of a pair of codes: a s / 16, (b + a / 16) s and (keys) 16 q_a - q_b. With a <= 15, and U16 of each:
+        #   keys:   2 (16 |q_a| + |q_b|) a s / 16 + |q_b| (b + a / 16) s  <=  2 sum |q| code s + 3 sum |q| s
+        #   values: a s, and b s + 2 a s / 16 <= b s + 2 s
+        # (or half the least fp16 number, at most 16 times: 2^-21). The least values are fp16 already, their factor is held in two halves (2^-22).
+        # Sums of products are fp32 (their length times U32). A score is off by at most ds, a weight by 2 ds and by the rounding of
+        # e^(s - reference) to fp16 (U16, and 2^-25 of the largest where it is small), which acts on the whole value.
+        dot = lambda x: np.einsum("hgd,htd->hgt", np.abs(q[b]), np.abs(x))
+        ds = scale * (U16 * dot(2 * kp + 3 * ks) + 2.0**-21 * np.abs(q[b]).sum(-1, keepdims=True) + (2.0**-22 + (hd + 8) * U32) * dot(np.abs(kk) + 3 * kp))
         ds = ds.max(-1, keepdims=True)
-        size, codes_size = (np.einsum("hgt,htd->hgd", w, np.abs(x)) for x in (vv, vp))
-        off[b] = ((2 * ds + 2 * U16) * size + U16 * codes_size + 2.0**-21 + (n + 64) * U32 * (size + 2 * codes_size)
+        size, codes_size = (np.einsum("hgt,htd->hgd", w, np.abs(x)) for x in (vv, vp + 2 * vs))
+        off[b] = ((2 * ds + 2 * U16) * size + U16 * codes_size + 2.0**-21 + (n + 64) * U32 * (size + 3 * codes_size)
                   + 2.0**-24 * n * w.max(-1, keepdims=True) * np.abs(vv).max(1)[:, None])
     return out.reshape(B, nh, hd), off.reshape(B, nh, hd)
 

@@ -5,19 +5,22 @@
 // (sequence, head) leaves its sums in a slot of its own, and a second small launch, started early by programmatic dependence, joins them
 // by their maxima, in the order of the runs: no atomics, the same bits every time.
 //
-// A CTA: its four warps take chunks of 32 tokens in turn, each with two stages of shared memory of its own that it fills by bulk copies (a chunk is
-// at most 8 contiguous runs; four for blocks of 32 and more) while it works on the other: no warp waits for another until the end of a segment,
-// where their sums meet in pairs, fragment by fragment.
-//   S^T[32 tokens, 8 heads] = K[32, hd] Q^T        keys are the A operand of m16n8k16: a thread's share of a token's row is one contiguous run
-//   O^T[hd, 8 heads]       += V^T[hd, 32] P^T      values are the A operand as well; P^T is S^T's accumulator through movmatrix
+// A CTA: its four warps take pieces in turn. Each has room for the keys and the values of one piece, which it fills by bulk copies (a half is at
+// most 8 contiguous runs, two for blocks of 64 and more): the next keys while it works on values, the next values while it works on keys. No
+// warp waits for another until the end of a segment, where their sums meet in pairs, fragment by fragment.
+//   S^T[64 tokens, 8 heads] = K[64, hd] Q^T        keys are the A operand of m16n8k16: a thread's share of a token's row is one contiguous run
+//   O^T[hd, 8 heads]       += V^T[hd, 64] P^T      values are the A operand as well; P^T is S^T's accumulator through movmatrix
 // so that with up to 8 heads to a KV head a matrix instruction takes 256 cache elements (query heads as the 16 rows would take 128).
 //
-// A code becomes a number without a conversion: (w & 0x000f000f) | 0x5400.. is 64 + q / 16 in fp16 and (w & 0x00f000f0) | 0x4400.. is 4 + q / 16, so
-// that one multiply-add, x s - 64 s, gives a pair of q s / 16, each rounded once (64 s is exact; it is finite because the append keeps s below 1024).
+// Codes become numbers without a conversion, two bytes at a time: a byte that holds codes (a, b) under the exponent of 64 is 64 + b + a / 16 in
+// fp16, and 64 + a / 16 with b masked off, so that one multiply-add, x s - 64 s, gives a pair of (b + a / 16) s or of a s / 16, each rounded
+// once (64 s is exact; it is finite because the append keeps s below 1024). b is not taken apart from a:
+//   q_a a + q_b b = q_b (b + a / 16) + (16 q_a - q_b) a / 16        for keys, where the queries are brought into that form once a segment
+//   sum p b       = sum p (b + a / 16) - sum p a / 16               for values, once at the end
 // The least values m of the groups go through the matrix unit apart from the codes:
 //   S gains m (sum of q over the thread's channels), one more k step of an instruction that has m twice against that sum's two fp16 halves;
 //   O gains sum_t p_t m_t, the same for all channels of a thread: one accumulator more, added at the end.
-// 1.2 instructions an element. Queries are scaled by a power of two per head so that fp16 holds them exactly; weights are e^(s - reference) <= 64 in fp16.
+// 1.1 instructions an element. Queries are scaled by a power of two per head, into fp16's range; weights are e^(s - reference) <= 64 in fp16.
 #include <math.h>
 
 #include "kv4_common.cuh"
@@ -29,12 +32,9 @@ namespace vb {
 int num_sms();
 
 constexpr int KD_PIECE = 64;                     // tokens that the plan counts in
-constexpr int KD_CHUNK = 32;                     // tokens of a stage
-constexpr int KD_PER_PIECE = KD_PIECE / KD_CHUNK;
 constexpr int KD_WARPS = 4;
 constexpr int KD_THREADS = KD_WARPS * 32;
-constexpr int KD_STAGES = 2;                     // of a warp
-constexpr int KD_TILES = KD_CHUNK / 16;
+constexpr int KD_TILES = KD_PIECE / 16;
 __host__ __device__ constexpr int kd_ctas(int nt) { return nt == 1 ? 4 : 3; }  // CTAs of an SM: what registers and shared memory hold
 constexpr int KD_MIN_PIECES = 4;                 // shortest run of a CTA
 
@@ -81,42 +81,33 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
   return d;
 }
-// Factors of a pair of codes: their scales, and what 64 and 4 become under them.
+// Factors of a pair of codes: their scales, and what -64 becomes under them.
 struct Scales {
-  uint32_t s, n64, n4;
-  __device__ __forceinline__ explicit Scales(uint32_t v) : s(v), n64(mul2(v, 0xd400d400u)), n4(mul2(v, 0xc400c400u)) {}
+  uint32_t s, n;
+  __device__ __forceinline__ explicit Scales(uint32_t v) : s(v), n(mul2(v, 0xd400d400u)) {}
 };
-// The exponents that codes are put under. An instruction takes one constant: these stay in registers, where the compiler would otherwise make
-// them again for each of the 256 uses in a piece.
-struct Magic {
-  uint32_t even, odd;
-  __device__ __forceinline__ Magic() {
-    asm volatile("mov.b32 %0, 0x54005400;" : "=r"(even));
-    asm volatile("mov.b32 %0, 0x44004400;" : "=r"(odd));
-  }
-};
-// q s / 16 for pairs 0 / 1 of the four that a word of codes holds: its nibbles (0, 4) and (1, 5); the other two after a shift by 8
-__device__ __forceinline__ uint32_t codes_even(uint32_t w, const Scales& f, const Magic& k) {
-  uint32_t x;
-  asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xea;" : "=r"(x) : "r"(w), "r"(k.even));
-  return fma2(x, f.s, f.n64);
-}
-__device__ __forceinline__ uint32_t codes_odd(uint32_t w, const Scales& f, const Magic& k) {
-  uint32_t x;
-  asm("lop3.b32 %0, %1, 0x00f000f0, %2, 0xea;" : "=r"(x) : "r"(w), "r"(k.odd));
-  return fma2(x, f.s, f.n4);
+// The four pairs of a word w of codes 0 .. 7: (0, 4) / 16, (1, 5) + (0, 4) / 16, (2, 6) / 16, (3, 7) + (2, 6) / 16, times their scales.
+// `magic` is 0x54005400 in a register: an instruction takes one constant.
+__device__ __forceinline__ void kd_numbers(uint32_t (&x)[4], uint32_t w, const Scales& f, uint32_t magic) {
+  const uint32_t high = __byte_perm(w, magic, 0x7351);  // bytes 1 and 3, each under the exponent
+  asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xea;" : "=r"(x[0]) : "r"(w), "r"(magic));
+  asm("lop3.b32 %0, %1, 0x00ff00ff, %2, 0xea;" : "=r"(x[1]) : "r"(w), "r"(magic));
+  x[0] = fma2(x[0], f.s, f.n);
+  x[1] = fma2(x[1], f.s, f.n);
+  x[2] = fma2(high & 0xff0fff0fu, f.s, f.n);
+  x[3] = fma2(high, f.s, f.n);
 }
 
 template <int HD, int NT>
 struct KDSmem {
-  static constexpr int CODES = KD_CHUNK * HD / 2;             // of keys, or of values
-  static constexpr int PARAMS = KD_CHUNK * (HD / KV4_GROUP) * 4;
+  static constexpr int CODES = KD_PIECE * HD / 2;             // of keys, or of values
+  static constexpr int PARAMS = KD_PIECE * (HD / KV4_GROUP) * 4;
   static constexpr int OFF_PK = 2 * CODES;
-  static constexpr int STAGE = 2 * CODES + 2 * PARAMS;        // a multiple of 128 bytes
+  static constexpr int STAGE = 2 * CODES + 2 * PARAMS;        // of a warp, a multiple of 128 bytes
   static constexpr int MEET = HD / 4 + 4;                     // floats of a lane: O of 8 heads, maxima and sums of weights of two
-  static constexpr int OFF_MEET = KD_WARPS * KD_STAGES * STAGE;
+  static constexpr int OFF_MEET = KD_WARPS * STAGE;
   static constexpr int OFF_BAR = OFF_MEET + 2 * 32 * MEET * 4;
-  static constexpr int TOTAL = OFF_BAR + KD_WARPS * KD_STAGES * 8;
+  static constexpr int TOTAL = OFF_BAR + KD_WARPS * 2 * 8;
 };
 
 // The sequence that piece u (over all heads) belongs to: the last one with plan[b] * nkv <= u. The whole warp searches, 32 places a round.
@@ -134,20 +125,19 @@ __device__ __forceinline__ int kd_locate(const int* plan, int B, int nkv, int u)
   return lo;
 }
 
-// Pieces of everything and of a CTA's run. The launcher sees that chunks, and tokens of a table row, are counted in 31 bits.
+// Pieces of everything and of a CTA's run. The launcher sees that pieces, and tokens of a table row, are counted in 31 bits.
 __device__ __forceinline__ int kd_total(const VbKv4Decode& p) {
   return min(max(p.plan[p.B], 0), p.B * ((p.width * p.block_size + KD_PIECE - 1) / KD_PIECE)) * p.nkv;
 }
 __device__ __forceinline__ int kd_per(int total, int ctas) { return max(KD_MIN_PIECES, (total + ctas - 1) / ctas); }
 __device__ __forceinline__ int kd_len(const VbKv4Decode& p, int b) { return min(max(p.ctx[b], 0), p.width * p.block_size); }
 
-// One (sequence, head), in chunks: two to a piece, the second one of a context's last piece may be empty.
+// One (sequence, head).
 struct KDSegment {
-  int b, kvh, base, end, len;  // its chunks in the numbering over everything, its tokens
+  int b, kvh, base, end, len;  // its pieces in the numbering over everything, its tokens
   __device__ __forceinline__ void find(const VbKv4Decode& p, int u) {
-    const int f = p.nkv * KD_PER_PIECE;
-    while (b + 1 < p.B && p.plan[b + 1] * f <= u) ++b;
-    const int at = p.plan[b] * f, n = max(p.plan[b + 1] - p.plan[b], 1) * KD_PER_PIECE;
+    while (b + 1 < p.B && p.plan[b + 1] * p.nkv <= u) ++b;
+    const int at = p.plan[b] * p.nkv, n = max(p.plan[b + 1] - p.plan[b], 1);
     kvh = min(max(u - at, 0) / n, p.nkv - 1);
     base = at + kvh * n;
     end = max(base + n, u + 1);
@@ -178,74 +168,76 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
   constexpr int CPR = HD / 4, VPR = HD / 8, KW = CPR / 8, VW = VPR / 8;  // channels of a thread's run, and words of them
   extern __shared__ __align__(16) uint8_t smem[];  // 16 bytes are what bulk copies ask for
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.nh / p.nkv, bs = p.block_size;
-  uint8_t* ring = smem + warp * KD_STAGES * L::STAGE;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR) + warp * KD_STAGES;
+  uint8_t* stage = smem + warp * L::STAGE;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR) + warp * 2;  // keys are there, values are there
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int total = kd_total(p), per = kd_per(total, gridDim.x);
   if (static_cast<long long>(blockIdx.x) * per >= total) return;
-  const int u0 = blockIdx.x * per * KD_PER_PIECE, u1 = min(total, static_cast<int>(blockIdx.x + 1) * per) * KD_PER_PIECE;  // this CTA's chunks
+  const int u0 = blockIdx.x * per, u1 = min(total, static_cast<int>(blockIdx.x + 1) * per);  // this CTA's pieces
   if (lane == 0) {
-    for (int s = 0; s < KD_STAGES; ++s) mbar_init(&full[s], 1);
+    mbar_init(&full[0], 1);
+    mbar_init(&full[1], 1);
     mbar_fence_init();
   }
   __syncwarp();
 
-  // ---- loading. Lanes 8 j .. 8 j + 7 look up and fetch the j-th of the warp's next four chunks: four lanes a page (keys' codes, values' codes,
-  // keys' parameters, values' parameters), one page or two a chunk
-  const int tokens = min(bs, KD_CHUNK), page = (lane >> 2) & 1, what = lane & 3;
+  // ---- loading. Lanes 16 j .. 16 j + 15 look up and fetch the j-th of the warp's next two pieces: four lanes a page (keys' codes, values'
+  // codes, keys' parameters, values' parameters), one, two or four pages a piece
+  const int tokens = min(bs, KD_PIECE), page = (lane >> 2) & 3, what = lane & 3;
   const uint32_t row = what < 2 ? HD / 2 : (HD / KV4_GROUP) * 4, bytes = tokens * row;
   const int dst_off = (what < 2 ? what * L::CODES : L::OFF_PK + (what - 2) * L::PARAMS) + page * bytes;
   const int src_off = what < 2 ? kv4_codes_at(bs, HD, what) : kv4_params_at(bs, HD, what - 2);
-  KDSegment ahead;  // of the chunk that this lane looks up
-  ahead.b = kd_locate(p.plan, p.B, p.nkv, u0 / KD_PER_PIECE);
+  KDSegment ahead;  // of the piece that this lane looks up
+  ahead.b = kd_locate(p.plan, p.B, p.nkv, u0);
   KDSegment g;
   g.b = ahead.b;
   g.end = u0;
   ahead.end = u0;
   const uint8_t* src = nullptr;  // what this lane fetches (null: nothing)
   bool missing = false;          // of a page that does not exist
-  const auto look = [&](int u) {  // chunk u is the first of the four; the answer is used a chunk later
-    u += (lane >> 3) * KD_WARPS;
+  const auto look = [&](int u) {  // piece u is the first of the two; the answer is used half a piece later
+    u += (lane >> 4) * KD_WARPS;
     src = nullptr;
     missing = false;
-    if (u >= u1 || page * tokens >= KD_CHUNK) return;
+    if (u >= u1 || page * tokens >= KD_PIECE) return;
     if (u >= ahead.end) ahead.find(p, u);
-    const int tok = (u - ahead.base) * KD_CHUNK + page * tokens;
+    const int tok = (u - ahead.base) * KD_PIECE + page * tokens;
     if (tok < 0 || tok >= ahead.len) return;
     const int blk = p.table[ahead.b * p.ldt + (tok >> block_shift)];
     missing = blk < 0 || blk >= p.num_blocks;
     if (!missing)
       src = p.pages + (static_cast<long long>(blk) * p.nkv + ahead.kvh) * kv4_page_bytes(bs, HD) + src_off + (tok & (bs - 1)) * row;
   };
-  const auto load = [&](int j, int s) {  // the j-th of the four into stage s; returns the pages of it that do not exist (bits 0 and 4)
-    const bool mine = (lane >> 3) == j;
-    const uint32_t copies = __ballot_sync(0xffffffffu, mine && src != nullptr && what == 0);
-    const uint32_t gone = __ballot_sync(0xffffffffu, mine && missing && what == 0);
-    if (lane == 0) mbar_expect_tx(&full[s], __popc(copies) * tokens * (HD + HD / 4));
+  const auto load = [&](int j, int value) {  // keys or values of the j-th of the two; returns the pages of it that do not exist (bits 0, 4, 8, 12)
+    const bool mine = (lane >> 4) == j && (what & 1) == value;
+    const uint32_t copies = __ballot_sync(0xffffffffu, mine && src != nullptr && what < 2), gone = __ballot_sync(0xffffffffu, mine && missing && what < 2);
+    if (lane == 0) mbar_expect_tx(&full[value], __popc(copies) * tokens * (HD / 2 + HD / 8));
     __syncwarp();
-    if (mine && src != nullptr) bulk_load(ring + s * L::STAGE + dst_off, src, bytes, &full[s]);
-    return gone >> (8 * j);
+    if (mine && src != nullptr) bulk_load(stage + dst_off, src, bytes, &full[value]);
+    return (gone >> (16 * j)) >> value;
   };
-  uint32_t lost[KD_STAGES] = {};
+  uint32_t lost = 0, lost_next = 0;
   look(u0 + warp);
-#pragma unroll
-  for (int s = 0; s < KD_STAGES; ++s)
-    if (u0 + warp + s * KD_WARPS < u1) lost[s] = load(s, s);
-  int looked = KD_STAGES;  // the next of the four
+  if (u0 + warp < u1) {
+    lost_next = load(0, 0);
+    load(0, 1);
+  }
+  int looked = 1;  // the next of the two
 
   // ---- computing
   const int r = lane >> 2, c = lane & 3;
   const int krow = (r & 1) * 4 + (r >> 1);  // row r of S^T is this token of the first 8 of 16, row r + 8 the same of the others: a thread's
                                             // share of V^T (rows 2c, 2c + 1, 2c + 8, 2c + 9) is then tokens c, c + 4, c + 8, c + 12
   float* meet = reinterpret_cast<float*>(smem + L::OFF_MEET);
-  const Magic magic;
-  int u = u0 + warp, stage_at = 0;  // this warp's next chunk and its stage
+  uint32_t magic;
+  asm volatile("mov.b32 %0, 0x54005400;" : "=r"(magic));
+  int u = u0 + warp;  // this warp's next piece
   uint32_t round = 0;
   bool ok = true;
   for (int seg = u0; seg < u1;) {
     g.find(p, seg);
     const int seg_end = min(u1, g.end);
-    uint32_t qf[NT][KW][4], qs[NT];  // a word's four pairs of channels (0, 4), (1, 5), (2, 6), (3, 7); the run's sum / 16 in two halves
+    uint32_t qf[NT][KW][4], qs[NT];  // per word of 8 channels: 16 q - q' and q' for (0, 4), (1, 5), (2, 6), (3, 7); the run's sum in two halves
     float o[NT][HD / 16][4], z[NT][4], m[NT][2], l[NT][2], sc[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -268,23 +260,25 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
       for (int j = 0; j < CPR; ++j) big = fmaxf(big, fabsf(x[j]));
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-      // largest magnitude into [2^10, 2^11): fp16 then holds all 11 bits of what is at least 2^-24 of it, and the sum of 32 channels
+      // largest magnitude into [2^9, 2^10): fp16 then holds all 11 bits of what is at least 2^-23 of it, 16 q - q', and the sum of 32 channels
       const int e = max(static_cast<int>(__float_as_uint(big) >> 23) - 127, -100);
-      const float f = copysignf(__uint_as_float(static_cast<uint32_t>(10 - e + 127) << 23), p.scale);
+      const float f = copysignf(__uint_as_float(static_cast<uint32_t>(9 - e + 127) << 23), p.scale);
 #pragma unroll
       for (int j = 0; j < CPR; ++j) {
         x[j] *= f;
         sum += x[j];
       }
-      sum *= 0.0625f;
 #pragma unroll
       for (int w = 0; w < KW; ++w)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) qf[t][w][j] = pack2(x[w * 8 + j], x[w * 8 + j + 4]);
+        for (int j = 0; j < 4; j += 2) {
+          qf[t][w][j] = pack2(fmaf(16.f, x[w * 8 + j], -x[w * 8 + j + 1]), fmaf(16.f, x[w * 8 + j + 4], -x[w * 8 + j + 5]));
+          qf[t][w][j + 1] = pack2(x[w * 8 + j + 1], x[w * 8 + j + 5]);
+        }
       const float hi = __half2float(__float2half_rn(sum));
       qs[t] = pack2(hi, sum - hi);
       // not zero, so that -inf stays what it is under it
-      const float back = fmaxf(fabsf(p.scale) * (16.f * 1.4426950408889634f) * __uint_as_float(static_cast<uint32_t>(e - 10 + 127) << 23), 1e-37f);
+      const float back = fmaxf(fabsf(p.scale) * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(e - 9 + 127) << 23), 1e-37f);
       sc[t][0] = __shfl_sync(0xffffffffu, back, 8 * c);
       sc[t][1] = __shfl_sync(0xffffffffu, back, 8 * c + 4);
       m[t][0] = m[t][1] = -INFINITY;
@@ -293,24 +287,23 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
 #pragma unroll
       for (int i = 0; i < HD / 16; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
     }
-    for (; u < seg_end; u += KD_WARPS) {
-      const uint8_t* stage = ring + stage_at * L::STAGE;
-      const int next = u + KD_STAGES * KD_WARPS;
-      if (looked == 4) {
+    for (; u < seg_end; u += KD_WARPS, ++round) {
+      const int next = u + KD_WARPS;
+      if (looked == 2) {
         looked = 0;
         if (next < u1) look(next);
       }
+      lost = lost_next;
       if (ok) {
-        ok = __all_sync(0xffffffffu, kd_wait(&full[stage_at], round & 1));
-        if (!ok)  // no more work, the barriers only; what is in flight gets another while to land
-          for (int s = 0; s < KD_STAGES; ++s) kd_wait(&full[s], (round + (s < stage_at)) & 1);
+        ok = __all_sync(0xffffffffu, kd_wait(&full[0], round & 1));
+        if (!ok) kd_wait(&full[1], round & 1);  // no more work, the barriers only; what is in flight gets another while to land
       }
-      const int left = min(g.len - (u - g.base) * KD_CHUNK, KD_CHUNK);  // tokens that count
-      if (ok && left > 0) {
-        const uint32_t gone = lost[0];
-        const bool ragged = left < KD_CHUNK || gone != 0;
-        // does token i of the chunk count?
-        const auto counts = [&](int i) { return i < left && !((gone >> (4 * (i / tokens))) & 1u); };
+      const int left = min(g.len - (u - g.base) * KD_PIECE, KD_PIECE);  // tokens that count
+      const bool work = ok && left > 0, ragged = left < KD_PIECE || lost != 0;
+      // does token i of the piece count?
+      const auto counts = [&](int i) { return i < left && !((lost >> (4 * (i / tokens))) & 1u); };
+      uint32_t pb[NT][KD_TILES][2];
+      if (work) {
         const uint8_t* kc = stage + krow * (HD / 2) + c * (CPR / 2);
         const uint8_t* kp = stage + L::OFF_PK + (krow * (HD / KV4_GROUP) + c * CPR / KV4_GROUP) * 4;
         float st[NT][KD_TILES][4];
@@ -337,17 +330,18 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
           }
 #pragma unroll
           for (int w = 0; w < KW; ++w) {
-            const uint32_t a = wk[0][w], b = wk[1][w], a8 = a >> 8, b8 = b >> 8;
-            const uint32_t a0 = codes_even(a, f0, magic), a1 = codes_even(b, f1, magic), a2 = codes_odd(a, f0, magic), a3 = codes_odd(b, f1, magic);
-            const uint32_t b0 = codes_even(a8, f0, magic), b1 = codes_even(b8, f1, magic), b2 = codes_odd(a8, f0, magic), b3 = codes_odd(b8, f1, magic);
+            uint32_t a[4], b[4];
+            kd_numbers(a, wk[0][w], f0, magic);
+            kd_numbers(b, wk[1][w], f1, magic);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-              mma_f16_16816(st[t][i], a0, a1, a2, a3, qf[t][w][0], qf[t][w][1]);
-              mma_f16_16816(st[t][i], b0, b1, b2, b3, qf[t][w][2], qf[t][w][3]);
+              mma_f16_16816(st[t][i], a[0], b[0], a[1], b[1], qf[t][w][0], qf[t][w][1]);
+              mma_f16_16816(st[t][i], a[2], b[2], a[3], b[3], qf[t][w][2], qf[t][w][3]);
             }
           }
         }
-        uint32_t pb[NT][KD_TILES][2];
+        __syncwarp();
+        if (next < u1) lost_next = load(looked, 0);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           float top[2];
@@ -400,6 +394,14 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
             pb[t][i][1] = movmatrix_t(pack2(st[t][i][2], st[t][i][3]));
           }
         }
+      } else if (ok && next < u1) {
+        lost_next = load(looked, 0);
+      }
+      if (ok) {
+        ok = __all_sync(0xffffffffu, kd_wait(&full[1], round & 1));
+        if (!ok && next < u1) kd_wait(&full[0], (round + 1) & 1);
+      }
+      if (ok && left > 0) {
         // values: this thread's run of channels of four tokens at a time
         const uint8_t* vc = stage + L::CODES + c * (HD / 2) + r * (VPR / 2);
         const uint8_t* vp = stage + L::OFF_PK + L::PARAMS + (c * (HD / KV4_GROUP) + r * VPR / KV4_GROUP) * 4;
@@ -431,28 +433,24 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
 #pragma unroll
             for (int half = 0; half < 2; ++half) {  // channels 0..3 and 4..7 of the word: a pair of tokens side by side
               const uint32_t sel = half == 0 ? 0x5410 : 0x7632;
-              const uint32_t x = __byte_perm(wv[0][w], wv[1][w], sel), y = __byte_perm(wv[2][w], wv[3][w], sel), x8 = x >> 8, y8 = y >> 8;
-              const uint32_t a0 = codes_even(x, f01, magic), a1 = codes_odd(x, f01, magic), a2 = codes_even(y, f23, magic), a3 = codes_odd(y, f23, magic);
-              const uint32_t b0 = codes_even(x8, f01, magic), b1 = codes_odd(x8, f01, magic), b2 = codes_even(y8, f23, magic), b3 = codes_odd(y8, f23, magic);
+              uint32_t x[4], y[4];
+              kd_numbers(x, __byte_perm(wv[0][w], wv[1][w], sel), f01, magic);
+              kd_numbers(y, __byte_perm(wv[2][w], wv[3][w], sel), f23, magic);
 #pragma unroll
               for (int t = 0; t < NT; ++t) {
-                mma_f16_16816(o[t][w * 4 + half * 2], a0, a1, a2, a3, pb[t][i][0], pb[t][i][1]);
-                mma_f16_16816(o[t][w * 4 + half * 2 + 1], b0, b1, b2, b3, pb[t][i][0], pb[t][i][1]);
+                mma_f16_16816(o[t][w * 4 + half * 2], x[0], x[1], y[0], y[1], pb[t][i][0], pb[t][i][1]);
+                mma_f16_16816(o[t][w * 4 + half * 2 + 1], x[2], x[3], y[2], y[3], pb[t][i][0], pb[t][i][1]);
               }
             }
         }
       }
       __syncwarp();
-      lost[0] = lost[1];
-      if (ok && next < u1) lost[1] = load(looked, stage_at);
+      if (ok && next < u1) load(looked, 1);
       ++looked;
-      if (++stage_at == KD_STAGES) {
-        stage_at = 0;
-        ++round;
-      }
     }
 
-    // ---- end of a segment: warps 1 and 3 hand their sums to 0 and 2, then 2 to 0, lane by lane. O^T[channel r VPR + 2 i (+ 1), head] = 16 o + z
+    // ---- end of a segment: warps 1 and 3 hand their sums to 0 and 2, then 2 to 0, lane by lane.
+    // O^T[channel r VPR + 2 i, head] = 16 o + z, and the channel behind it o' - o + z
     const bool whole = seg == g.base && seg_end == g.end;
     float* part = p.part + (2LL * blockIdx.x + (seg == u0 ? 0 : 1)) * G * (HD + 4);
 #pragma unroll
@@ -466,8 +464,8 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
         sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 16);
 #pragma unroll
         for (int i = 0; i < HD / 16; ++i) {
+          o[t][i][2 + h] = o[t][i][2 + h] - o[t][i][h] + z[t][h];
           o[t][i][h] = fmaf(16.f, o[t][i][h], z[t][h]);
-          o[t][i][2 + h] = fmaf(16.f, o[t][i][2 + h], z[t][h]);
         }
       }
 #pragma unroll
@@ -662,7 +660,7 @@ extern "C" int vb_kv4_decode(const VbKv4Decode* a, cudaStream_t s) {
   if (a->B == 0) return 0;
   if ((a->hd != 64 && a->hd != 128) || a->nh % a->nkv || a->nh / a->nkv > 16 || a->B > 65535 || (a->block_size & (a->block_size - 1)) || a->block_size < 16) return -2;
   const long long tokens = static_cast<long long>(a->width) * a->block_size;
-  if (tokens > 1LL << 30 || ((tokens + KD_PIECE - 1) / KD_PIECE) * KD_PER_PIECE * a->B * a->nkv > 0x7fffffffLL) return -4;  // counted in 31 bits
+  if (tokens > 1LL << 30 || (tokens + KD_PIECE - 1) / KD_PIECE * a->B * a->nkv > 0x7fffffffLL) return -4;  // counted in 31 bits
   VbKv4Decode p = *a;
   int* status = nullptr;
   cudaError_t e = cudaGetSymbolAddress(reinterpret_cast<void**>(&status), g_kv4_status);
