@@ -145,8 +145,8 @@ Tensor paged_decode_kv4(const Tensor& q, const Tensor& pages, const Tensor& tabl
   TORCH_CHECK((bs & (bs - 1)) == 0 && bs <= 256, "paged_decode_kv4: blocks of 16, 32, 64, 128 or 256 tokens, got ", bs);
   check_table(table, "paged_decode_kv4");
   TORCH_CHECK(table.size(0) == B && pages.size(0) <= INT_MAX && B <= 65535, "paged_decode_kv4: one table row for each of at most 65535 sequences");
-  TORCH_CHECK(table.size(1) * bs <= (1LL << 30) && (table.size(1) * bs + 63) / 64 * 2 * B * nkv <= INT_MAX, "paged_decode_kv4: a table of ", B, " x ",
-              table.size(1), " blocks of ", bs, " is more than the kernel counts in 31 bits");
+  TORCH_CHECK(table.size(1) * bs <= (1LL << 30) && (table.size(1) * bs + 63) / 64 * B * nkv <= (1LL << 30) - 1, "paged_decode_kv4: a table of ", B, " x ",
+              table.size(1), " blocks of ", bs, " is more than the kernel counts in 30 bits");
   check_vec(ctx, at::kInt, B, q, "paged_decode_kv4: ctx_len");
   if (plan.has_value()) check_vec(*plan, at::kInt, B + 1, q, "paged_decode_kv4: plan");
   const c10::cuda::CUDAGuard guard(q.device());

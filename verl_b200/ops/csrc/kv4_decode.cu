@@ -1,13 +1,12 @@
 // Attention of one query token per sequence over the 4-bit cache (layout: kv4_common.cuh): one pass over the codes, running maximum and sum.
 //
-// Work: contexts are cut into pieces of 64 tokens; the pieces of all (sequence, KV head) pairs, laid end to end, are dealt to the CTAs of one
-// wave in equal runs, whatever the lengths are (the plan holds the pieces in front of every sequence). A CTA that starts or ends inside a
+// Work: contexts are cut into pieces of 64 tokens; the pieces of all (sequence, KV head) pairs, laid end to end, are dealt to the warps of one
+// wave in equal runs, whatever the lengths are (the plan holds the pieces in front of every sequence). A warp that starts or ends inside a
 // (sequence, head) leaves its sums in a slot of its own, and a second small launch, started early by programmatic dependence, joins them
 // by their maxima, in the order of the runs: no atomics, the same bits every time.
 //
-// A CTA: its four warps take pieces in turn. Each has room for the keys and the values of one piece, which it fills by bulk copies (a half is at
-// most 8 contiguous runs, two for blocks of 64 and more): the next keys while it works on values, the next values while it works on keys. No
-// warp waits for another until the end of a segment, where their sums meet in pairs, fragment by fragment.
+// No warp waits for another. Each has room for the keys and the values of one piece, which it fills by bulk copies (a half is at most 8
+// contiguous runs, two for blocks of 64 and more): the next keys while it works on values, the next values while it works on keys.
 //   S^T[64 tokens, 8 heads] = K[64, hd] Q^T        keys are the A operand of m16n8k16: a thread's share of a token's row is one contiguous run
 //   O^T[hd, 8 heads]       += V^T[hd, 64] P^T      values are the A operand as well; P^T is S^T's accumulator through movmatrix
 // so that with up to 8 heads to a KV head a matrix instruction takes 256 cache elements (query heads as the 16 rows would take 128).
@@ -36,7 +35,7 @@ constexpr int KD_WARPS = 4;
 constexpr int KD_THREADS = KD_WARPS * 32;
 constexpr int KD_TILES = KD_PIECE / 16;
 __host__ __device__ constexpr int kd_ctas(int nt) { return nt == 1 ? 4 : 3; }  // CTAs of an SM: what registers and shared memory hold
-constexpr int KD_MIN_PIECES = 4;                 // shortest run of a CTA
+constexpr int KD_MIN_PIECES = 2;                 // shortest run of a warp
 
 __device__ int g_kv4_status[4];
 
@@ -104,9 +103,7 @@ struct KDSmem {
   static constexpr int PARAMS = KD_PIECE * (HD / KV4_GROUP) * 4;
   static constexpr int OFF_PK = 2 * CODES;
   static constexpr int STAGE = 2 * CODES + 2 * PARAMS;        // of a warp, a multiple of 128 bytes
-  static constexpr int MEET = HD / 4 + 4;                     // floats of a lane: O of 8 heads, maxima and sums of weights of two
-  static constexpr int OFF_MEET = KD_WARPS * STAGE;
-  static constexpr int OFF_BAR = OFF_MEET + 2 * 32 * MEET * 4;
+  static constexpr int OFF_BAR = KD_WARPS * STAGE;
   static constexpr int TOTAL = OFF_BAR + KD_WARPS * 2 * 8;
 };
 
@@ -125,11 +122,11 @@ __device__ __forceinline__ int kd_locate(const int* plan, int B, int nkv, int u)
   return lo;
 }
 
-// Pieces of everything and of a CTA's run. The launcher sees that pieces, and tokens of a table row, are counted in 31 bits.
+// Pieces of everything and of a run. The launcher sees that pieces, and tokens of a table row, are counted in 31 bits.
 __device__ __forceinline__ int kd_total(const VbKv4Decode& p) {
   return min(max(p.plan[p.B], 0), p.B * ((p.width * p.block_size + KD_PIECE - 1) / KD_PIECE)) * p.nkv;
 }
-__device__ __forceinline__ int kd_per(int total, int ctas) { return max(KD_MIN_PIECES, (total + ctas - 1) / ctas); }
+__device__ __forceinline__ int kd_per(int total, int runs) { return max(KD_MIN_PIECES, (total + runs - 1) / runs); }
 __device__ __forceinline__ int kd_len(const VbKv4Decode& p, int b) { return min(max(p.ctx[b], 0), p.width * p.block_size); }
 
 // One (sequence, head).
@@ -171,9 +168,9 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
   uint8_t* stage = smem + warp * L::STAGE;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR) + warp * 2;  // keys are there, values are there
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int total = kd_total(p), per = kd_per(total, gridDim.x);
-  if (static_cast<long long>(blockIdx.x) * per >= total) return;
-  const int u0 = blockIdx.x * per, u1 = min(total, static_cast<int>(blockIdx.x + 1) * per);  // this CTA's pieces
+  const int run = blockIdx.x * KD_WARPS + warp, total = kd_total(p), per = kd_per(total, gridDim.x * KD_WARPS);
+  if (static_cast<long long>(run) * per >= total) return;
+  const int u0 = run * per, u1 = min(total - u0, per) + u0;  // this warp's pieces
   if (lane == 0) {
     mbar_init(&full[0], 1);
     mbar_init(&full[1], 1);
@@ -196,7 +193,7 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
   const uint8_t* src = nullptr;  // what this lane fetches (null: nothing)
   bool missing = false;          // of a page that does not exist
   const auto look = [&](int u) {  // piece u is the first of the two; the answer is used half a piece later
-    u += (lane >> 4) * KD_WARPS;
+    u += lane >> 4;
     src = nullptr;
     missing = false;
     if (u >= u1 || page * tokens >= KD_PIECE) return;
@@ -217,24 +214,21 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
     return (gone >> (16 * j)) >> value;
   };
   uint32_t lost = 0, lost_next = 0;
-  look(u0 + warp);
-  if (u0 + warp < u1) {
-    lost_next = load(0, 0);
-    load(0, 1);
-  }
+  look(u0);
+  lost_next = load(0, 0);
+  load(0, 1);
   int looked = 1;  // the next of the two
 
   // ---- computing
   const int r = lane >> 2, c = lane & 3;
   const int krow = (r & 1) * 4 + (r >> 1);  // row r of S^T is this token of the first 8 of 16, row r + 8 the same of the others: a thread's
                                             // share of V^T (rows 2c, 2c + 1, 2c + 8, 2c + 9) is then tokens c, c + 4, c + 8, c + 12
-  float* meet = reinterpret_cast<float*>(smem + L::OFF_MEET);
   uint32_t magic;
   asm volatile("mov.b32 %0, 0x54005400;" : "=r"(magic));
-  int u = u0 + warp;  // this warp's next piece
-  uint32_t round = 0;
+  uint32_t round = 0;  // pieces that were here
   bool ok = true;
-  for (int seg = u0; seg < u1;) {
+  for (int u = u0; u < u1;) {
+    const int seg = u;
     g.find(p, seg);
     const int seg_end = min(u1, g.end);
     uint32_t qf[NT][KW][4], qs[NT];  // per word of 8 channels: 16 q - q' and q' for (0, 4), (1, 5), (2, 6), (3, 7); the run's sum in two halves
@@ -287,8 +281,8 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
 #pragma unroll
       for (int i = 0; i < HD / 16; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
     }
-    for (; u < seg_end; u += KD_WARPS, ++round) {
-      const int next = u + KD_WARPS;
+    for (; u < seg_end; ++u, ++round) {
+      const int next = u + 1;
       if (looked == 2) {
         looked = 0;
         if (next < u1) look(next);
@@ -296,7 +290,7 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
       lost = lost_next;
       if (ok) {
         ok = __all_sync(0xffffffffu, kd_wait(&full[0], round & 1));
-        if (!ok) kd_wait(&full[1], round & 1);  // no more work, the barriers only; what is in flight gets another while to land
+        if (!ok) kd_wait(&full[1], round & 1);  // no more work; what is in flight gets another while to land
       }
       const int left = min(g.len - (u - g.base) * KD_PIECE, KD_PIECE);  // tokens that count
       const bool work = ok && left > 0, ragged = left < KD_PIECE || lost != 0;
@@ -449,134 +443,108 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
       ++looked;
     }
 
-    // ---- end of a segment: warps 1 and 3 hand their sums to 0 and 2, then 2 to 0, lane by lane.
-    // O^T[channel r VPR + 2 i, head] = 16 o + z, and the channel behind it o' - o + z
+    // ---- end of a segment. O^T[channel r VPR + 2 i, head] = 16 o + z, and the channel behind it o' - o + z
     const bool whole = seg == g.base && seg_end == g.end;
-    float* part = p.part + (2LL * blockIdx.x + (seg == u0 ? 0 : 1)) * G * (HD + 4);
+    float* part = p.part + (2LL * run + (seg == u0 ? 0 : 1)) * G * (HD + 4);
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      float sum[2];
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        sum[h] = l[t][h];
-        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 4);
-        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 8);
-        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 16);
+        float sum = l[t][h];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        const int head = t * 8 + 2 * c + h;
+        if (head >= G) continue;
+        float x[VPR];
 #pragma unroll
         for (int i = 0; i < HD / 16; ++i) {
-          o[t][i][2 + h] = o[t][i][2 + h] - o[t][i][h] + z[t][h];
-          o[t][i][h] = fmaf(16.f, o[t][i][h], z[t][h]);
+          x[2 * i] = fmaf(16.f, o[t][i][h], z[t][h]);
+          x[2 * i + 1] = o[t][i][2 + h] - o[t][i][h] + z[t][h];
+        }
+        if (whole) {
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          T* out = static_cast<T*>(p.out) + (static_cast<long long>(g.b) * p.nh + g.kvh * G + head) * HD + r * VPR;
+#pragma unroll
+          for (int i = 0; i < VPR; i += 8) {
+            uint4 v;
+            T* e = reinterpret_cast<T*>(&v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) e[j] = static_cast<T>(x[i + j] * inv);
+            *reinterpret_cast<uint4*>(out + i) = v;
+          }
+        } else {
+          float* to = part + head * (HD + 4);
+#pragma unroll
+          for (int i = 0; i < VPR; i += 4) *reinterpret_cast<float4*>(to + r * VPR + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+          if (r == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(m[t][h], sum);
         }
       }
-#pragma unroll
-      for (int step = 1; step < KD_WARPS; step *= 2) {
-        float4* mine = reinterpret_cast<float4*>(meet + (step == 1 ? warp >> 1 : 0) * 32 * L::MEET) + lane;  // float4 i of lane: 32 i + lane
-        if ((warp & (2 * step - 1)) == step) {
-#pragma unroll
-          for (int i = 0; i < HD / 16; ++i) mine[32 * i] = make_float4(o[t][i][0], o[t][i][1], o[t][i][2], o[t][i][3]);
-          mine[32 * (HD / 16)] = make_float4(m[t][0], m[t][1], sum[0], sum[1]);
-        }
-        __syncthreads();
-        if ((warp & (2 * step - 1)) == 0) {
-          const float4 other = mine[32 * (HD / 16)];
-          float fa[2], fb[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float mo = h == 0 ? other.x : other.y, M = fmaxf(m[t][h], mo), mu = M == -INFINITY ? 0.f : M;
-            fa[h] = fast_exp2(m[t][h] - mu);
-            fb[h] = fast_exp2(mo - mu);
-            m[t][h] = M;
-            sum[h] = sum[h] * fa[h] + (h == 0 ? other.z : other.w) * fb[h];
-          }
-#pragma unroll
-          for (int i = 0; i < HD / 16; ++i) {
-            const float4 v = mine[32 * i];
-            o[t][i][0] = o[t][i][0] * fa[0] + v.x * fb[0];
-            o[t][i][1] = o[t][i][1] * fa[1] + v.y * fb[1];
-            o[t][i][2] = o[t][i][2] * fa[0] + v.z * fb[0];
-            o[t][i][3] = o[t][i][3] * fa[1] + v.w * fb[1];
-          }
-        }
-        if (step * 2 < KD_WARPS || NT > 1) __syncthreads();  // what was handed over is read
-      }
-      if (warp == 0) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int head = t * 8 + 2 * c + h;
-          if (head >= G) continue;
-          if (whole) {
-            const float inv = sum[h] == 0.f ? 0.f : 1.f / sum[h];
-            T* out = static_cast<T*>(p.out) + (static_cast<long long>(g.b) * p.nh + g.kvh * G + head) * HD + r * VPR;
-#pragma unroll
-            for (int i = 0; i < HD / 16; i += 4) {
-              uint4 v;
-              T* e = reinterpret_cast<T*>(&v);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                e[2 * j] = static_cast<T>(o[t][i + j][h] * inv);
-                e[2 * j + 1] = static_cast<T>(o[t][i + j][2 + h] * inv);
-              }
-              *reinterpret_cast<uint4*>(out + 2 * i) = v;
-            }
-          } else {
-            float* to = part + head * (HD + 4);
-#pragma unroll
-            for (int i = 0; i < HD / 16; i += 2)
-              *reinterpret_cast<float4*>(to + r * VPR + 2 * i) = make_float4(o[t][i][h], o[t][i][2 + h], o[t][i + 1][h], o[t][i + 1][2 + h]);
-            if (r == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(m[t][h], sum[h]);
-          }
-        }
-      }
-    }
-    if (NT == 1) __syncthreads();
-    seg = seg_end;
   }
   if (!ok && lane == 0) atomicExch(status, ST_TIMEOUT_EPILOGUE);
 }
 
-// Joins the runs of every (sequence, head) that more than one CTA worked on, and writes zeros for contexts of no tokens.
+// Joins the runs of every (sequence, head) that more than one warp worked on, and writes zeros for contexts of no tokens. A block per
+// (sequence, KV head): four channels a thread, what threads are left share the runs and meet in shared memory.
+struct KDSum {
+  float m, s;
+  float4 x;
+  __device__ __forceinline__ void add(float mo, float so, float4 v) {
+    const float M = fmaxf(m, mo), mu = M == -INFINITY ? 0.f : M, fa = fast_exp2(m - mu), fb = fast_exp2(mo - mu);
+    m = M;
+    s = s * fa + so * fb;
+    x.x = x.x * fa + v.x * fb;
+    x.y = x.y * fa + v.y * fb;
+    x.z = x.z * fa + v.z * fb;
+    x.w = x.w * fa + v.w * fb;
+  }
+};
+
 template <int HD, typename T>
-__global__ void __launch_bounds__(HD)
-kv4_join_kernel(const VbKv4Decode p, int ctas) {
-  __shared__ float red[HD / 32];
-  __shared__ float wgt[HD];
-  const int b = blockIdx.y, h = blockIdx.x, G = p.nh / p.nkv, kvh = h / G, head = h % G;
-  const int total = kd_total(p), per = kd_per(total, ctas), n = p.plan[b + 1] - p.plan[b];
-  T* out = static_cast<T*>(p.out) + (static_cast<long long>(b) * p.nh + h) * HD + threadIdx.x;
+__global__ void __launch_bounds__(1024)
+kv4_join_kernel(const VbKv4Decode p, int runs) {
+  extern __shared__ __align__(16) KDSum sums[];  // one a thread
+  const int b = blockIdx.y, kvh = blockIdx.x, G = p.nh / p.nkv;
+  const int total = kd_total(p), per = kd_per(total, runs), n = p.plan[b + 1] - p.plan[b];
+  T* out = static_cast<T*>(p.out) + (static_cast<long long>(b) * p.nh + kvh * G) * HD;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the runs' sums, and what came before them
+  const auto store = [&](int at, float4 v) {
+    T e[4] = {static_cast<T>(v.x), static_cast<T>(v.y), static_cast<T>(v.z), static_cast<T>(v.w)};
+    *reinterpret_cast<uint2*>(out + at * 4) = *reinterpret_cast<const uint2*>(e);
+  };
+  const int lanes = G * HD / 4, groups = max(1, static_cast<int>(blockDim.x) / lanes), group = threadIdx.x / lanes;
   if (n <= 0 || kd_len(p, b) == 0) {
-    *out = static_cast<T>(0.f);
+    for (int at = threadIdx.x; at < lanes; at += blockDim.x) store(at, make_float4(0.f, 0.f, 0.f, 0.f));
     return;
   }
-  const int base = p.plan[b] * p.nkv + kvh * n, i0 = max(base, 0) / per, i1 = min((base + n - 1) / per, ctas - 1);
+  const int base = p.plan[b] * p.nkv + kvh * n, i0 = max(base, 0) / per, i1 = min((base + n - 1) / per, runs - 1);
   if (i0 >= i1) return;
-  const auto slot = [&](int i) { return p.part + ((2LL * i + (i * per >= base ? 0 : 1)) * G + head) * (HD + 4); };
-  float M = -INFINITY;
-  for (int i = i0 + threadIdx.x; i <= i1; i += HD) M = fmaxf(M, slot(i)[HD]);
-#pragma unroll
-  for (int k = 16; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = M;
-  __syncthreads();
-  M = red[0];
-#pragma unroll
-  for (int w = 1; w < HD / 32; ++w) M = fmaxf(M, red[w]);
-  float acc = 0.f, sum = 0.f;
-  for (int at = i0; at <= i1; at += HD) {
-    const int k = min(HD, i1 - at + 1);
-    __syncthreads();
-    if (threadIdx.x < k) {
-      const float mi = slot(at + threadIdx.x)[HD];
-      wgt[threadIdx.x] = mi == -INFINITY ? 0.f : fast_exp2(mi - M);
+  for (int at0 = 0; at0 < lanes; at0 += blockDim.x) {  // more than once for more channels than threads, with one group then
+    const int at = at0 + static_cast<int>(threadIdx.x) - (groups > 1 ? group * lanes : 0), head = at / (HD / 4), d = at % (HD / 4) * 4;
+    KDSum a{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+    if (group < groups && at < lanes) {
+      const auto slot = [&](int i) { return p.part + ((2LL * i + (i * per >= base ? 0 : 1)) * G + head) * (HD + 4); };
+#pragma unroll 4
+      for (int i = i0 + (groups > 1 ? group : 0); i <= i1; i += groups) {
+        const float* s = slot(i);
+        const float2 ms = *reinterpret_cast<const float2*>(s + HD);
+        a.add(ms.x, ms.y, *reinterpret_cast<const float4*>(s + d));
+      }
     }
-    __syncthreads();
-#pragma unroll 8
-    for (int i = 0; i < k; ++i) {
-      const float* s = slot(at + i);
-      acc += wgt[i] * s[threadIdx.x];
-      sum += wgt[i] * s[HD + 1];
+    if (groups > 1) {
+      sums[threadIdx.x] = a;
+      __syncthreads();
+      if (group == 0)
+        for (int k = 1; k < groups; ++k) {
+          const KDSum o = sums[threadIdx.x + k * lanes];
+          a.add(o.m, o.s, o.x);
+        }
+    }
+    if (at < lanes && (groups == 1 || group == 0)) {
+      const float inv = a.s == 0.f ? 0.f : 1.f / a.s;
+      store(at, make_float4(a.x.x * inv, a.x.y * inv, a.x.z * inv, a.x.w * inv));
     }
   }
-  *out = static_cast<T>(sum == 0.f ? 0.f : acc / sum);
 }
 
 // Pieces in front of every sequence, for calls without a plan.
@@ -622,12 +590,15 @@ static cudaError_t kd_launch(const VbKv4Decode& p, int* status, cudaStream_t s) 
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(p.nh, p.B);
-  cfg.blockDim = dim3(HD);
+  // a block per (sequence, KV head); many runs to each are shared by more threads
+  const int runs = ctas * KD_WARPS, threads = runs / (p.B * p.nkv) >= 16 ? 1024 : 256;
+  cfg.gridDim = dim3(p.nkv, p.B);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = threads * sizeof(KDSum);
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<HD, T>, p, ctas);
+  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<HD, T>, p, runs);
 }
 
 template <typename T>
@@ -643,7 +614,7 @@ using namespace vb;
 
 extern "C" long long vb_kv4_decode_scratch(int B, int nh, int nkv, int hd) {
   const int G = nh / nkv;
-  return 2LL * num_sms() * kd_ctas(G <= 8 ? 1 : 2) * G * (hd + 4);
+  return 2LL * num_sms() * kd_ctas(G <= 8 ? 1 : 2) * KD_WARPS * G * (hd + 4);
 }
 
 extern "C" int vb_kv4_status() {
@@ -660,7 +631,7 @@ extern "C" int vb_kv4_decode(const VbKv4Decode* a, cudaStream_t s) {
   if (a->B == 0) return 0;
   if ((a->hd != 64 && a->hd != 128) || a->nh % a->nkv || a->nh / a->nkv > 16 || a->B > 65535 || (a->block_size & (a->block_size - 1)) || a->block_size < 16) return -2;
   const long long tokens = static_cast<long long>(a->width) * a->block_size;
-  if (tokens > 1LL << 30 || (tokens + KD_PIECE - 1) / KD_PIECE * a->B * a->nkv > 0x7fffffffLL) return -4;  // counted in 31 bits
+  if (tokens > 1LL << 30 || (tokens + KD_PIECE - 1) / KD_PIECE * a->B * a->nkv > 0x3fffffffLL) return -4;  // counted in 31 bits
   VbKv4Decode p = *a;
   int* status = nullptr;
   cudaError_t e = cudaGetSymbolAddress(reinterpret_cast<void**>(&status), g_kv4_status);
