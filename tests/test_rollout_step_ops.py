@@ -431,6 +431,25 @@ def test_scores_of_masked_tied_and_undefined_rows(dev, V, dtype):
     assert (d[0] == 0).all() and d[4].isnan().all() and d[5].isnan().all() and d[good].isfinite().all()
 
 
+@pytest.mark.parametrize("V", [40, 30011])
+def test_rows_of_the_type_s_lowest_value_are_uniform(dev, V):
+    """A mask that is added as the type's lowest value and leaves nothing: all tokens alike, log-sum-exp at the value itself."""
+    for dtype in (torch.bfloat16, torch.float32):
+        low = torch.finfo(dtype).min
+        x = torch.full((2, V), low, dtype=dtype, device=dev)
+        x[1, 3] = 2.0
+        ids = torch.tensor([V - 1, 3], device=dev)
+        out = F.token_scores(x, ids, 4)
+        assert out.lse[0] == low and out.top_ids.tolist() == [[0, 1, 2, 3], [3, 0, 1, 2]]
+        tol = 16 * U32 * math.log(V)      # a logarithm of V ones, and their sum
+        assert abs(float(out.logprob[0]) + math.log(V)) <= tol and abs(float(out.entropy[0]) - math.log(V)) <= tol
+        assert abs(float(out.top_logprob[0, 0]) + math.log(V)) <= tol and out.logprob[1] == 0 and out.entropy[1] == 0
+        d = F.token_scores_bwd(x, ids, out.lse, out.entropy, torch.ones(2, device=dev), None).double().cpu()
+        want = torch.full((V,), -1.0 / V, dtype=torch.float64)
+        want[V - 1] += 1
+        assert ((d[0] - want).abs() <= want.abs() * (HALF[dtype] + 64 * U32)).all() and (d[1] == 0).all()
+
+
 def grad_64(logits, ids, g_lp, g_ent, temperature, valid):
     z = (logits[:, :valid].double().cpu() / temperature).requires_grad_(True)
     logp = torch.log_softmax(z, -1)

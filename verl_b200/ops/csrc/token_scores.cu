@@ -1,9 +1,19 @@
 // Scores of rows of logits: log-probs of given tokens, entropy, log-sum-exp, the most likely tokens; and the gradient of log-probs and entropy.
 //
-// With z = x / temperature and m the largest z so far, a row is read once for
-//   s = sum e^(z - m),  w = sum e^(z - m) (z - m):   lse = m + log s,  H = log s - w / s
-// and the gradient of sum_j g_j logprob_j + h H is
-//   dL/dx_v = 1/T (sum_j g_j [v = id_j] - p_v (sum_j g_j + h (log p_v + H))).
+// With y = x log2(e) / temperature and a reference M near the largest y, a row is read once for
+//   s = sum 2^(y - M),  w = sum 2^(y - M) (y - M):   lse = ln2 (M + log2 s),  H = ln2 (log2 s - w / s)
+// five instructions and one exponential a value. A thread keeps a reference of its own, which moves only when a value is 2^60 above it.
+//
+// The most likely tokens come with the same pass: every thread also keeps the largest value that it met, and the k-th largest of those of a
+// block is a bound that at least k values of the row reach. Only the columns of threads that reach it are looked at again (about k of 512
+// threads, from L2); what reaches the bound there is hardly more than k values, which are ranked by counting. Rows that this does not fit (over
+// 1024 values at the bound: a row of few different values) and rows with NaN, +inf or nothing above -1e30 take a slow path, right for any values.
+//
+// A row belongs to a cluster of 1 to 8 blocks, as many as the card holds at once; they exchange their sums, bounds and candidates through
+// distributed shared memory. The gradient needs no exchange:
+//   dL/dx_v = 1/T (sum_j g_j [v = id_j] - p_v (sum_j g_j + h (log p_v + H)))
+// is one more pass, 2^y p (a + b y) a value, with the given tokens' columns written again behind it.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -14,20 +24,90 @@
 
 namespace vb {
 
-constexpr int TS_THREADS = 256;
+namespace cg = cooperative_groups;
+int num_sms();
 
-struct Stat {
-  float m, s, w;  // largest z, sum e^(z - m), sum e^(z - m) (z - m)
-};
-__device__ __forceinline__ Stat join(Stat a, Stat b) {
-  if (!(b.s == b.s)) return b;
-  if (!(a.s == a.s)) return a;
-  const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) return {m, 0.f, 0.f};
-  const float da = a.m - m, db = b.m - m, ea = expf(da), eb = expf(db);
-  const float wa = ea > 0.f ? ea * (a.w + a.s * da) : 0.f, wb = eb > 0.f ? eb * (b.w + b.s * db) : 0.f;
-  return {m, a.s * ea + b.s * eb, wa + wb};
+constexpr int TS_THREADS = 512;
+constexpr int TS_BATCH = 4;        // 16-byte vectors of a thread in flight
+constexpr int TS_CANDIDATES = 1024;
+constexpr float TS_LOG2E = 1.4426950408889634f, TS_LN2 = 0.6931471805599453f;
+constexpr float TS_FLOOR = -200.f;  // exponents below this are zeros: keeps 0 * inf out of the sums
+
+__device__ __forceinline__ float ts_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
+__device__ __forceinline__ float ts_max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 16 bytes of a row as floats
+template <typename T> struct Lane;
+template <> struct Lane<float> {
+  static constexpr int N = 4, LOW = 0;  // values in 16 bytes, bits of a value as a float that are always zero
+  static __device__ __forceinline__ uint4 none() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+  static __device__ __forceinline__ void open(const uint4& v, float (&f)[N]) {
+    f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
+  }
+  static __device__ __forceinline__ uint4 close(const float (&f)[N]) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+};
+template <> struct Lane<__nv_bfloat16> {
+  static constexpr int N = 8, LOW = 16;
+  static __device__ __forceinline__ uint4 none() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+  static __device__ __forceinline__ void open(const uint4& v, float (&f)[N]) {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(u[i] << 16);
+      f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ uint4 close(const float (&f)[N]) {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(f[2 * i + 1]), "f"(f[2 * i]));
+    return make_uint4(u[0], u[1], u[2], u[3]);
+  }
+};
+template <> struct Lane<__half> {
+  static constexpr int N = 8, LOW = 13;
+  static __device__ __forceinline__ uint4 none() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
+  static __device__ __forceinline__ void open(const uint4& v, float (&f)[N]) {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+      f[2 * i] = a.x;
+      f[2 * i + 1] = a.y;
+    }
+  }
+  static __device__ __forceinline__ uint4 close(const float (&f)[N]) {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(f[2 * i + 1]), "f"(f[2 * i]));
+    return make_uint4(u[0], u[1], u[2], u[3]);
+  }
+};
+
+// A row cut for 16-byte accesses: `head` values up to the first boundary, `vecs` vectors, the rest.
+template <typename T>
+struct Row {
+  const T* x;
+  int V, head, vecs;
+  __device__ __forceinline__ Row(const T* row, int n) : x(row), V(n) {
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15) / static_cast<int>(sizeof(T));
+    head = min(off == 0 ? 0 : Lane<T>::N - off, n);
+    vecs = (n - head) / Lane<T>::N;
+  }
+  __device__ __forceinline__ const uint4* vec() const { return reinterpret_cast<const uint4*>(x + head); }
+  __device__ __forceinline__ int loose() const { return V - vecs * Lane<T>::N; }                            // values outside the vectors
+  __device__ __forceinline__ int loose_at(int i) const { return i < head ? i : i + vecs * Lane<T>::N; }
+};
 
 // Order of the values as whole numbers: NaN above everything, -0 with +0.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -35,84 +115,399 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   const uint32_t u = __float_as_uint(x + 0.f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+
+struct Stat {
+  float m, s, w;  // reference, sum 2^(y - m), sum 2^(y - m) (y - m)
+  __device__ __forceinline__ void move(float to) {
+    const float d = m - to, f = ts_exp2(fmaxf(d, -1e4f));
+    w = f * (w + s * fmaxf(d, -1e4f));
+    s *= f;
+    m = to;
+  }
+  __device__ __forceinline__ void add(float y) {
+    const float d = ts_max_nan(y - m, TS_FLOOR), e = ts_exp2(d);
+    s += e;
+    w = fmaf(e, d, w);
+  }
+};
+
+// The sums of all threads of a block, in every thread. `red` holds 3 x 16 floats.
+__device__ __forceinline__ Stat block_stat(Stat a, float* red) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float m = a.m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  a.move(m);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+    a.w += __shfl_xor_sync(0xffffffffu, a.w, o);
+  }
+  __syncthreads();
+  if (lane == 0) { red[warp] = a.m; red[16 + warp] = a.s; red[32 + warp] = a.w; }
+  __syncthreads();
+  constexpr int W = TS_THREADS / 32;
+  Stat b{lane < W ? red[lane] : -1e30f, lane < W ? red[16 + lane] : 0.f, lane < W ? red[32 + lane] : 0.f};
+  m = b.m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  b.move(m);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    b.s += __shfl_xor_sync(0xffffffffu, b.s, o);
+    b.w += __shfl_xor_sync(0xffffffffu, b.w, o);
+  }
+  return b;
+}
+
+__device__ __forceinline__ unsigned long long block_max(unsigned long long v, unsigned long long* red) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+  __syncthreads();
+  if (lane == 0) red[warp] = v;
+  __syncthreads();
+  v = lane < TS_THREADS / 32 ? red[lane] : 0ull;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// Log-prob of value f of a row with reference m and ls = log2 s. A value near the type's lowest is its own log-prob: log2(e) times it is not finite.
+__device__ __forceinline__ float scaled_logprob(float f, float inv_temp, float m, float ls) {
+  const float d = fmaf(f, inv_temp * TS_LOG2E, -m);
+  return d == -INFINITY ? f * inv_temp : TS_LN2 * (d - ls);
+}
+
+// Largest z = x / temperature and sum e^(z - m), sum e^(z - m) (z - m) of any row, by one block: for a row whose largest value is NaN or +inf
+// the sums are NaN, for one of nothing but -inf m is -inf.
+template <typename T>
+__device__ Stat any_stat(const T* x, int V, float inv_temp, float* red) {
+  float m = -INFINITY;
+  for (int v = threadIdx.x; v < V; v += TS_THREADS) m = ts_max_nan(m, static_cast<float>(x[v]) * inv_temp);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = ts_max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+  __syncthreads();
+  for (int i = 0; i < TS_THREADS / 32; ++i) m = ts_max_nan(m, red[i]);
+  Stat a{0.f, 0.f, 0.f};
+  if (m > -INFINITY || m != m)
+    for (int v = threadIdx.x; v < V; v += TS_THREADS) {
+      const float d = static_cast<float>(x[v]) * inv_temp - m, e = expf(d);
+      a.s += e;
+      if (e > 0.f) a.w = fmaf(e, d, a.w);
+      if (e != e) a.w = e;
+    }
+  a = block_stat(a, red);
+  a.m = m;
+  return a;
+}
+
+struct Shared {
+  float red[48];
+  Stat stat;               // of this block's part of the row
+  uint32_t bound;          // at least top values of the part have this key or a larger one (0: the part has fewer threads with values)
+  int threads, found;
+  unsigned long long wide[16];
+  uint16_t who[TS_THREADS];
+  unsigned long long list[TS_CANDIDATES];  // (key, place backwards)
+};
 
 template <typename T>
-__global__ void __launch_bounds__(TS_THREADS)
-token_scores_simple_kernel(const VbScores p) {
-  const long long t = blockIdx.x;
-  const T* x = static_cast<const T*>(p.x) + t * p.ldx;
-  __shared__ Stat red[TS_THREADS];
-  __shared__ unsigned long long best[TS_THREADS];
-  Stat a{-INFINITY, 0.f, 0.f};
-  for (int v = threadIdx.x; v < p.V; v += TS_THREADS) {
-    const float z = static_cast<float>(x[v]) * p.inv_temp;
-    a = join(a, Stat{z, z - z == 0.f || z == -INFINITY ? 1.f : NAN, 0.f});
-  }
-  red[threadIdx.x] = a;
-  __syncthreads();
-  for (int o = TS_THREADS / 2; o > 0; o >>= 1) {
-    if (threadIdx.x < o) red[threadIdx.x] = join(red[threadIdx.x], red[threadIdx.x + o]);
-    __syncthreads();
-  }
-  a = red[0];
-  const float lse = a.m == -INFINITY && a.s == a.s ? -INFINITY : a.m + logf(a.s);
-  const auto logprob = [&](float z) { return lse == -INFINITY ? -INFINITY : z - lse; };
+__device__ void scores_any(const VbScores& p, long long t, const T* x, Shared& sh) {
+  const Stat a = any_stat(x, p.V, p.inv_temp, sh.red);
+  const float ls = logf(a.s), none = -INFINITY;
+  const bool empty = a.m == -INFINITY;
+  const auto logprob = [&](float v) { return empty ? none : v * p.inv_temp - a.m - ls; };
   if (threadIdx.x == 0) {
-    p.lse[t] = lse;
-    p.entropy[t] = lse == -INFINITY ? 0.f : logf(a.s) - a.w / a.s;
+    p.lse[t] = empty ? none : a.m + ls;
+    p.entropy[t] = empty ? 0.f : ls - a.w / a.s;
   }
   for (int j = threadIdx.x; j < p.K; j += TS_THREADS) {
     const long long id = p.ids[t * p.K + j];
-    p.logprob[t * p.K + j] = id >= 0 && id < p.V ? logprob(static_cast<float>(x[id]) * p.inv_temp) : 0.f;
+    p.logprob[t * p.K + j] = id >= 0 && id < p.V ? logprob(static_cast<float>(x[id])) : 0.f;
   }
+}
+
+// The largest (value, lowest place) below the last one, `top` times over.
+template <typename T>
+__device__ void top_any(const VbScores& p, long long t, const T* x, Shared& sh, float m, float ls, bool scaled) {
   unsigned long long last = ~0ull;
-  for (int k = 0; k < p.top; ++k) {  // the largest (value, lowest place) below the last one
+  for (int k = 0; k < p.top; ++k) {
     unsigned long long b = 0;
     for (int v = threadIdx.x; v < p.V; v += TS_THREADS) {
       const unsigned long long key = (static_cast<unsigned long long>(order_key(static_cast<float>(x[v]))) << 32) | (0xffffffffu - v);
       if (key < last && key > b) b = key;
     }
-    __syncthreads();
-    best[threadIdx.x] = b;
-    __syncthreads();
-    for (int o = TS_THREADS / 2; o > 0; o >>= 1) {
-      if (threadIdx.x < o) best[threadIdx.x] = max(best[threadIdx.x], best[threadIdx.x + o]);
-      __syncthreads();
-    }
-    last = best[0];
+    last = block_max(b, sh.wide);
     if (threadIdx.x == 0) {
       const uint32_t v = 0xffffffffu - static_cast<uint32_t>(last);
+      const float f = static_cast<float>(x[v]);
       p.top_ids[t * p.top + k] = v;
-      p.top_lp[t * p.top + k] = logprob(static_cast<float>(x[v]) * p.inv_temp);
+      p.top_lp[t * p.top + k] = scaled ? scaled_logprob(f, p.inv_temp, m, ls) : m == -INFINITY ? -INFINITY : f * p.inv_temp - m - ls;
     }
-    __syncthreads();
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(TS_THREADS)
-token_scores_bwd_simple_kernel(const VbScores p, const float* g_lp, const float* g_ent, T* dx, long long lddx, int columns) {
+__global__ void __launch_bounds__(TS_THREADS, 2)
+token_scores_kernel(const VbScores p) {
+  using L = Lane<T>;
+  __shared__ Shared sh;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int parts = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
+  const long long t = blockIdx.x / parts;
+  const T* x = static_cast<const T*>(p.x) + t * p.ldx;
+  const Row<T> row(x, p.V);
+  const int per = (row.vecs + parts - 1) / parts, v0 = min(row.vecs, part * per), n = min(row.vecs, v0 + per) - v0;
+  const uint4* vec = row.vec() + v0;
+  const float c = p.inv_temp * TS_LOG2E;
+  if (threadIdx.x == 0) sh.threads = sh.found = 0;
+
+  // ---- the pass
+  Stat a{-1e30f, 0.f, 0.f};
+  float s1 = 0.f, w1 = 0.f, most = -INFINITY;
+  bool any = false;
+  for (int v = threadIdx.x; v < n; v += TS_THREADS * TS_BATCH) {
+    uint4 raw[TS_BATCH];
+#pragma unroll
+    for (int u = 0; u < TS_BATCH; ++u) raw[u] = v + u * TS_THREADS < n ? __ldg(vec + v + u * TS_THREADS) : L::none();
+    any = true;
+    float f[TS_BATCH][L::N], big = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < TS_BATCH; ++u) {
+      L::open(raw[u], f[u]);
+#pragma unroll
+      for (int i = 0; i < L::N; ++i) big = fmaxf(big, f[u][i]);
+    }
+    most = fmaxf(most, big);
+    if (big * c > a.m + 60.f) {
+      a.s += s1;
+      a.w += w1;
+      s1 = w1 = 0.f;
+      a.move(big * c);
+    }
+#pragma unroll
+    for (int u = 0; u < TS_BATCH; ++u)
+#pragma unroll
+      for (int i = 0; i < L::N; i += 2) {
+        const float d0 = ts_max_nan(fmaf(f[u][i], c, -a.m), TS_FLOOR), e0 = ts_exp2(d0);
+        const float d1 = ts_max_nan(fmaf(f[u][i + 1], c, -a.m), TS_FLOOR), e1 = ts_exp2(d1);
+        a.s += e0;
+        a.w = fmaf(e0, d0, a.w);
+        s1 += e1;
+        w1 = fmaf(e1, d1, w1);
+      }
+  }
+  const bool has_loose = part == 0 && static_cast<int>(threadIdx.x) < row.loose();
+  const int loose_at = has_loose ? row.loose_at(threadIdx.x) : 0;
+  const float loose = has_loose ? static_cast<float>(x[loose_at]) : -INFINITY;
+  a.s += s1;
+  a.w += w1;
+  if (has_loose) {
+    any = true;
+    most = fmaxf(most, loose);
+    if (loose * c > a.m + 60.f) a.move(loose * c);
+    a.add(loose * c);
+  }
+  a = block_stat(a, sh.red);
+
+  // ---- the bound: bit by bit, the largest key that `top` threads' largest values reach
+  uint32_t bound = 0;
+  const uint32_t mine = any ? order_key(most) : 0u;
+  if (p.top > 0) {
+    for (int bit = 31; bit >= L::LOW; --bit) {  // below, all keys of one sign are alike
+      const uint32_t want = bound | (1u << bit);
+      if (__syncthreads_count(mine >= want) >= p.top) bound = want;
+    }
+  }
+  if (threadIdx.x == 0) {
+    sh.stat = a;
+    sh.bound = bound;
+  }
+  if (parts > 1) {
+    cluster.sync();
+    Stat all = *cluster.map_shared_rank(&sh.stat, 0);
+    float m = all.m;
+    for (int i = 1; i < parts; ++i) m = fmaxf(m, cluster.map_shared_rank(&sh, i)->stat.m);
+    all.move(m);
+    for (int i = 1; i < parts; ++i) {
+      Stat o = cluster.map_shared_rank(&sh, i)->stat;
+      o.move(m);
+      all.s += o.s;
+      all.w += o.w;
+    }
+    for (int i = 0; i < parts; ++i) bound = max(bound, cluster.map_shared_rank(&sh, i)->bound);
+    a = all;
+  } else {
+    __syncthreads();
+  }
+  const bool odd = !(a.s > 0.f && a.s < INFINITY && fabsf(a.m) < 1e30f);  // NaN, +inf, or nothing that the reference can be compared with
+
+  // ---- what reaches the bound, into the first block's list
+  Shared* first = parts > 1 ? cluster.map_shared_rank(&sh, 0) : &sh;
+  if (p.top > 0 && !odd) {
+    const float limit = bound <= order_key(-INFINITY) ? -INFINITY : key_value(bound);
+    if (any && mine >= bound) sh.who[atomicAdd(&sh.threads, 1)] = static_cast<uint16_t>(threadIdx.x);
+    __syncthreads();
+    const int lane = threadIdx.x & 31, who = sh.threads, rounds = (n + TS_THREADS - 1) / TS_THREADS;
+    const auto put = [&](float f, int at) {
+      const int k = atomicAdd(&first->found, 1);
+      if (k < TS_CANDIDATES) first->list[k] = (static_cast<unsigned long long>(order_key(f)) << 32) | (0xffffffffu - at);
+    };
+    for (int j = threadIdx.x >> 5; j < who; j += TS_THREADS / 32)
+      for (int q = lane; q < rounds; q += 32) {
+        const int v = q * TS_THREADS + sh.who[j];
+        if (v >= n) continue;
+        float f[L::N];
+        L::open(__ldg(vec + v), f);
+#pragma unroll
+        for (int i = 0; i < L::N; ++i)
+          if (f[i] >= limit) put(f[i], row.head + (v0 + v) * L::N + i);
+      }
+    if (has_loose && loose >= limit) put(loose, loose_at);
+  }
+  if (parts > 1) cluster.sync(); else __syncthreads();
+  if (part != 0) return;
+
+  if (odd) {
+    scores_any(p, t, x, sh);
+    __syncthreads();
+    if (p.top > 0) {
+      const Stat b = any_stat(x, p.V, p.inv_temp, sh.red);
+      top_any(p, t, x, sh, b.m, logf(b.s), false);
+    }
+    return;
+  }
+  const float ls = log2f(a.s);
+  if (threadIdx.x == 0) {
+    p.lse[t] = TS_LN2 * (a.m + ls);
+    p.entropy[t] = TS_LN2 * (ls - a.w / a.s);
+  }
+  for (int j = threadIdx.x; j < p.K; j += TS_THREADS) {
+    const long long id = p.ids[t * p.K + j];
+    p.logprob[t * p.K + j] = id >= 0 && id < p.V ? scaled_logprob(static_cast<float>(x[id]), p.inv_temp, a.m, ls) : 0.f;
+  }
+  if (p.top == 0) return;
+  const int found = sh.found;
+  if (found > TS_CANDIDATES || found < p.top) {
+    top_any(p, t, x, sh, a.m, ls, true);
+    return;
+  }
+  for (int i = threadIdx.x; i < found; i += TS_THREADS) {
+    const unsigned long long key = sh.list[i];
+    int rank = 0;
+    for (int j = 0; j < found; ++j) rank += sh.list[j] > key;
+    if (rank < p.top) {
+      const uint32_t v = 0xffffffffu - static_cast<uint32_t>(key);
+      p.top_ids[t * p.top + rank] = v;
+      p.top_lp[t * p.top + rank] = scaled_logprob(static_cast<float>(x[v]), p.inv_temp, a.m, ls);
+    }
+  }
+}
+
+// ---- gradient: blockIdx.x is the row, blockIdx.y one of gridDim.y parts of its columns
+template <typename T>
+__global__ void __launch_bounds__(TS_THREADS, 2)
+token_scores_bwd_kernel(const VbScores p, const float* __restrict__ g_lp, const float* __restrict__ g_ent, T* __restrict__ dx, long long lddx, int columns) {
+  using L = Lane<T>;
+  __shared__ Shared sh;
   const long long t = blockIdx.x;
   const T* x = static_cast<const T*>(p.x) + t * p.ldx;
   T* d = dx + t * lddx;
   const float lse = p.lse[t], H = p.entropy[t], h = g_ent != nullptr ? g_ent[t] : 0.f;
-  float g = 0.f;
-  for (int j = 0; j < p.K; ++j) {
-    const long long id = p.ids[t * p.K + j];
-    if (id >= 0 && id < p.V) g += g_lp[t * p.K + j];
+  const long long* ids = p.ids + t * p.K;
+  const float* gl = g_lp + t * p.K;
+  Stat gs{0.f, 0.f, 0.f};
+  for (int j = threadIdx.x; j < p.K; j += TS_THREADS)
+    if (ids[j] >= 0 && ids[j] < p.V) gs.s += gl[j];
+  const float g = block_stat(gs, sh.red).s;
+  // log2 p = x c - m - ls
+  float m = lse * TS_LOG2E, ls = 0.f, c = p.inv_temp * TS_LOG2E;
+  bool apart = false;
+  if (fabsf(lse) > 1e5f && lse > -INFINITY) {  // too large to hold log s as well: both again, and the differences before they are scaled
+    const Stat b = any_stat(x, p.V, p.inv_temp, sh.red);
+    m = b.m;
+    ls = logf(b.s) * TS_LOG2E;
+    apart = true;
   }
-  const auto slope = [&](int v, float extra) {
-    const float lp = static_cast<float>(x[v]) * p.inv_temp - lse;
-    if (lse == -INFINITY) return 0.f;
-    const float pv = expf(lp);
-    return p.inv_temp * (extra - (pv == 0.f ? 0.f : pv * (g + h * (lp + H))));
+  const bool empty = lse == -INFINITY;
+  const float a0 = -p.inv_temp * (g + h * H), a1 = -p.inv_temp * h * TS_LN2;
+  const auto slope = [&](float f) {
+    const float y = ts_max_nan(apart ? (f * p.inv_temp - m) * TS_LOG2E - ls : fmaf(f, c, -m), TS_FLOOR);
+    return empty ? 0.f : ts_exp2(y) * fmaf(a1, y, a0);
   };
-  for (int v = threadIdx.x; v < columns; v += TS_THREADS) {
-    float extra = 0.f;
-    for (int j = 0; j < p.K; ++j)
-      if (p.ids[t * p.K + j] == v) extra += g_lp[t * p.K + j];
-    d[v] = static_cast<T>(v < p.V ? slope(v, extra) : 0.f);
+  // vectors where the row and its gradient lie alike
+  const Row<T> row(x, p.V);
+  const bool alike = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0;
+  const int head = alike ? row.head : 0, vecs = alike ? row.vecs : 0;
+  const int per = (vecs + gridDim.y - 1) / gridDim.y, v0 = min(vecs, static_cast<int>(blockIdx.y) * per), v1 = min(vecs, v0 + per);
+  const uint4* from = reinterpret_cast<const uint4*>(x + head);
+  uint4* to = reinterpret_cast<uint4*>(d + head);
+  for (int v = v0 + threadIdx.x; v < v1; v += TS_THREADS * TS_BATCH) {
+    uint4 raw[TS_BATCH];
+#pragma unroll
+    for (int u = 0; u < TS_BATCH; ++u) raw[u] = v + u * TS_THREADS < v1 ? __ldg(from + v + u * TS_THREADS) : L::none();
+#pragma unroll
+    for (int u = 0; u < TS_BATCH; ++u) {
+      float f[L::N];
+      L::open(raw[u], f);
+#pragma unroll
+      for (int i = 0; i < L::N; ++i) f[i] = slope(f[i]);
+      if (v + u * TS_THREADS < v1) to[v + u * TS_THREADS] = L::close(f);
+    }
   }
+  // the columns outside the vectors, and those that do not count: the last part's
+  const int behind = head + vecs * L::N;
+  if (blockIdx.y == gridDim.y - 1) {
+    for (int v = threadIdx.x; v < head; v += TS_THREADS) d[v] = static_cast<T>(slope(static_cast<float>(x[v])));
+    for (int v = behind + threadIdx.x; v < columns; v += TS_THREADS) d[v] = static_cast<T>(v < p.V ? slope(static_cast<float>(x[v])) : 0.f);
+  }
+  __syncthreads();
+  // the given tokens: a token's first place in the list gathers all its gradients, in their order
+  for (int j = threadIdx.x; j < p.K; j += TS_THREADS) {
+    const long long id = ids[j];
+    if (id < 0 || id >= p.V) continue;
+    const int in_vec = id >= head && id < behind ? (static_cast<int>(id) - head) / L::N : -1;
+    if (in_vec >= 0 ? in_vec < v0 || in_vec >= v1 : blockIdx.y != gridDim.y - 1) continue;
+    float sum = 0.f;
+    bool earlier = false;
+    for (int i = 0; i < p.K; ++i)
+      if (ids[i] == id) {
+        earlier |= i < j;
+        sum += gl[i];
+      }
+    if (!earlier && !empty) d[id] = static_cast<T>(fmaf(p.inv_temp, sum, slope(static_cast<float>(x[id]))));
+  }
+}
+
+template <typename T>
+static cudaError_t ts_forward(const VbScores& a, cudaStream_t s) {
+  // as many blocks to a row as the card holds at once (two an SM), with at least 1024 vectors for each
+  int parts = 1;
+  while (parts < 8 && 2LL * parts * a.T <= 2LL * num_sms() && a.V / Lane<T>::N >= 2048 * parts) parts *= 2;
+  if (static_cast<long long>(a.T) * parts > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = parts;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(a.T * parts);
+  cfg.blockDim = dim3(TS_THREADS);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, token_scores_kernel<T>, a);
+}
+
+template <typename T>
+static cudaError_t ts_backward(const VbScores& a, const float* g_lp, const float* g_ent, void* dx, long long lddx, int columns, cudaStream_t s) {
+  int parts = 1;
+  while (parts < 32 && 2LL * parts * a.T <= 2LL * num_sms() && a.V / Lane<T>::N >= 2048 * parts) parts *= 2;
+  token_scores_bwd_kernel<T><<<dim3(a.T, parts), TS_THREADS, 0, s>>>(a, g_lp, g_ent, static_cast<T*>(dx), lddx, columns);
+  return cudaGetLastError();
 }
 
 }  // namespace vb
@@ -121,18 +516,14 @@ using namespace vb;
 
 extern "C" int vb_token_scores(const VbScores* a, cudaStream_t s) {
   if (a->T == 0) return 0;
-  if (a->type == 0) token_scores_simple_kernel<__nv_bfloat16><<<a->T, TS_THREADS, 0, s>>>(*a);
-  else if (a->type == 1) token_scores_simple_kernel<__half><<<a->T, TS_THREADS, 0, s>>>(*a);
-  else token_scores_simple_kernel<float><<<a->T, TS_THREADS, 0, s>>>(*a);
   verl_count_launches(1);
-  return static_cast<int>(cudaGetLastError());
+  return static_cast<int>(a->type == 0 ? ts_forward<__nv_bfloat16>(*a, s) : a->type == 1 ? ts_forward<__half>(*a, s) : ts_forward<float>(*a, s));
 }
 
 extern "C" int vb_token_scores_bwd(const VbScores* a, const float* g_lp, const float* g_ent, void* dx, long long lddx, int columns, cudaStream_t s) {
   if (a->T == 0 || columns == 0) return 0;
-  if (a->type == 0) token_scores_bwd_simple_kernel<<<a->T, TS_THREADS, 0, s>>>(*a, g_lp, g_ent, static_cast<__nv_bfloat16*>(dx), lddx, columns);
-  else if (a->type == 1) token_scores_bwd_simple_kernel<<<a->T, TS_THREADS, 0, s>>>(*a, g_lp, g_ent, static_cast<__half*>(dx), lddx, columns);
-  else token_scores_bwd_simple_kernel<<<a->T, TS_THREADS, 0, s>>>(*a, g_lp, g_ent, static_cast<float*>(dx), lddx, columns);
   verl_count_launches(1);
-  return static_cast<int>(cudaGetLastError());
+  return static_cast<int>(a->type == 0   ? ts_backward<__nv_bfloat16>(*a, g_lp, g_ent, dx, lddx, columns, s)
+                          : a->type == 1 ? ts_backward<__half>(*a, g_lp, g_ent, dx, lddx, columns, s)
+                                         : ts_backward<float>(*a, g_lp, g_ent, dx, lddx, columns, s));
 }

@@ -955,7 +955,7 @@ def token_scores(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0, temper
     s = e.sum(-1, keepdim=True)
     lse = m + torch.log(s)
     ent = torch.where(empty, 0.0, torch.log(s) - torch.where(e == 0, 0.0, e * (z - m)).sum(-1, keepdim=True) / s)
-    score = lambda at: torch.where(empty, float("-inf"), z.gather(1, at) - lse)
+    score = lambda at: torch.where(empty, float("-inf"), z.gather(1, at) - m - torch.log(s))
     ok = (flat >= 0) & (flat < V)
     lp = torch.where(ok, score(flat.clamp(0, V - 1)), 0.0)
     top = torch.sort(x, dim=-1, descending=True, stable=True).indices[:, : int(top_k)]
@@ -976,7 +976,7 @@ def token_scores_bwd(logits: torch.Tensor, ids: torch.Tensor, lse: torch.Tensor,
         return _ops().token_scores_bwd(x, flat.contiguous(), lse.contiguous(), entropy.contiguous(), g.contiguous(),
                                        g_entropy.float().contiguous() if g_entropy is not None else None, float(temperature), V)
     inv = 1.0 / float(temperature)
-    logp = logits[:, :V].float() * inv - lse[:, None]
+    logp = torch.log_softmax(logits[:, :V].float() * inv, -1)
     p = torch.exp(logp)
     g = torch.where((flat >= 0) & (flat < V), g, 0.0)
     slope = g.sum(-1, keepdim=True)
