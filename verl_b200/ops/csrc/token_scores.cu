@@ -9,10 +9,11 @@
 // threads, from L2); what reaches the bound there is hardly more than k values, which are ranked by counting. Rows that this does not fit (over
 // 1024 values at the bound: a row of few different values) and rows with NaN, +inf or nothing above -1e30 take a slow path, right for any values.
 //
-// A row belongs to a cluster of 1 to 8 blocks, as many as the card holds at once; they exchange their sums, bounds and candidates through
-// distributed shared memory. The gradient needs no exchange:
+// Blocks stay for many rows. One warp of a block brings the rows into a ring of shared memory by bulk copies, so that the next row is on its way
+// while the block ranks the last one. Where rows are few, a row belongs to a cluster of up to 8 blocks, which exchange their sums, bounds and
+// candidates through distributed shared memory. The gradient needs no exchange:
 //   dL/dx_v = 1/T (sum_j g_j [v = id_j] - p_v (sum_j g_j + h (log p_v + H)))
-// is one more pass, 2^y p (a + b y) a value, with the given tokens' columns written again behind it.
+// is one more pass, 2^y (a + b y) a value, with the given tokens' columns written again behind it.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -21,14 +22,18 @@
 #include <stdint.h>
 
 #include "rollout_ops.h"
+#include "tcgen05_common.cuh"
 
 namespace vb {
 
 namespace cg = cooperative_groups;
 int num_sms();
 
-constexpr int TS_THREADS = 512;
-constexpr int TS_BATCH = 4;        // 16-byte vectors of a thread in flight
+constexpr int TS_THREADS = 512;    // that compute
+constexpr int TS_BATCH = 4;        // 16-byte vectors of a thread in flight (gradient)
+constexpr int TS_STAGES = 3;
+constexpr int TS_PER = 4;                      // 16-byte vectors of a thread in a stage
+constexpr int TS_CHUNK = TS_PER * TS_THREADS;  // vectors of a stage: 32 KB
 constexpr int TS_CANDIDATES = 1024;
 constexpr float TS_LOG2E = 1.4426950408889634f, TS_LN2 = 0.6931471805599453f;
 constexpr float TS_FLOOR = -200.f;  // exponents below this are zeros: keeps 0 * inf out of the sums
@@ -37,6 +42,15 @@ __device__ __forceinline__ float ts_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ int g_ts_status[4];
+
+// barrier of the threads that compute
+__device__ __forceinline__ void ts_sync() { asm volatile("bar.sync 1, %0;" ::"n"(TS_THREADS) : "memory"); }
+__device__ __forceinline__ int ts_count(bool p) {
+  int n;
+  asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %1, 0;\nbarrier.cta.red.popc.aligned.u32 %0, 1, %2, q;\n}\n" : "=r"(n) : "r"(static_cast<uint32_t>(p)), "n"(TS_THREADS) : "memory");
+  return n;
 }
 __device__ __forceinline__ float ts_max_nan(float a, float b) {
   float r;
@@ -56,6 +70,14 @@ template <> struct Lane<float> {
     return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
   }
 };
+// The larger of two pairs of 16-bit floats, by their bits: right where either is not negative, and negative (by its sign bit) where neither is.
+__device__ __forceinline__ uint32_t pair_max(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.s16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t pair_max(const uint4& v) { return pair_max(pair_max(v.x, v.y), pair_max(v.z, v.w)); }
+
 template <> struct Lane<__nv_bfloat16> {
   static constexpr int N = 8, LOW = 16;
   static __device__ __forceinline__ uint4 none() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
@@ -144,9 +166,9 @@ __device__ __forceinline__ Stat block_stat(Stat a, float* red) {
     a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
     a.w += __shfl_xor_sync(0xffffffffu, a.w, o);
   }
-  __syncthreads();
+  ts_sync();
   if (lane == 0) { red[warp] = a.m; red[16 + warp] = a.s; red[32 + warp] = a.w; }
-  __syncthreads();
+  ts_sync();
   constexpr int W = TS_THREADS / 32;
   Stat b{lane < W ? red[lane] : -1e30f, lane < W ? red[16 + lane] : 0.f, lane < W ? red[32 + lane] : 0.f};
   m = b.m;
@@ -165,9 +187,9 @@ __device__ __forceinline__ unsigned long long block_max(unsigned long long v, un
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
+  ts_sync();
   if (lane == 0) red[warp] = v;
-  __syncthreads();
+  ts_sync();
   v = lane < TS_THREADS / 32 ? red[lane] : 0ull;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -188,9 +210,9 @@ __device__ Stat any_stat(const T* x, int V, float inv_temp, float* red) {
   for (int v = threadIdx.x; v < V; v += TS_THREADS) m = ts_max_nan(m, static_cast<float>(x[v]) * inv_temp);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = ts_max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-  __syncthreads();
+  ts_sync();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
-  __syncthreads();
+  ts_sync();
   for (int i = 0; i < TS_THREADS / 32; ++i) m = ts_max_nan(m, red[i]);
   Stat a{0.f, 0.f, 0.f};
   if (m > -INFINITY || m != m)
@@ -212,7 +234,7 @@ struct Shared {
   int threads, found;
   unsigned long long wide[16];
   uint16_t who[TS_THREADS];
-  unsigned long long list[TS_CANDIDATES];  // (key, place backwards)
+  __align__(16) unsigned long long list[TS_CANDIDATES];  // (key, place backwards)
 };
 
 template <typename T>
@@ -252,160 +274,252 @@ __device__ void top_any(const VbScores& p, long long t, const T* x, Shared& sh, 
 }
 
 template <typename T>
-__global__ void __launch_bounds__(TS_THREADS, 2)
-token_scores_kernel(const VbScores p) {
+__device__ __forceinline__ void bulk_row(void* dst, const T* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+
+template <typename T>
+__global__ void __launch_bounds__(TS_THREADS + 32, 2)
+token_scores_kernel(const VbScores p, int* status) {
   using L = Lane<T>;
+  extern __shared__ __align__(16) uint4 ring[];  // TS_STAGES x TS_CHUNK
   __shared__ Shared sh;
+  __shared__ uint64_t full[TS_STAGES], empty[TS_STAGES];
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
-  const long long t = blockIdx.x / parts;
-  const T* x = static_cast<const T*>(p.x) + t * p.ldx;
-  const Row<T> row(x, p.V);
-  const int per = (row.vecs + parts - 1) / parts, v0 = min(row.vecs, part * per), n = min(row.vecs, v0 + per) - v0;
-  const uint4* vec = row.vec() + v0;
+  const int t0 = blockIdx.x / parts, dt = gridDim.x / parts;  // rows of this cluster: with several parts, one
   const float c = p.inv_temp * TS_LOG2E;
-  if (threadIdx.x == 0) sh.threads = sh.found = 0;
-
-  // ---- the pass
-  Stat a{-1e30f, 0.f, 0.f};
-  float s1 = 0.f, w1 = 0.f, most = -INFINITY;
-  bool any = false;
-  for (int v = threadIdx.x; v < n; v += TS_THREADS * TS_BATCH) {
-    uint4 raw[TS_BATCH];
-#pragma unroll
-    for (int u = 0; u < TS_BATCH; ++u) raw[u] = v + u * TS_THREADS < n ? __ldg(vec + v + u * TS_THREADS) : L::none();
-    any = true;
-    float f[TS_BATCH][L::N], big = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < TS_BATCH; ++u) {
-      L::open(raw[u], f[u]);
-#pragma unroll
-      for (int i = 0; i < L::N; ++i) big = fmaxf(big, f[u][i]);
-    }
-    most = fmaxf(most, big);
-    if (big * c > a.m + 60.f) {
-      a.s += s1;
-      a.w += w1;
-      s1 = w1 = 0.f;
-      a.move(big * c);
-    }
-#pragma unroll
-    for (int u = 0; u < TS_BATCH; ++u)
-#pragma unroll
-      for (int i = 0; i < L::N; i += 2) {
-        const float d0 = ts_max_nan(fmaf(f[u][i], c, -a.m), TS_FLOOR), e0 = ts_exp2(d0);
-        const float d1 = ts_max_nan(fmaf(f[u][i + 1], c, -a.m), TS_FLOOR), e1 = ts_exp2(d1);
-        a.s += e0;
-        a.w = fmaf(e0, d0, a.w);
-        s1 += e1;
-        w1 = fmaf(e1, d1, w1);
-      }
-  }
-  const bool has_loose = part == 0 && static_cast<int>(threadIdx.x) < row.loose();
-  const int loose_at = has_loose ? row.loose_at(threadIdx.x) : 0;
-  const float loose = has_loose ? static_cast<float>(x[loose_at]) : -INFINITY;
-  a.s += s1;
-  a.w += w1;
-  if (has_loose) {
-    any = true;
-    most = fmaxf(most, loose);
-    if (loose * c > a.m + 60.f) a.move(loose * c);
-    a.add(loose * c);
-  }
-  a = block_stat(a, sh.red);
-
-  // ---- the bound: bit by bit, the largest key that `top` threads' largest values reach
-  uint32_t bound = 0;
-  const uint32_t mine = any ? order_key(most) : 0u;
-  if (p.top > 0) {
-    for (int bit = 31; bit >= L::LOW; --bit) {  // below, all keys of one sign are alike
-      const uint32_t want = bound | (1u << bit);
-      if (__syncthreads_count(mine >= want) >= p.top) bound = want;
-    }
-  }
   if (threadIdx.x == 0) {
-    sh.stat = a;
-    sh.bound = bound;
-  }
-  if (parts > 1) {
-    cluster.sync();
-    Stat all = *cluster.map_shared_rank(&sh.stat, 0);
-    float m = all.m;
-    for (int i = 1; i < parts; ++i) m = fmaxf(m, cluster.map_shared_rank(&sh, i)->stat.m);
-    all.move(m);
-    for (int i = 1; i < parts; ++i) {
-      Stat o = cluster.map_shared_rank(&sh, i)->stat;
-      o.move(m);
-      all.s += o.s;
-      all.w += o.w;
+    for (int i = 0; i < TS_STAGES; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], TS_THREADS / 32);
     }
-    for (int i = 0; i < parts; ++i) bound = max(bound, cluster.map_shared_rank(&sh, i)->bound);
-    a = all;
-  } else {
-    __syncthreads();
+    mbar_fence_init();
   }
-  const bool odd = !(a.s > 0.f && a.s < INFINITY && fabsf(a.m) < 1e30f);  // NaN, +inf, or nothing that the reference can be compared with
+  __syncthreads();
 
-  // ---- what reaches the bound, into the first block's list
-  Shared* first = parts > 1 ? cluster.map_shared_rank(&sh, 0) : &sh;
-  if (p.top > 0 && !odd) {
-    const float limit = bound <= order_key(-INFINITY) ? -INFINITY : key_value(bound);
-    if (any && mine >= bound) sh.who[atomicAdd(&sh.threads, 1)] = static_cast<uint16_t>(threadIdx.x);
-    __syncthreads();
-    const int lane = threadIdx.x & 31, who = sh.threads, rounds = (n + TS_THREADS - 1) / TS_THREADS;
-    const auto put = [&](float f, int at) {
-      const int k = atomicAdd(&first->found, 1);
-      if (k < TS_CANDIDATES) first->list[k] = (static_cast<unsigned long long>(order_key(f)) << 32) | (0xffffffffu - at);
-    };
-    for (int j = threadIdx.x >> 5; j < who; j += TS_THREADS / 32)
-      for (int q = lane; q < rounds; q += 32) {
-        const int v = q * TS_THREADS + sh.who[j];
-        if (v >= n) continue;
+  if (threadIdx.x >= TS_THREADS) {
+    // ---- the warp that loads
+    if (threadIdx.x == TS_THREADS) {
+      bool ok = true;
+      long long k = 0;
+      for (int t = t0; t < p.T && ok; t += dt) {
+        const Row<T> row(static_cast<const T*>(p.x) + t * p.ldx, p.V);
+        const int per = (row.vecs + parts - 1) / parts, v0 = min(row.vecs, part * per), n = min(row.vecs, v0 + per) - v0;
+        for (int v = 0; v < n && ok; v += TS_CHUNK, ++k) {
+          const int s = static_cast<int>(k % TS_STAGES);
+          if (k >= TS_STAGES) ok = mbar_wait(&empty[s], static_cast<uint32_t>((k / TS_STAGES - 1) & 1));
+          if (!ok) break;
+          const uint32_t bytes = min(TS_CHUNK, n - v) * 16;
+          mbar_expect_tx(&full[s], bytes);
+          bulk_row(ring + s * TS_CHUNK, row.vec() + v0 + v, bytes, &full[s]);
+        }
+      }
+      if (!ok) atomicExch(status, ST_TIMEOUT_PRODUCER);
+      for (long long i = max(k - TS_STAGES, 0LL); i < k; ++i) mbar_wait(&full[i % TS_STAGES], static_cast<uint32_t>((i / TS_STAGES) & 1));  // no copy outlives the block
+    }
+    return;
+  }
+
+  bool ok = true;
+  int stage = 0;
+  uint32_t round = 0;
+  for (int t = t0; t < p.T; t += dt) {
+    const T* x = static_cast<const T*>(p.x) + t * p.ldx;
+    const Row<T> row(x, p.V);
+    const int per = (row.vecs + parts - 1) / parts, v0 = min(row.vecs, part * per), n = min(row.vecs, v0 + per) - v0;
+    const uint4* vec = row.vec() + v0;
+    if (threadIdx.x == 0) sh.threads = sh.found = 0;
+    // the value of this thread's given token, on its way during the pass
+    const long long id0 = part == 0 && static_cast<int>(threadIdx.x) < p.K ? p.ids[static_cast<long long>(t) * p.K + threadIdx.x] : -1;
+    const T given = x[id0 >= 0 && id0 < p.V ? id0 : 0];
+
+    // ---- the pass
+    Stat a{-1e30f, 0.f, 0.f};
+    float most = -INFINITY;
+    for (int v = 0; v < n; v += TS_CHUNK) {
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], round & 1));
+      const uint4* at = ring + stage * TS_CHUNK + threadIdx.x;
+      const int left = n - v - static_cast<int>(threadIdx.x);
+      // The vectors are read from shared memory for the maximum and again for the sums: held in between, they would not fit the registers.
+      float big = -INFINITY;
+      if constexpr (sizeof(T) == 2) {
+        uint32_t top = 0x80008000u;
+#pragma unroll
+        for (int u = 0; u < TS_PER; ++u)
+          if (left > u * TS_THREADS) top = pair_max(top, pair_max(at[u * TS_THREADS]));
+        top = pair_max(top, top >> 16 | 0x80000000u) & 0xffffu;
+        if (top < 0x8000u) big = static_cast<float>(*reinterpret_cast<const T*>(&top));
+      }
+      if (big == -INFINITY)  // 32-bit values, or nothing that is not negative (NaN left aside)
+#pragma unroll
+        for (int u = 0; u < TS_PER; ++u) {
+          float f[L::N];
+          L::open(left > u * TS_THREADS ? at[u * TS_THREADS] : L::none(), f);
+#pragma unroll
+          for (int i = 0; i < L::N; i += 2) big = fmaxf(big, fmaxf(f[i], f[i + 1]));
+        }
+      most = fmaxf(most, big);
+      if (big * c > a.m + 60.f) a.move(big * c);
+      float s0 = a.s, s1 = 0.f, w0 = a.w, w1 = 0.f;
+#pragma unroll
+      for (int u = 0; u < TS_PER; ++u) {
+        if (left <= u * TS_THREADS) break;
         float f[L::N];
-        L::open(__ldg(vec + v), f);
+        L::open(at[u * TS_THREADS], f);
 #pragma unroll
-        for (int i = 0; i < L::N; ++i)
-          if (f[i] >= limit) put(f[i], row.head + (v0 + v) * L::N + i);
+        for (int i = 0; i < L::N; i += 2) {
+          const float d0 = fmaf(f[i], c, -a.m), e0 = ts_exp2(d0), d1 = fmaf(f[i + 1], c, -a.m), e1 = ts_exp2(d1);
+          s0 += e0;
+          w0 = fmaf(e0, d0, w0);
+          s1 += e1;
+          w1 = fmaf(e1, d1, w1);
+        }
       }
-    if (has_loose && loose >= limit) put(loose, loose_at);
-  }
-  if (parts > 1) cluster.sync(); else __syncthreads();
-  if (part != 0) return;
+      if (w0 + w1 == w0 + w1) {
+        a.s = s0 + s1;
+        a.w = w0 + w1;
+      } else {  // 0 * -inf got into the sums: again with a floor under the exponents
+#pragma unroll 1
+        for (int u = 0; u < TS_PER; ++u) {
+          if (left <= u * TS_THREADS) break;
+          float f[L::N];
+          L::open(at[u * TS_THREADS], f);
+#pragma unroll
+          for (int i = 0; i < L::N; ++i) a.add(fmaf(f[i], c, 0.f));
+        }
+      }
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(&empty[stage]);
+      if (++stage == TS_STAGES) {
+        stage = 0;
+        ++round;
+      }
+    }
+    const bool has_loose = part == 0 && static_cast<int>(threadIdx.x) < row.loose();
+    const int loose_at = has_loose ? row.loose_at(threadIdx.x) : 0;
+    const float loose = has_loose ? static_cast<float>(x[loose_at]) : -INFINITY;
+    const bool any = has_loose || static_cast<int>(threadIdx.x) < n;
+    if (has_loose) {
+      most = fmaxf(most, loose);
+      if (loose * c > a.m + 60.f) a.move(loose * c);
+      a.add(loose * c);
+    }
+    a = block_stat(a, sh.red);
 
-  if (odd) {
-    scores_any(p, t, x, sh);
-    __syncthreads();
+    // ---- the bound: bit by bit, the largest key that `top` threads' largest values reach
+    uint32_t bound = 0;
+    const uint32_t mine = any ? order_key(most) : 0u;
+    if (p.top > 0)
+      for (int bit = 31; bit >= L::LOW; --bit) {  // below, all keys of one sign are alike
+        const uint32_t want = bound | (1u << bit);
+        if (ts_count(mine >= want) >= p.top) bound = want;
+      }
+    if (parts > 1) {
+      if (threadIdx.x == 0) {
+        sh.stat = a;
+        sh.bound = bound;
+      }
+      cluster.sync();
+      a = *cluster.map_shared_rank(&sh.stat, 0);
+      float m = a.m;
+      for (int i = 1; i < parts; ++i) m = fmaxf(m, cluster.map_shared_rank(&sh, i)->stat.m);
+      a.move(m);
+      for (int i = 1; i < parts; ++i) {
+        Stat o = cluster.map_shared_rank(&sh, i)->stat;
+        o.move(m);
+        a.s += o.s;
+        a.w += o.w;
+      }
+      for (int i = 0; i < parts; ++i) bound = max(bound, cluster.map_shared_rank(&sh, i)->bound);
+    }
+    const bool odd = !(a.s > 0.f && a.s < INFINITY && fabsf(a.m) < 1e30f);  // NaN, +inf, or nothing that the reference can be compared with
+
+    // ---- what reaches the bound, into the first block's list
+    Shared* first = parts > 1 ? cluster.map_shared_rank(&sh, 0) : &sh;
+    if (p.top > 0 && !odd) {
+      const float limit = bound <= order_key(-INFINITY) ? -INFINITY : key_value(bound);
+      if (any && mine >= bound) sh.who[atomicAdd(&sh.threads, 1)] = static_cast<uint16_t>(threadIdx.x);
+      ts_sync();
+      const int who = sh.threads, items = who * ((n + TS_THREADS - 1) / TS_THREADS);
+      const float inv_who = 1.f / static_cast<float>(who);
+      const auto put = [&](float f, int at) {
+        const int k = atomicAdd(&first->found, 1);
+        if (k < TS_CANDIDATES) first->list[k] = (static_cast<unsigned long long>(order_key(f)) << 32) | (0xffffffffu - at);
+      };
+      // item i: vector i / who of the (i % who)-th of those threads, four on their way at a time
+      for (int i0 = threadIdx.x; i0 < items; i0 += 4 * TS_THREADS) {
+        uint4 raw[4];
+        int at[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int i = i0 + u * TS_THREADS;
+          int q = static_cast<int>(static_cast<float>(i) * inv_who);
+          q -= q * who > i;
+          q += (q + 1) * who <= i;
+          at[u] = i < items ? q * TS_THREADS + sh.who[i - q * who] : n;
+          raw[u] = at[u] < n ? __ldg(vec + at[u]) : L::none();
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          float f[L::N];
+          L::open(raw[u], f);
+#pragma unroll
+          for (int k = 0; k < L::N; ++k)
+            if (f[k] >= limit && at[u] < n) put(f[k], row.head + (v0 + at[u]) * L::N + k);
+        }
+      }
+      if (has_loose && loose >= limit) put(loose, loose_at);
+    }
+    if (parts > 1) cluster.sync(); else ts_sync();
+    if (part != 0) return;
+
+    if (odd) {
+      scores_any(p, t, x, sh);
+      ts_sync();
+      if (p.top > 0) {
+        const Stat b = any_stat(x, p.V, p.inv_temp, sh.red);
+        top_any(p, t, x, sh, b.m, logf(b.s), false);
+      }
+      ts_sync();
+      continue;
+    }
+    const float ls = log2f(a.s);
+    if (threadIdx.x == 0) {
+      p.lse[t] = TS_LN2 * (a.m + ls);
+      p.entropy[t] = TS_LN2 * (ls - a.w / a.s);
+    }
+    for (int j = threadIdx.x; j < p.K; j += TS_THREADS) {
+      const long long at = static_cast<long long>(t) * p.K + j, id = j < TS_THREADS ? id0 : p.ids[at];
+      const bool there = id >= 0 && id < p.V;
+      p.logprob[at] = there ? scaled_logprob(static_cast<float>(j < TS_THREADS ? given : x[id]), p.inv_temp, a.m, ls) : 0.f;
+    }
     if (p.top > 0) {
-      const Stat b = any_stat(x, p.V, p.inv_temp, sh.red);
-      top_any(p, t, x, sh, b.m, logf(b.s), false);
+      const int found = sh.found;
+      if (found > TS_CANDIDATES || found < p.top) {
+        top_any(p, t, x, sh, a.m, ls, true);
+      } else {
+        for (int i = threadIdx.x; i < found; i += TS_THREADS) {
+          const unsigned long long key = sh.list[i];
+          int rank = 0;
+          for (int j = 0; j + 1 < found; j += 2) {
+            const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(&sh.list[j]);
+            rank += (two.x > key) + (two.y > key);
+          }
+          if (found & 1) rank += sh.list[found - 1] > key;
+          if (rank < p.top) {
+            const long long at = static_cast<long long>(t) * p.top + rank;
+            p.top_ids[at] = 0xffffffffu - static_cast<uint32_t>(key);
+            p.top_lp[at] = scaled_logprob(key_value(static_cast<uint32_t>(key >> 32)), p.inv_temp, a.m, ls);
+          }
+        }
+      }
     }
-    return;
+    ts_sync();  // the next row starts with an empty list
   }
-  const float ls = log2f(a.s);
-  if (threadIdx.x == 0) {
-    p.lse[t] = TS_LN2 * (a.m + ls);
-    p.entropy[t] = TS_LN2 * (ls - a.w / a.s);
-  }
-  for (int j = threadIdx.x; j < p.K; j += TS_THREADS) {
-    const long long id = p.ids[t * p.K + j];
-    p.logprob[t * p.K + j] = id >= 0 && id < p.V ? scaled_logprob(static_cast<float>(x[id]), p.inv_temp, a.m, ls) : 0.f;
-  }
-  if (p.top == 0) return;
-  const int found = sh.found;
-  if (found > TS_CANDIDATES || found < p.top) {
-    top_any(p, t, x, sh, a.m, ls, true);
-    return;
-  }
-  for (int i = threadIdx.x; i < found; i += TS_THREADS) {
-    const unsigned long long key = sh.list[i];
-    int rank = 0;
-    for (int j = 0; j < found; ++j) rank += sh.list[j] > key;
-    if (rank < p.top) {
-      const uint32_t v = 0xffffffffu - static_cast<uint32_t>(key);
-      p.top_ids[t * p.top + rank] = v;
-      p.top_lp[t * p.top + rank] = scaled_logprob(static_cast<float>(x[v]), p.inv_temp, a.m, ls);
-    }
-  }
+  if (!ok && (threadIdx.x & 31) == 0) atomicExch(status, ST_TIMEOUT_EPILOGUE);
 }
 
 // ---- gradient: blockIdx.x is the row, blockIdx.y one of gridDim.y parts of its columns
@@ -465,7 +579,7 @@ token_scores_bwd_kernel(const VbScores p, const float* __restrict__ g_lp, const 
     for (int v = threadIdx.x; v < head; v += TS_THREADS) d[v] = static_cast<T>(slope(static_cast<float>(x[v])));
     for (int v = behind + threadIdx.x; v < columns; v += TS_THREADS) d[v] = static_cast<T>(v < p.V ? slope(static_cast<float>(x[v])) : 0.f);
   }
-  __syncthreads();
+  ts_sync();
   // the given tokens: a token's first place in the list gathers all its gradients, in their order
   for (int j = threadIdx.x; j < p.K; j += TS_THREADS) {
     const long long id = ids[j];
@@ -485,27 +599,33 @@ token_scores_bwd_kernel(const VbScores p, const float* __restrict__ g_lp, const 
 
 template <typename T>
 static cudaError_t ts_forward(const VbScores& a, cudaStream_t s) {
-  // as many blocks to a row as the card holds at once (two an SM), with at least 1024 vectors for each
+  // as many blocks to a row as the card holds at once (two an SM), with at least 1024 vectors for each; with more rows than that, blocks that stay
   int parts = 1;
-  while (parts < 8 && 2LL * parts * a.T <= 2LL * num_sms() && a.V / Lane<T>::N >= 2048 * parts) parts *= 2;
-  if (static_cast<long long>(a.T) * parts > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+  while (parts < 8 && static_cast<long long>(parts) * a.T <= num_sms() && a.V / Lane<T>::N >= 2048 * parts) parts *= 2;
+  constexpr int smem = TS_STAGES * TS_CHUNK * 16;
+  auto kern = token_scores_kernel<T>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  int* status = nullptr;
+  if (e == cudaSuccess) e = cudaGetSymbolAddress(reinterpret_cast<void**>(&status), g_ts_status);
+  if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = parts;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(a.T * parts);
-  cfg.blockDim = dim3(TS_THREADS);
+  cfg.gridDim = dim3(parts > 1 ? a.T * parts : min(a.T, 2 * num_sms()));
+  cfg.blockDim = dim3(TS_THREADS + 32);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, token_scores_kernel<T>, a);
+  return cudaLaunchKernelEx(&cfg, kern, a, status);
 }
 
 template <typename T>
 static cudaError_t ts_backward(const VbScores& a, const float* g_lp, const float* g_ent, void* dx, long long lddx, int columns, cudaStream_t s) {
   int parts = 1;
-  while (parts < 32 && 2LL * parts * a.T <= 2LL * num_sms() && a.V / Lane<T>::N >= 2048 * parts) parts *= 2;
+  while (parts < 32 && static_cast<long long>(parts) * a.T <= num_sms() && a.V / Lane<T>::N >= 2048 * parts) parts *= 2;
   token_scores_bwd_kernel<T><<<dim3(a.T, parts), TS_THREADS, 0, s>>>(a, g_lp, g_ent, static_cast<T*>(dx), lddx, columns);
   return cudaGetLastError();
 }
@@ -513,6 +633,16 @@ static cudaError_t ts_backward(const VbScores& a, const float* g_lp, const float
 }  // namespace vb
 
 using namespace vb;
+
+extern "C" int vb_token_scores_status() {
+  int h[4] = {0, 0, 0, 0};
+  if (cudaMemcpyFromSymbol(h, g_ts_status, sizeof(h)) != cudaSuccess) return -1;
+  if (h[0] != 0) {
+    int z[4] = {0, 0, 0, 0};
+    cudaMemcpyToSymbol(g_ts_status, z, sizeof(z));
+  }
+  return h[0];
+}
 
 extern "C" int vb_token_scores(const VbScores* a, cudaStream_t s) {
   if (a->T == 0) return 0;
