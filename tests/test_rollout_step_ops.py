@@ -535,6 +535,21 @@ def test_log_probs_for_any_leading_shape_and_without_a_use(dev):
         assert (token_logprobs(wide, one.view(-1)[:4] % 5)[1] > 0).all()
 
 
+def test_log_probs_are_differentiated_once(dev):
+    x = torch.randn(3, 20, device=dev, requires_grad=True)
+    lp, ent = token_logprobs(x, torch.zeros(3, dtype=torch.int64, device=dev))
+    (g,) = torch.autograd.grad(lp.sum() + ent.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(g.square().sum(), x)
+    lp, _ = token_logprobs(x, torch.zeros(3, dtype=torch.int64, device=dev))
+    with torch.no_grad():
+        x.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        lp.sum().backward()
+    with torch.no_grad():
+        assert not token_logprobs(x, torch.zeros(3, dtype=torch.int64, device=dev))[0].requires_grad
+
+
 def test_refusals_of_the_scores(dev):
     x, ids = torch.zeros(2, 9, device=dev), torch.zeros(2, dtype=torch.int64, device=dev)
     for bad in (lambda: F.token_scores(x[0], ids), lambda: F.token_scores(x, ids[:1]), lambda: F.token_scores(x, ids.int()),

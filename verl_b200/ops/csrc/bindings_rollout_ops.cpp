@@ -2,6 +2,8 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include <tuple>
@@ -183,12 +185,12 @@ VbScores scores_of(const Tensor& x, const Tensor& ids, double temperature, int64
               ": logits [rows, vocabulary] with contiguous rows");
   TORCH_CHECK(valid > 0 && valid <= x.size(1), what, ": valid_vocab must lie in 1 .. ", x.size(1), ", got ", valid);
   TORCH_CHECK(temperature > 0, what, ": temperature must be positive");
-  TORCH_CHECK(ids.device() == x.device() && ids.scalar_type() == at::kLong && ids.dim() == 2 && ids.size(0) == x.size(0) && ids.is_contiguous(), what,
-              ": ids must be a contiguous int64 matrix with a row for each row of logits");
-  TORCH_CHECK(ids.size(1) <= 4096, what, ": at most 4096 given tokens a row");
+  TORCH_CHECK(ids.device() == x.device() && ids.scalar_type() == at::kLong && (ids.dim() == 1 || ids.dim() == 2) && ids.size(0) == x.size(0) &&
+              ids.is_contiguous(), what, ": ids must be a contiguous int64 tensor on ", x.device(), " with an entry or a row for each row of logits");
+  TORCH_CHECK(ids.dim() == 1 || ids.size(1) <= 4096, what, ": at most 4096 given tokens a row");
   a.x = x.data_ptr(); a.ldx = x.size(0) <= 1 ? 0 : x.stride(0); a.T = (int)x.size(0); a.V = (int)valid;
   a.inv_temp = (float)(1.0 / temperature);
-  a.ids = lptr(ids); a.K = (int)ids.size(1);
+  a.ids = lptr(ids); a.K = ids.dim() == 1 ? 1 : (int)ids.size(1);
   return a;
 }
 
@@ -224,6 +226,46 @@ Tensor token_scores_bwd(const Tensor& x, const Tensor& ids, const Tensor& lse, c
   return dx;
 }
 
+// Log-probs and entropy with their gradient. In C++, because a function written in Python costs more on the host (146 us a step, 36 of them
+// forward) than the kernels of most batches on the device.
+struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& ids, double temperature, int64_t valid) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [lp, ent, lse, top, top_lp] = token_scores(x, ids, 0, temperature, valid);
+    ctx->save_for_backward({x, ids, lse, ent.detach()});
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["valid"] = valid;
+    ctx->set_materialize_grads(false);
+    return {lp, ent};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+    Tensor none, dx;
+    if (g[0].defined() || g[1].defined()) {
+      const bool again = at::GradMode::is_enabled();
+      const auto saved = ctx->get_saved_variables();
+      {
+        at::NoGradGuard guard;
+        const Tensor g_lp = g[0].defined() ? g[0].contiguous() : at::zeros(saved[1].sizes(), saved[2].options());
+        OptTensor g_ent;
+        if (g[1].defined()) g_ent = g[1].contiguous();
+        dx = token_scores_bwd(saved[0].detach(), saved[1], saved[2], saved[3], g_lp, g_ent, ctx->saved_data["temperature"].toDouble(), ctx->saved_data["valid"].toInt());
+      }
+      if (again)  // a graph of the gradient is asked for: an error where it is used
+        dx = std::make_shared<torch::autograd::DelayedError>("token_logprobs can be differentiated once", 2)->apply({dx, saved[0]})[0];
+    }
+    return {dx, none, none, none};
+  }
+};
+
+std::tuple<Tensor, Tensor> token_logprobs(const Tensor& x, const Tensor& ids, double temperature, int64_t valid) {
+  if (at::GradMode::is_enabled() && x.requires_grad()) {
+    auto out = TokenLogprobs::apply(x, ids, temperature, valid);
+    return {out[0], out[1]};
+  }
+  auto out = token_scores(x, ids, 0, temperature, valid);
+  return {std::get<0>(out), std::get<1>(out)};
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(verl_b200, m) {
@@ -235,4 +277,5 @@ TORCH_LIBRARY_FRAGMENT(verl_b200, m) {
   m.def("paged_decode_kv4", &paged_decode_kv4);
   m.def("token_scores", &token_scores);
   m.def("token_scores_bwd", &token_scores_bwd);
+  m.def("token_logprobs", &token_logprobs);
 }

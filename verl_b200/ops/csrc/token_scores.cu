@@ -5,9 +5,10 @@
 // five instructions and one exponential a value. A thread keeps a reference of its own, which moves only when a value is 2^60 above it.
 //
 // The most likely tokens come with the same pass: every thread also keeps the largest value that it met, and the k-th largest of those of a
-// block is a bound that at least k values of the row reach. Only the columns of threads that reach it are looked at again (about k of 512
-// threads, from L2); what reaches the bound there is hardly more than k values, which are ranked by counting. Rows that this does not fit (over
-// 1024 values at the bound: a row of few different values) and rows with NaN, +inf or nothing above -1e30 take a slow path, right for any values.
+// block is a bound that at least k values of the row reach. The largest value of each group of 32 (16 of 32 bits) stays in shared memory, and
+// only groups that reach the bound are looked at again (hardly more than k, from L2); what reaches it there is again hardly more than k
+// values, which are ranked by counting. Rows that this does not fit (over 768 values at the bound: few different values) and rows with NaN,
+// +inf or nothing above -1e30 take a slow path, right for any values.
 //
 // Blocks stay for many rows. One warp of a block brings the rows into a ring of shared memory by bulk copies, so that the next row is on its way
 // while the block ranks the last one. Where rows are few, a row belongs to a cluster of up to 8 blocks, which exchange their sums, bounds and
@@ -29,12 +30,14 @@ namespace vb {
 namespace cg = cooperative_groups;
 int num_sms();
 
-constexpr int TS_THREADS = 512;    // that compute
+constexpr int TS_THREADS = 256;    // that compute
+constexpr int TS_BLOCKS = 4;       // blocks of an SM
 constexpr int TS_BATCH = 4;        // 16-byte vectors of a thread in flight (gradient)
-constexpr int TS_STAGES = 3;
+constexpr int TS_STAGES = 2;
 constexpr int TS_PER = 4;                      // 16-byte vectors of a thread in a stage
-constexpr int TS_CHUNK = TS_PER * TS_THREADS;  // vectors of a stage: 32 KB
-constexpr int TS_CANDIDATES = 1024;
+constexpr int TS_CHUNK = TS_PER * TS_THREADS;  // vectors of a stage: 16 KB
+constexpr int TS_CANDIDATES = 768;
+constexpr int TS_SLOTS = 24;       // groups of a thread that are told apart: stages of the row, modulo this
 constexpr float TS_LOG2E = 1.4426950408889634f, TS_LN2 = 0.6931471805599453f;
 constexpr float TS_FLOOR = -200.f;  // exponents below this are zeros: keeps 0 * inf out of the sums
 
@@ -231,10 +234,11 @@ struct Shared {
   float red[48];
   Stat stat;               // of this block's part of the row
   uint32_t bound;          // at least top values of the part have this key or a larger one (0: the part has fewer threads with values)
-  int threads, found;
+  int groups, found;
   unsigned long long wide[16];
-  uint16_t who[TS_THREADS];
-  __align__(16) unsigned long long list[TS_CANDIDATES];  // (key, place backwards)
+  uint16_t group[TS_CANDIDATES];           // slot * TS_THREADS + thread of the groups that reach the bound
+  uint16_t top[TS_SLOTS][TS_THREADS];      // upper halves of the keys of the groups' largest values
+  unsigned long long list[TS_CANDIDATES];  // (key, place backwards)
 };
 
 template <typename T>
@@ -281,7 +285,7 @@ __device__ __forceinline__ void bulk_row(void* dst, const T* src, uint32_t bytes
 }
 
 template <typename T>
-__global__ void __launch_bounds__(TS_THREADS + 32, 2)
+__global__ void __launch_bounds__(TS_THREADS + 32, TS_BLOCKS)
 token_scores_kernel(const VbScores p, int* status) {
   using L = Lane<T>;
   extern __shared__ __align__(16) uint4 ring[];  // TS_STAGES x TS_CHUNK
@@ -331,7 +335,7 @@ token_scores_kernel(const VbScores p, int* status) {
     const Row<T> row(x, p.V);
     const int per = (row.vecs + parts - 1) / parts, v0 = min(row.vecs, part * per), n = min(row.vecs, v0 + per) - v0;
     const uint4* vec = row.vec() + v0;
-    if (threadIdx.x == 0) sh.threads = sh.found = 0;
+    if (threadIdx.x == 0) sh.groups = sh.found = 0;
     // the value of this thread's given token, on its way during the pass
     const long long id0 = part == 0 && static_cast<int>(threadIdx.x) < p.K ? p.ids[static_cast<long long>(t) * p.K + threadIdx.x] : -1;
     const T given = x[id0 >= 0 && id0 < p.V ? id0 : 0];
@@ -339,7 +343,7 @@ token_scores_kernel(const VbScores p, int* status) {
     // ---- the pass
     Stat a{-1e30f, 0.f, 0.f};
     float most = -INFINITY;
-    for (int v = 0; v < n; v += TS_CHUNK) {
+    for (int v = 0, slot = 0; v < n; v += TS_CHUNK, ++slot) {
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], round & 1));
       const uint4* at = ring + stage * TS_CHUNK + threadIdx.x;
       const int left = n - v - static_cast<int>(threadIdx.x);
@@ -362,6 +366,11 @@ token_scores_kernel(const VbScores p, int* status) {
           for (int i = 0; i < L::N; i += 2) big = fmaxf(big, fmaxf(f[i], f[i + 1]));
         }
       most = fmaxf(most, big);
+      if (p.top > 0) {
+        uint16_t* keep = &sh.top[slot % TS_SLOTS][threadIdx.x];
+        const uint16_t key = static_cast<uint16_t>(order_key(big) >> 16);
+        *keep = slot < TS_SLOTS ? key : max(*keep, key);
+      }
       if (big * c > a.m + 60.f) a.move(big * c);
       float s0 = a.s, s1 = 0.f, w0 = a.w, w1 = 0.f;
 #pragma unroll
@@ -441,35 +450,30 @@ token_scores_kernel(const VbScores p, int* status) {
     Shared* first = parts > 1 ? cluster.map_shared_rank(&sh, 0) : &sh;
     if (p.top > 0 && !odd) {
       const float limit = bound <= order_key(-INFINITY) ? -INFINITY : key_value(bound);
-      if (any && mine >= bound) sh.who[atomicAdd(&sh.threads, 1)] = static_cast<uint16_t>(threadIdx.x);
+      const int chunks = (n + TS_CHUNK - 1) / TS_CHUNK, low = static_cast<int>(bound >> 16);
+      if (mine >= bound)
+        for (int slot = 0; slot < min(chunks, TS_SLOTS); ++slot)
+          if (sh.top[slot][threadIdx.x] >= low) {
+            const int k = atomicAdd(&sh.groups, 1);
+            if (k < TS_CANDIDATES) sh.group[k] = static_cast<uint16_t>(slot * TS_THREADS + threadIdx.x);
+          }
       ts_sync();
-      const int who = sh.threads, items = who * ((n + TS_THREADS - 1) / TS_THREADS);
-      const float inv_who = 1.f / static_cast<float>(who);
+      const int groups = min(sh.groups, TS_CANDIDATES), turns = (chunks + TS_SLOTS - 1) / TS_SLOTS, items = groups * TS_PER * turns;
+      if (sh.groups > TS_CANDIDATES && threadIdx.x == 0) atomicAdd(&first->found, TS_CANDIDATES + 1);  // too many: the slow path
       const auto put = [&](float f, int at) {
         const int k = atomicAdd(&first->found, 1);
         if (k < TS_CANDIDATES) first->list[k] = (static_cast<unsigned long long>(order_key(f)) << 32) | (0xffffffffu - at);
       };
-      // item i: vector i / who of the (i % who)-th of those threads, four on their way at a time
-      for (int i0 = threadIdx.x; i0 < items; i0 += 4 * TS_THREADS) {
-        uint4 raw[4];
-        int at[4];
+      // item i: vector i % TS_PER of group i / TS_PER, and for rows of more stages than slots the same place some stages on
+      for (int i = threadIdx.x; i < items; i += TS_THREADS) {
+        const int turn = i / (groups * TS_PER), k = i - turn * groups * TS_PER, g = sh.group[k / TS_PER];
+        const int at = ((turn * TS_SLOTS + g / TS_THREADS) * TS_PER + k % TS_PER) * TS_THREADS + g % TS_THREADS;
+        if (at >= n) continue;
+        float f[L::N];
+        L::open(__ldg(vec + at), f);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int i = i0 + u * TS_THREADS;
-          int q = static_cast<int>(static_cast<float>(i) * inv_who);
-          q -= q * who > i;
-          q += (q + 1) * who <= i;
-          at[u] = i < items ? q * TS_THREADS + sh.who[i - q * who] : n;
-          raw[u] = at[u] < n ? __ldg(vec + at[u]) : L::none();
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          float f[L::N];
-          L::open(raw[u], f);
-#pragma unroll
-          for (int k = 0; k < L::N; ++k)
-            if (f[k] >= limit && at[u] < n) put(f[k], row.head + (v0 + at[u]) * L::N + k);
-        }
+        for (int j = 0; j < L::N; ++j)
+          if (f[j] >= limit) put(f[j], row.head + (v0 + at) * L::N + j);
       }
       if (has_loose && loose >= limit) put(loose, loose_at);
     }
@@ -501,14 +505,16 @@ token_scores_kernel(const VbScores p, int* status) {
       if (found > TS_CANDIDATES || found < p.top) {
         top_any(p, t, x, sh, a.m, ls, true);
       } else {
-        for (int i = threadIdx.x; i < found; i += TS_THREADS) {
-          const unsigned long long key = sh.list[i];
+        // four lanes a candidate count the larger ones
+        for (int i0 = 0; i0 < found; i0 += TS_THREADS / 4) {
+          const int i = i0 + (threadIdx.x >> 2), quarter = threadIdx.x & 3;
+          const unsigned long long key = sh.list[min(i, found - 1)];
           int rank = 0;
-          for (int j = 0; j + 1 < found; j += 2) {
-            const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(&sh.list[j]);
-            rank += (two.x > key) + (two.y > key);
-          }
-          if (found & 1) rank += sh.list[found - 1] > key;
+#pragma unroll 4
+          for (int j = quarter; j < found; j += 4) rank += sh.list[j] > key;
+          rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+          rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+          if (i >= found || quarter != 0) continue;
           if (rank < p.top) {
             const long long at = static_cast<long long>(t) * p.top + rank;
             p.top_ids[at] = 0xffffffffu - static_cast<uint32_t>(key);
@@ -524,7 +530,7 @@ token_scores_kernel(const VbScores p, int* status) {
 
 // ---- gradient: blockIdx.x is the row, blockIdx.y one of gridDim.y parts of its columns
 template <typename T>
-__global__ void __launch_bounds__(TS_THREADS, 2)
+__global__ void __launch_bounds__(TS_THREADS, TS_BLOCKS)
 token_scores_bwd_kernel(const VbScores p, const float* __restrict__ g_lp, const float* __restrict__ g_ent, T* __restrict__ dx, long long lddx, int columns) {
   using L = Lane<T>;
   __shared__ Shared sh;
@@ -599,9 +605,9 @@ token_scores_bwd_kernel(const VbScores p, const float* __restrict__ g_lp, const 
 
 template <typename T>
 static cudaError_t ts_forward(const VbScores& a, cudaStream_t s) {
-  // as many blocks to a row as the card holds at once (two an SM), with at least 1024 vectors for each; with more rows than that, blocks that stay
+  // as many blocks to a row as the card holds at once, with at least 1024 vectors for each; with more rows than that, blocks that stay
   int parts = 1;
-  while (parts < 8 && static_cast<long long>(parts) * a.T <= num_sms() && a.V / Lane<T>::N >= 2048 * parts) parts *= 2;
+  while (parts < 8 && 2LL * parts * a.T <= TS_BLOCKS * num_sms() && a.V / Lane<T>::N >= 2048 * parts) parts *= 2;
   constexpr int smem = TS_STAGES * TS_CHUNK * 16;
   auto kern = token_scores_kernel<T>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -613,7 +619,7 @@ static cudaError_t ts_forward(const VbScores& a, cudaStream_t s) {
   attr[0].val.clusterDim.x = parts;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(parts > 1 ? a.T * parts : min(a.T, 2 * num_sms()));
+  cfg.gridDim = dim3(parts > 1 ? a.T * parts : min(a.T, TS_BLOCKS * num_sms()));
   cfg.blockDim = dim3(TS_THREADS + 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
@@ -625,7 +631,7 @@ static cudaError_t ts_forward(const VbScores& a, cudaStream_t s) {
 template <typename T>
 static cudaError_t ts_backward(const VbScores& a, const float* g_lp, const float* g_ent, void* dx, long long lddx, int columns, cudaStream_t s) {
   int parts = 1;
-  while (parts < 32 && static_cast<long long>(parts) * a.T <= num_sms() && a.V / Lane<T>::N >= 2048 * parts) parts *= 2;
+  while (parts < 32 && 2LL * parts * a.T <= TS_BLOCKS * num_sms() && a.V / Lane<T>::N >= 2048 * parts) parts *= 2;
   token_scores_bwd_kernel<T><<<dim3(a.T, parts), TS_THREADS, 0, s>>>(a, g_lp, g_ent, static_cast<T*>(dx), lddx, columns);
   return cudaGetLastError();
 }

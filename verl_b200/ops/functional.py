@@ -47,6 +47,7 @@ __all__ = [
     "paged_decode_attention_kv4",
     "TokenScores",
     "token_scores",
+    "token_logprobs",
     "token_scores_bwd",
     "sample_tokens",
     "grpo_advantage",
@@ -942,11 +943,10 @@ def token_scores(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0, temper
     V = _scores_args("token_scores", logits, ids, temperature, valid_vocab)
     if not 0 <= top_k <= min(TOP_K_LIMIT, V):
         raise ValueError(f"token_scores: top_k must lie in 0 .. {min(TOP_K_LIMIT, V)}, got {top_k}")
-    flat = ids if ids.dim() == 2 else ids[:, None]
     if logits.is_cuda:
         x = logits if logits.stride(1) == 1 else logits.contiguous()
-        out = _ops().token_scores(x, flat.contiguous(), int(top_k), float(temperature), V)
-        return TokenScores(out[0].view(ids.shape), *out[1:])
+        return TokenScores._make(_ops().token_scores(x, ids.contiguous(), int(top_k), float(temperature), V))
+    flat = ids if ids.dim() == 2 else ids[:, None]
     x = logits[:, :V].float()
     z = x * (1.0 / float(temperature))
     m = z.amax(-1, keepdim=True)
@@ -962,6 +962,14 @@ def token_scores(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0, temper
     return TokenScores(lp.view(ids.shape), ent[:, 0], lse[:, 0], top, score(top))
 
 
+def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, temperature: float = 1.0, valid_vocab: int = 0):
+    """``logprob`` and ``entropy`` of :func:`token_scores` with their gradient, on a GPU (``utils.kernel.token_logprobs`` is the form for any device
+    and leading shape)."""
+    V = _scores_args("token_logprobs", logits, ids, temperature, valid_vocab)
+    x = logits if logits.stride(1) == 1 else logits.contiguous()
+    return _ops().token_logprobs(x, ids.contiguous(), float(temperature), V)
+
+
 def token_scores_bwd(logits: torch.Tensor, ids: torch.Tensor, lse: torch.Tensor, entropy: torch.Tensor, g_logprob: torch.Tensor,
                      g_entropy: Optional[torch.Tensor], temperature: float = 1.0, valid_vocab: int = 0) -> torch.Tensor:
     """Gradient of the logits, in their type, from those of ``logprob`` and ``entropy`` (None: none) of :func:`token_scores`. A token that is given
@@ -970,11 +978,11 @@ def token_scores_bwd(logits: torch.Tensor, ids: torch.Tensor, lse: torch.Tensor,
     T = logits.shape[0]
     if g_logprob.shape != ids.shape or (g_entropy is not None and g_entropy.shape != (T,)) or lse.shape != (T,) or entropy.shape != (T,):
         raise ValueError("token_scores_bwd: g_logprob has the shape of ids; lse, entropy and g_entropy have an entry for each row")
-    flat, g = (t if t.dim() == 2 else t[:, None] for t in (ids, g_logprob.float()))
     if logits.is_cuda:
         x = logits if logits.stride(1) == 1 else logits.contiguous()
-        return _ops().token_scores_bwd(x, flat.contiguous(), lse.contiguous(), entropy.contiguous(), g.contiguous(),
+        return _ops().token_scores_bwd(x, ids.contiguous(), lse.contiguous(), entropy.contiguous(), g_logprob.float().contiguous(),
                                        g_entropy.float().contiguous() if g_entropy is not None else None, float(temperature), V)
+    flat, g = (t if t.dim() == 2 else t[:, None] for t in (ids, g_logprob.float()))
     inv = 1.0 / float(temperature)
     logp = torch.log_softmax(logits[:, :V].float() * inv, -1)
     p = torch.exp(logp)

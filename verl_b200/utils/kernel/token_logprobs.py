@@ -9,14 +9,25 @@ Parity target: ``verl/utils/torch_functional.py`` (``logprobs_from_logits``, ``e
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from ...ops import functional as F
 
 __all__ = ["TokenLogprobs", "token_logprobs"]
 
 
+class _Once(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, grad, logits):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, g):
+        raise RuntimeError("token_logprobs can be differentiated once")
+
+
 class TokenLogprobs(torch.autograd.Function):
+    """The form on the host; on a GPU the same function is part of the native library."""
+
     @staticmethod
     def forward(ctx, logits: torch.Tensor, ids: torch.Tensor, temperature: float, valid_vocab: int):
         out = F.token_scores(logits, ids, 0, temperature, valid_vocab)
@@ -26,14 +37,17 @@ class TokenLogprobs(torch.autograd.Function):
         return out.logprob, out.entropy
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_lp, g_ent):
         if g_lp is None and g_ent is None:
             return None, None, None, None
         logits, ids, lse, entropy = ctx.saved_tensors
         if g_lp is None:
             g_lp = torch.zeros(ids.shape, dtype=torch.float32, device=logits.device)
-        return F.token_scores_bwd(logits, ids, lse, entropy, g_lp, g_ent, *ctx.meta), None, None, None
+        with torch.no_grad():
+            d = F.token_scores_bwd(logits, ids, lse, entropy, g_lp, g_ent, *ctx.meta)
+        if torch.is_grad_enabled():   # a graph of the gradient is asked for: an error where it is used
+            d = _Once.apply(d, logits)
+        return d, None, None, None
 
 
 def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, temperature: float = 1.0, valid_vocab: int = 0):
@@ -42,6 +56,9 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, temperature: float =
     lead = logits.shape[:-1]
     if ids.shape != lead and ids.shape[:-1] != lead:
         raise ValueError(f"token_logprobs: ids {tuple(ids.shape)} do not fit logits {tuple(logits.shape)}")
+    run = F.token_logprobs if logits.is_cuda else TokenLogprobs.apply
+    if logits.dim() == 2:
+        return run(logits, ids, float(temperature), int(valid_vocab))
     flat = ids.reshape(-1) if ids.shape == lead else ids.reshape(-1, ids.shape[-1])
-    lp, ent = TokenLogprobs.apply(logits.reshape(-1, logits.shape[-1]), flat, float(temperature), int(valid_vocab))
+    lp, ent = run(logits.reshape(-1, logits.shape[-1]), flat, float(temperature), int(valid_vocab))
     return lp.view(ids.shape), ent.view(lead)
