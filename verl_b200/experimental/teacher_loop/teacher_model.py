@@ -18,6 +18,7 @@ from typing import Optional
 import torch
 
 from ...models.decoder import DecoderModel, PackedBatch
+from ...ops import functional as F
 from ...workers.rollout.llm_server import GlobalRequestLoadBalancer
 
 __all__ = ["TeacherServer", "TeacherModelManager", "MultiTeacherModelManager"]
@@ -75,8 +76,15 @@ class TeacherServer:
         nxt = torch.roll(flat, -1)
         for lo in range(0, hidden.size(0), self.chunk):
             h = hidden[lo : lo + self.chunk]
-            logits = (h @ W.t()).float()
-            lp = torch.log_softmax(logits, -1)
+            logits = h @ W.t()
+            k = min(self.topk, logits.size(-1))
+            if logits.is_cuda and k <= F.TOP_K_LIMIT:  # one pass over the logits, no fp32 copy of them
+                at = nxt[lo : lo + self.chunk]
+                rec = F.token_scores(logits, at, max(k, 0))
+                ids_l.append(rec.top_ids if k > 0 else at[:, None])
+                lps_l.append(rec.top_logprob if k > 0 else rec.logprob[:, None])
+                continue
+            lp = torch.log_softmax(logits.float(), -1)
             if self.topk <= 0:
                 i = nxt[lo : lo + self.chunk, None]
                 v = lp.gather(-1, i)

@@ -180,6 +180,10 @@ class ModuleFlatParams:
 
 
 def _logprob_entropy_from_logits(logits: torch.Tensor, labels: torch.Tensor):
+    if logits.is_cuda:
+        from ..utils.kernel import token_logprobs
+
+        return token_logprobs(logits.float(), labels.long())
     logp = torch.log_softmax(logits.float(), -1)
     lp = logp.gather(-1, labels.long()[:, None]).squeeze(-1)
     ent = -(logp.exp() * logp).sum(-1)

@@ -5,7 +5,6 @@
 #include <torch/library.h>
 
 #include "launchers.h"
-#include "rollout_ops.h"
 
 #include <algorithm>
 #include <atomic>

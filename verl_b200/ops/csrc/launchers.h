@@ -110,6 +110,9 @@ int vb_paged_decode_v2(const void* q, long long ldq, const void* kc, const void*
                        int nkv, int hd, int block_size, float scale, int nsplit, float* part_o, float* part_ml,
                        cudaStream_t stream);
 int vb_pd_status();
+// kv4_decode.cu, token_scores.cu (their launchers: rollout_ops.h)
+int vb_kv4_status();
+int vb_token_scores_status();
 // comm_fused.cu
 int vb_peer_barrier(const unsigned long long* pad_ptrs, int rank, int W, unsigned int epoch, double limit_s,
                     float* poison_on_timeout, cudaStream_t s);

@@ -31,7 +31,6 @@ struct VbKv4Decode {
 };
 long long vb_kv4_decode_scratch(int B, int nh, int nkv, int hd);
 int vb_kv4_decode(const VbKv4Decode* a, cudaStream_t s);
-int vb_kv4_status();
 // token_scores.cu: type 0 = bf16, 1 = fp16, 2 = fp32
 struct VbScores {
   const void* x; long long ldx; int type; int T, V;    // V: columns that count
@@ -41,7 +40,6 @@ struct VbScores {
   float* logprob; float* entropy; float* lse;
   long long* top_ids; float* top_lp;                   // [T, top]
 };
-int vb_token_scores_status();
 int vb_token_scores(const VbScores* a, cudaStream_t s);
 int vb_token_scores_bwd(const VbScores* a, const float* g_lp, const float* g_ent, void* dx, long long lddx, int columns, cudaStream_t s);
 }

@@ -126,6 +126,10 @@ def compute_forward_kl_topk(student_logits: Optional[torch.Tensor], teacher_topk
                             config: DistillationLossConfig, student_topk_logp: Optional[torch.Tensor] = None) -> dict:
     """Per-token forward KL on the teacher's support. Give either full ``student_logits`` [..., V] or the already
     gathered ``student_topk_logp`` [..., k]. Returns ``distillation_losses``, ``student_mass``, ``teacher_mass``."""
+    if student_topk_logp is None and student_logits.is_cuda and student_logits.dtype in (torch.float32, torch.bfloat16, torch.float16):
+        from ...utils.kernel import token_logprobs
+
+        student_topk_logp = token_logprobs(student_logits, teacher_topk_ids)[0]   # logits read once forward and once backward
     if student_topk_logp is None:
         student_topk_logp = torch.log_softmax(student_logits.float(), -1).gather(-1, teacher_topk_ids)
     lp_t = teacher_topk_log_probs.float()

@@ -128,6 +128,7 @@ class RolloutConfig(BaseConfig):
     prometheus: dict = field(default_factory=dict)
     quantization: Optional[str] = None  # None | fp8
     quantization_config_file: Optional[str] = None
+    kv_cache_dtype: str = "auto"  # auto (the model's type) | int4
     enable_rollout_routing_replay: bool = False
     enable_sleep_mode: bool = True
     layered_summon: bool = False

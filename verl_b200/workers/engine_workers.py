@@ -385,6 +385,7 @@ class ActorRolloutRefWorker(Worker, DistProfilerExtension):
                                          record_routing=(self._router_replay_mode() == "R3"),
                                          enable_prefix_caching=bool(rc.get("enable_prefix_caching", False)),
                                          quantization=(rc.get("quantization") if tp == 1 else None),
+                                         kv_cache_dtype=rc.get("kv_cache_dtype"),
                                          max_num_batched_tokens=rc.max_num_batched_tokens, max_model_len=max_len + 1,
                                          block_size=rc.block_size, gpu_memory_utilization=rc.gpu_memory_utilization,
                                          use_cuda_graph=not rc.enforce_eager, sync_interval=rc.sync_interval,

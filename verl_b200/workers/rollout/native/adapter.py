@@ -22,7 +22,7 @@ class NativeRollout(BaseRollout):
         self.engine = RolloutEngine(arch, params, max_num_seqs=config.max_num_seqs, max_num_batched_tokens=config.max_num_batched_tokens,
                                     max_model_len=max_len, block_size=config.block_size,
                                     gpu_memory_utilization=config.gpu_memory_utilization, use_cuda_graph=not config.enforce_eager,
-                                    sync_interval=config.sync_interval)
+                                    sync_interval=config.sync_interval, kv_cache_dtype=getattr(config, "kv_cache_dtype", None))
 
     async def resume(self, tags: list[str]):
         if "kv_cache" in tags:

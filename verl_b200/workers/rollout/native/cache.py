@@ -1,6 +1,7 @@
 """What the rollout engine keeps per token and per sequence, behind one interface for its two kinds of models.
 
 * :class:`DenseKVCache`: keys and values of a uniform decoder, one pool ``[layers, 2, blocks, block_size, kv_heads, head_dim]``.
+* :class:`Kv4Cache`: the same in 4 bits (``kv_cache_dtype="int4"``): 0.31 of the bytes, one pool ``[layers, blocks, kv_heads, page bytes]``.
 * :class:`StackCache`: mixer stacks. Attention layers that cache a row per token share a page pool (a block holds the rows of
   all such layers for ``block_size`` tokens); recurrent layers and convolutions own parts of one fp32 state row per sequence slot.
 
@@ -14,7 +15,9 @@ from typing import Optional
 
 import torch
 
-__all__ = ["DenseKVCache", "StackCache", "make_cache"]
+from ....ops import functional as F
+
+__all__ = ["DenseKVCache", "Kv4Cache", "StackCache", "make_cache"]
 
 
 class DenseKVCache:
@@ -46,7 +49,32 @@ class DenseKVCache:
         return {"kv": self.kv[:, :, blocks].clone()}
 
     def install(self, blocks: torch.Tensor, slot: int, data: dict) -> None:
+        assert data["kv"].dtype != torch.uint8, "prefill and decode engines must use the same kv_cache_dtype"
         self.kv[:, :, blocks] = data["kv"].to(self.device, dtype=self.kv.dtype)
+
+
+class Kv4Cache(DenseKVCache):
+    """Keys and values in 4 bits with a scale and a least value for each 32 channels of a token's head (``ops.functional.kv4_page_bytes``)."""
+
+    def bytes_per_block(self) -> int:
+        c = self.cfg
+        return c.num_hidden_layers * (c.num_key_value_heads // self.tp) * F.kv4_page_bytes(self.bs, c.head_dim)
+
+    def allocate(self, blocks: int) -> None:
+        c = self.cfg
+        self.kv = torch.zeros(c.num_hidden_layers, blocks, c.num_key_value_heads // self.tp, F.kv4_page_bytes(self.bs, c.head_dim),
+                              dtype=torch.uint8, device=self.device)
+
+    def copy_blocks(self, dst: torch.Tensor, src: torch.Tensor) -> None:
+        self.kv[:, dst] = self.kv[:, src]
+
+    def export(self, blocks: torch.Tensor, slot: int) -> dict:
+        return {"kv": self.kv[:, blocks].clone()}
+
+    def install(self, blocks: torch.Tensor, slot: int, data: dict) -> None:
+        kv = data["kv"]
+        assert kv.dtype == torch.uint8 and kv.shape[2:] == self.kv.shape[2:], "prefill and decode engines must use the same kv_cache_dtype"
+        self.kv[:, blocks] = kv.to(self.device)
 
 
 class StackCache:
@@ -115,5 +143,6 @@ class StackCache:
             self.states[slot] = data["state"].to(self.device)
 
 
-def make_cache(cfg, dtype, device, block_size: int, num_slots: int, tp_size: int = 1):
-    return (StackCache if cfg.is_stack else DenseKVCache)(cfg, dtype, device, block_size, num_slots, tp_size)
+def make_cache(cfg, dtype, device, block_size: int, num_slots: int, tp_size: int = 1, four_bits: bool = False):
+    kind = StackCache if cfg.is_stack else Kv4Cache if four_bits else DenseKVCache
+    return kind(cfg, dtype, device, block_size, num_slots, tp_size)

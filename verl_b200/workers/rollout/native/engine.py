@@ -18,6 +18,10 @@ Design (one engine per GPU, or per tensor-parallel group):
   trainer between rollout phases.
 * **Mixer stacks** (decoders whose layers differ, ``models/mixer_stack.py``) share the slots, blocks, scheduler, decode loop
   and sampler; their cache (``cache.py``) is a page pool of latent rows plus one recurrent-state row per slot.
+* **4-bit cache** (``kv_cache_dtype="int4"``): keys and values are quantised as they are appended (4 bits, a scale and a least value per 32
+  channels) and the decode attention reads the codes; 3.2 times the tokens in the same pool.
+* **Records**: beside the sampled token's log-prob, ``SamplingParams.top_logprobs`` asks for the most likely tokens with their log-probs and
+  for the entropy of every position (under the sampling temperature, before top-k / top-p).
 * **Prefill** runs the packed varlen forward of the training model with a hook that scatters rotated
   K/V into the cache, in chunks of at most ``max_num_batched_tokens`` tokens.
 
@@ -59,6 +63,7 @@ class SamplingParams:
     ignore_eos: bool = False
     stop_token_ids: Sequence[int] = ()
     logprobs: bool = True
+    top_logprobs: int = 0              # most likely tokens to record per position, with the entropy (at most 128)
     seed: Optional[int] = None
     repetition_penalty: float = 1.0
 
@@ -101,13 +106,18 @@ class RolloutEngine:
                  num_blocks: Optional[int] = None, gpu_memory_utilization: float = 0.5, eos_token_id=None,
                  valid_vocab_size: int = 0, use_cuda_graph: bool = True, sync_interval: int = 16, seed: int = 0,
                  tp_group=None, quantization: Optional[str] = None, share_prefill: bool = True, record_routing: bool = False,
-                 enable_prefix_caching: bool = False):
-        """``tp_group``: process group of the ranks that serve the same requests tensor-parallel (each holds the
+                 enable_prefix_caching: bool = False, kv_cache_dtype: Optional[str] = None):
+        """``kv_cache_dtype``: None / "auto" (the model's type) or "int4" (keys and values in 4 bits; heads of 64 or 128 channels, blocks of 16 to
+        256 tokens and a bf16 model on a GPU).
+
+        ``tp_group``: process group of the ranks that serve the same requests tensor-parallel (each holds the
         full replicated weights and uses its shard of them in place; see ``TensorParallelShard``). All ranks of the
         group must be fed the same requests in the same order."""
         self.cfg = cfg
         assert quantization in (None, "", "fp8"), f"unsupported rollout quantization: {quantization}"
         self.quantization = quantization or None
+        assert kv_cache_dtype in (None, "", "auto", "int4"), f"unsupported kv_cache_dtype: {kv_cache_dtype}"
+        self.kv4 = kv_cache_dtype == "int4"
         self.share_prefill = bool(share_prefill)
         # Prefix cache across requests: full pages stay indexed by a chain hash of their tokens after their last user has
         # finished (evicted least-recently-used when fresh pages run out); a new prompt that starts with cached pages (the
@@ -133,6 +143,12 @@ class RolloutEngine:
         self.params = params
         self.device = params.flat.device
         self.is_cuda = self.device.type == "cuda"
+        if self.kv4:
+            assert not cfg.is_stack, f"{cfg.model_type}: no 4-bit cache for mixer stacks"
+            F.kv4_page_bytes(int(block_size), cfg.head_dim)   # refuses sizes that the layout does not have
+            assert not self.is_cuda or (cfg.head_dim in (64, 128) and int(block_size) in (16, 32, 64, 128, 256) and params.flat.dtype == torch.bfloat16
+                                        and cfg.num_attention_heads // cfg.num_key_value_heads <= 16), \
+                "kv_cache_dtype=int4 on a GPU: bf16, heads of 64 or 128 channels, at most 16 to a KV head, blocks of 16 to 256 tokens (a power of two)"
         self.S = int(max_num_seqs)
         self.max_batched = int(max_num_batched_tokens)
         self.max_model_len = int(max_model_len)
@@ -148,7 +164,7 @@ class RolloutEngine:
         self.model.kv_hook = self._prefill_kv_hook
         if not cfg.is_stack:
             self.model.decode_kernels = not cfg.is_moe
-        self.cache = make_cache(cfg, params.flat.dtype, self.device, self.bs, self.S, self.tp_size)
+        self.cache = make_cache(cfg, params.flat.dtype, self.device, self.bs, self.S, self.tp_size, self.kv4)
         self.sequences: dict[str, _Sequence] = {}
         self._tp_share = None
         if self.tp_size > 1:
@@ -310,6 +326,8 @@ class RolloutEngine:
         self.block_table = torch.zeros(S, self.max_blocks_per_seq, dtype=torch.int32, device=dev)
         self.out_cap = 0
         self.out_tok = self.out_lp = None
+        self.n_top = 0              # alternatives recorded per position by the running wave
+        self.out_top_ids = self.out_top_lp = self.out_ent = None
         self.temperature = 1.0
         self.top_k, self.top_p = -1, 1.0
         self.free_slots = list(range(S - 1, -1, -1))
@@ -322,7 +340,7 @@ class RolloutEngine:
         nkv_l = self.cfg.num_key_value_heads // self.tp_size
         # VERL_B200_FUSED_ROPE_APPEND=0: rotate q, rotate k and append to the cache as three launches instead of one
         self.fused_rope_append = os.environ.get("VERL_B200_FUSED_ROPE_APPEND", "1") != "0"
-        self.grouped_decode = (self.is_cuda and self.share_prefill and not self.cfg.is_stack and self.bs == 64 and self.cfg.head_dim in (64, 128)
+        self.grouped_decode = (self.is_cuda and self.share_prefill and not self.cfg.is_stack and not self.kv4 and self.bs == 64 and self.cfg.head_dim in (64, 128)
                                and nh_l // max(1, nkv_l) <= 16 and os.environ.get("VERL_B200_GROUPED_DECODE", "0") == "1")
         self._groups: dict[int, list[int]] = {}
         self._slot_group: dict[int, int] = {}
@@ -394,7 +412,18 @@ class RolloutEngine:
             if self.record_routing:
                 self.out_routed = torch.zeros(self.S, self.out_cap, self.cfg.num_hidden_layers, self.cfg.num_experts_per_tok,
                                               dtype=torch.int16, device=self.device)
+            self.out_top_ids = None
             self._graph = None
+        if self.n_top and (self.out_top_ids is None or self.out_top_ids.shape[2] != self.n_top):
+            assert not self.running, "the number of recorded alternatives can only change while idle"
+            self.out_top_ids = torch.zeros(self.S, self.out_cap, self.n_top, dtype=torch.int64, device=self.device)
+            self.out_top_lp = torch.zeros(self.S, self.out_cap, self.n_top, dtype=torch.float32, device=self.device)
+            self.out_ent = torch.zeros(self.S, self.out_cap, dtype=torch.float32, device=self.device)
+            self._graph = None
+
+    def _score(self, logits: torch.Tensor, tok: torch.Tensor) -> F.TokenScores:
+        """The record of a position: most likely tokens and entropy under the sampling temperature (greedy: 1)."""
+        return F.token_scores(logits, tok, self.n_top, self.temperature if self.temperature > 0 else 1.0, self.valid_vocab)
 
     # ------------------------------------------------------------------------------------ requests
     def add_request(self, prompt_ids: Sequence[int], params: SamplingParams, request_id: Optional[str] = None) -> str:
@@ -404,6 +433,8 @@ class RolloutEngine:
         assert 0 < len(prompt) < self.max_model_len, f"prompt of {len(prompt)} tokens does not fit max_model_len"
         p = SamplingParams(**{**params.__dict__})
         p.max_tokens = max(1, min(p.max_tokens, self.max_model_len - len(prompt)))
+        if not 0 <= p.top_logprobs <= min(F.TOP_K_LIMIT, self.valid_vocab):
+            raise ValueError(f"top_logprobs must lie in 0 .. {min(F.TOP_K_LIMIT, self.valid_vocab)}, got {p.top_logprobs}")
         self.waiting.append(_Request(rid, prompt, p, arrival=time.time()))
         return rid
 
@@ -427,7 +458,9 @@ class RolloutEngine:
 
     # ------------------------------------------------------------------------------------ prefill
     def _prefill_kv_hook(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
-        if self._prefill_slots is not None:
+        if self._prefill_slots is not None and self.kv4:
+            F.kv4_append_(k, v, self._prefill_slots, self.kv[layer])
+        elif self._prefill_slots is not None:
             F.kv_append_(k, v, self._prefill_slots, self.kv[layer, 0], self.kv[layer, 1])
 
     _prefill_slots: Optional[torch.Tensor] = None
@@ -451,12 +484,12 @@ class RolloutEngine:
             if need - len(hit) > len(self.free_blocks) + len(self._idle_cached) - idle_hit or \
                     (batch and tokens + len(r.prompt) - len(hit) * self.bs > self.max_batched):
                 break
-            want = (r.params.temperature, r.params.top_k, r.params.top_p)
+            want = (r.params.temperature, r.params.top_k, r.params.top_p, r.params.top_logprobs)
             idle = not self.running and not batch
             if idle:
-                self.temperature, self.top_k, self.top_p = want  # one sampling configuration per running wave
+                self.temperature, self.top_k, self.top_p, self.n_top = want  # one sampling configuration per running wave
                 self._ensure_out(r.params.max_tokens)
-            elif want != (self.temperature, self.top_k, self.top_p) or r.params.max_tokens > self.out_cap:
+            elif want != (self.temperature, self.top_k, self.top_p, self.n_top) or r.params.max_tokens > self.out_cap:
                 break
             self.waiting.popleft()
             r.slot = self.free_slots.pop()
@@ -492,6 +525,8 @@ class RolloutEngine:
                 out[r.rid] = dict(prompt=list(r.prompt), **self.cache.export(blk, r.slot), token=int(self.tok[r.slot]),
                                   logprob=float(self.out_lp[r.slot, 0]), seed=int(self.seeds[r.slot]), block_size=self.bs,
                                   routed_prompt=getattr(r, "routed_prompt", None))
+                if self.n_top:
+                    out[r.rid]["top"] = tuple(t[r.slot, 0].clone() for t in (self.out_top_ids, self.out_top_lp, self.out_ent))
             idx = torch.tensor([r.slot for r in reqs], dtype=torch.int64, device=self.device)
             for r in reqs:
                 self.running.pop(r.slot)
@@ -513,9 +548,8 @@ class RolloutEngine:
     def _install_prefilled(self, reqs: list[_Request]) -> None:
         dev = self.device
         lens = [len(r.prompt) for r in reqs]
-        bt_rows = torch.zeros(len(reqs), self.max_blocks_per_seq, dtype=torch.int32)
+        self._write_tables([r.slot for r in reqs], [r.blocks for r in reqs])
         for i, r in enumerate(reqs):
-            bt_rows[i, : len(r.blocks)] = torch.tensor(r.blocks, dtype=torch.int32)
             nb = (lens[i] + self.bs - 1) // self.bs
             dst = torch.tensor(r.blocks[:nb], dtype=torch.int64, device=dev)
             self.cache.install(dst, r.slot, r.handoff)   # the KV transfer (a peer copy between GPUs)
@@ -540,7 +574,6 @@ class RolloutEngine:
             for r in reqs:
                 self.seen[r.slot, torch.tensor(r.prompt + [r.handoff["token"]], dtype=torch.int64, device=dev)] = True
         n = torch.tensor(lens, dtype=torch.int32, device=dev)
-        self.block_table[slots] = bt_rows.to(dev)
         self.tok[slots] = tok
         self.pos[slots] = n
         self.ctx[slots] = n + 1
@@ -550,6 +583,10 @@ class RolloutEngine:
         self.seeds[slots] = torch.tensor([r.handoff["seed"] for r in reqs], dtype=torch.int64, device=dev)
         self.out_tok[slots, 0] = tok
         self.out_lp[slots, 0] = lp
+        for r in reqs if self.n_top else ():
+            assert "top" in r.handoff and r.handoff["top"][0].numel() == self.n_top, "the prefill engine must record as many alternatives"
+            for buf, t in zip((self.out_top_ids, self.out_top_lp, self.out_ent), r.handoff["top"]):
+                buf[r.slot, 0] = t.to(dev)
         done = (self.gen[slots] >= self.max_new[slots])
         if self.eos is not None:
             done |= (tok == self.eos) & ~self.ignore_eos[slots]
@@ -558,36 +595,38 @@ class RolloutEngine:
         for r in reqs:
             self.running[r.slot] = r
 
+    def _write_tables(self, slots: Sequence[int], blocks: Sequence[Sequence[int]]) -> None:
+        """The block tables of some sequence slots, from their block lists (one transfer and one launch)."""
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32).to(self.device)
+        F.extend_block_tables_(self.block_table, i32(list(slots)), torch.zeros(len(slots), dtype=torch.int32, device=self.device),
+                               i32([len(b) * self.bs for b in blocks]), i32([b for row in blocks for b in row]), self.bs)
+
     @torch.no_grad()
-    def _run_portions(self, ids: torch.Tensor, starts: list[int], ends: list[int], bt_rows: torch.Tensor, slots: list[int]):
+    def _run_portions(self, ids: torch.Tensor, starts: list[int], ends: list[int], slots: list[int]):
         """Tokens ``starts[i] .. ends[i]`` of every sequence (packed in ``ids``, host) through the model in one batch, appended to
-        the cache behind the ``starts[i]`` tokens it already holds. ``bt_rows`` [B, blocks] (host): the sequences' block tables;
-        ``slots``: their slots. Returns (final hidden states [T, H], the packed batch)."""
+        the cache behind the ``starts[i]`` tokens it already holds. ``slots``: the sequences' slots, whose block tables are written.
+        Returns (final hidden states [T, H], the packed batch)."""
         dev = self.device
-        slot_rows = []
-        for i, (a, b) in enumerate(zip(starts, ends)):
-            p = torch.arange(a, b)
-            slot_rows.append(bt_rows[i, p // self.bs].long() * self.bs + p % self.bs)
-        slot_map = torch.cat(slot_rows)
         if self.is_cuda:
-            ids, slot_map = ids.pin_memory().to(dev, non_blocking=True), slot_map.pin_memory().to(dev, non_blocking=True)
+            ids = ids.pin_memory().to(dev, non_blocking=True)
         batch = PackedBatch.from_lengths(ids, [b - a for a, b in zip(starts, ends)], device=dev)
+        rows, a, b, zero = torch.tensor([list(slots), list(starts), list(ends), [0] * len(slots)], dtype=torch.int32).to(dev)
+        _, positions, slot_map = F.build_slot_map(self.block_table, rows, a, b, self.bs, sum(ends) - sum(starts))
         if any(starts):
-            batch.positions = torch.cat([torch.arange(a, b, dtype=torch.int32) for a, b in zip(starts, ends)]).to(dev)
+            batch.positions = positions
         if self.cfg.is_stack:
             from ....models.mixer_stack import PortionCache
 
-            pc = PortionCache(self.cache, slot_map, torch.tensor(slots, dtype=torch.int32).to(dev), list(starts), bt_rows.to(dev))
+            pc = PortionCache(self.cache, slot_map, rows, list(starts), self.block_table[rows.long()])
             return self.model.forward_hidden(batch, pc), batch
         if any(starts):
-            rows = []
-            for i, a in enumerate(starts):
-                p = torch.arange(a)
-                rows.append(bt_rows[i, p // self.bs].long() * self.bs + p % self.bs)
-            cached_slots = torch.cat(rows).to(dev)
-            nkv_l, hd = self.kv.shape[-2], self.kv.shape[-1]
-            self.model.prefix_kv = lambda layer: (self.kv[layer, 0].view(-1, nkv_l, hd)[cached_slots],
-                                                  self.kv[layer, 1].view(-1, nkv_l, hd)[cached_slots], list(starts))
+            cached_slots = F.build_slot_map(self.block_table, rows, zero, a, self.bs, sum(starts))[2]
+            if self.kv4:
+                self.model.prefix_kv = lambda layer: (*F.kv4_gather(self.kv[layer], cached_slots, self.cfg.head_dim, self.params.flat.dtype), list(starts))
+            else:
+                nkv_l, hd = self.kv.shape[-2], self.kv.shape[-1]
+                self.model.prefix_kv = lambda layer: (self.kv[layer, 0].view(-1, nkv_l, hd)[cached_slots],
+                                                      self.kv[layer, 1].view(-1, nkv_l, hd)[cached_slots], list(starts))
             self.model._ensure_rope(max(ends) + 1)
         self._prefill_slots = slot_map
         try:
@@ -634,9 +673,7 @@ class RolloutEngine:
                 r.blocks[:nfull] = shared
                 for b in shared:
                     self._block_users[b] = self._block_users.get(b, 1) + 1
-        bt_rows = torch.zeros(len(reqs), self.max_blocks_per_seq, dtype=torch.int32)
-        for i, r in enumerate(reqs):
-            bt_rows[i, : len(r.blocks)] = torch.tensor(r.blocks, dtype=torch.int32)
+        self._write_tables([r.slot for r in reqs], [r.blocks for r in reqs])
         skip = [reqs[i].cached for i in leaders]        # tokens whose pages came from the prefix cache: not recomputed
         ids = torch.tensor([t for i in leaders for t in reqs[i].prompt[reqs[i].cached:]], dtype=torch.int64)
         if any(skip):
@@ -645,7 +682,7 @@ class RolloutEngine:
             from ....models.decoder import RouterReplay
 
             self.model.router_replay = RouterReplay("record")
-        h, batch = self._run_portions(ids, skip, [lens[i] for i in leaders], bt_rows[leaders], [reqs[i].slot for i in leaders])
+        h, batch = self._run_portions(ids, skip, [lens[i] for i in leaders], [reqs[i].slot for i in leaders])
         if self.enable_prefix_caching:
             for i in leaders:
                 self._index_pages(reqs[i].prompt, reqs[i].blocks, lens[i])
@@ -696,10 +733,11 @@ class RolloutEngine:
                 self.seen[r.slot, torch.tensor(r.prompt, dtype=torch.int64, device=dev)] = True
             logits = self._penalise(logits, slots)
         tok, lp = F.sample_tokens(logits, self.temperature, seeds, 0, self.valid_vocab, self.top_k, self.top_p)
+        if self.n_top:
+            first = self._score(logits, tok)
         if self._use_penalty:
             self.seen[slots, tok] = True
         n = torch.tensor(lens, dtype=torch.int32, device=dev)
-        self.block_table[slots] = bt_rows.to(dev)
         if len(leaders) < len(reqs):
             self._form_groups(reqs, leaders, lead_idx, lens)
         self.tok[slots] = tok
@@ -711,6 +749,8 @@ class RolloutEngine:
         self.seeds[slots] = seeds * 6364136223846793005 + 1442695040888963407
         self.out_tok[slots, 0] = tok
         self.out_lp[slots, 0] = lp
+        if self.n_top:
+            self.out_top_ids[slots, 0], self.out_top_lp[slots, 0], self.out_ent[slots, 0] = first.top_ids, first.top_logprob, first.entropy
         done = (self.gen[slots] >= self.max_new[slots])
         if self.eos is not None:
             done |= (tok == self.eos) & ~self.ignore_eos[slots]
@@ -737,11 +777,7 @@ class RolloutEngine:
         cfg, P = self.cfg, self.params
         S = self.S
         act = self.active
-        acti = act.to(torch.int32)
-        pos_l = self.pos.long()
-        blk = torch.gather(self.block_table, 1, (pos_l // self.bs).unsqueeze(1)).squeeze(1).long()
-        slot_map = torch.where(act, blk * self.bs + pos_l % self.bs, torch.full_like(pos_l, -1))
-        ctx_eff = self.ctx * acti
+        slot_map, ctx_eff, plan = F.decode_slot_map(self.block_table, self.pos, self.ctx, act, self.bs)
         if cfg.is_stack:
             return self.model.decode_hidden(self.tok, self.pos, slot_map, ctx_eff, act, self.block_table, self.cache)
         tp = self.model.tp
@@ -766,7 +802,14 @@ class RolloutEngine:
             q = qkv[:, :Q].view(S, nh, hd)
             k = qkv[:, Q : Q + KV].view(S, nkv, hd)
             v = qkv[:, Q + KV :].view(S, nkv, hd)
-            if cfg.qk_norm:  # one launch: norm and rotation of q and k in the projection output, append of k and v to the cache
+            if self.kv4:
+                if cfg.qk_norm:
+                    F.qk_norm_rope_(qkv, self.pos, cos, sin, W["self_attn.q_norm.weight"], W["self_attn.k_norm.weight"], cfg.rms_norm_eps, nh, nkv, hd)
+                else:
+                    F.apply_rope_(q, self.pos, cos, sin)
+                    F.apply_rope_(k, self.pos, cos, sin)
+                F.kv4_append_(k, v, slot_map, self.kv[i])
+            elif cfg.qk_norm:  # one launch: norm and rotation of q and k in the projection output, append of k and v to the cache
                 F.qk_norm_rope_(qkv, self.pos, cos, sin, W["self_attn.q_norm.weight"], W["self_attn.k_norm.weight"], cfg.rms_norm_eps,
                                 nh, nkv, hd, slot_map, self.kv[i, 0], self.kv[i, 1])
             elif not qkv.is_contiguous() or not self.fused_rope_append:
@@ -775,7 +818,10 @@ class RolloutEngine:
                 F.kv_append_(k, v, slot_map, self.kv[i, 0], self.kv[i, 1])
             else:  # one launch: rotate q and k in the projection output, append k and v to the cache
                 F.rope_kv_append_(qkv, self.pos, cos, sin, slot_map, self.kv[i, 0], self.kv[i, 1], nh, nkv, hd)
-            attn = F.paged_decode_attention(q, self.kv[i, 0], self.kv[i, 1], self.block_table, ctx_eff, groups=pd_groups)
+            if self.kv4:
+                attn = F.paged_decode_attention_kv4(q, self.kv[i], self.block_table, ctx_eff, plan=plan)
+            else:
+                attn = F.paged_decode_attention(q, self.kv[i, 0], self.kv[i, 1], self.block_table, ctx_eff, groups=pd_groups)
             if tp is not None:
                 o = tp.row_linear(attn.reshape(S, Q), W["self_attn.o_proj.weight"][:, tp.rows(cfg.q_size)], None)
             else:
@@ -793,7 +839,7 @@ class RolloutEngine:
         acti = act.to(torch.int32)
         tp = self.model.tp
         hN = self._decode_hidden()
-        if tp is not None and self._tp_share is not None and not self._use_penalty:
+        if tp is not None and self._tp_share is not None and not self._use_penalty and not self.n_top:
             sh = S // tp.size
             mine = slice(tp.rank * sh, (tp.rank + 1) * sh)
             logits = F.gemm(hN[mine], P.lm_head_weight)
@@ -819,6 +865,11 @@ class RolloutEngine:
         col = self.gen.long().clamp(max=self.out_cap - 1)
         self.out_tok[rows, col] = torch.where(act, tok, self.out_tok[rows, col])
         self.out_lp[rows, col] = torch.where(act, lp, self.out_lp[rows, col])
+        if self.n_top:
+            rec = self._score(logits, tok)
+            self.out_top_ids[rows, col] = torch.where(act[:, None], rec.top_ids, self.out_top_ids[rows, col])
+            self.out_top_lp[rows, col] = torch.where(act[:, None], rec.top_logprob, self.out_top_lp[rows, col])
+            self.out_ent[rows, col] = torch.where(act, rec.entropy, self.out_ent[rows, col])
         self.gen.add_(acti)
         done = self.gen >= self.max_new
         if self.eos is not None:
@@ -841,12 +892,14 @@ class RolloutEngine:
             for _ in range(n):
                 self._decode_body()
         else:
-            key = (self.temperature, self.top_k, self.top_p, self.out_cap, id(self.kv))
+            key = (self.temperature, self.top_k, self.top_p, self.n_top, self.out_cap, id(self.kv))
             if self._graph is None or self._graph_key != key:
                 # what a step changes and the first replay has to find as it is now (cached keys and recorded routing are written again alike)
                 kept = [self.tok, self.pos, self.ctx, self.gen, self.active, self.seeds, self.out_tok, self.out_lp]
                 if self._use_penalty:
                     kept.append(self.seen)
+                if self.n_top:
+                    kept += [self.out_top_ids, self.out_top_lp, self.out_ent]
                 snap = [t.clone() for t in kept]
                 side = torch.cuda.Stream(device=self.device)
                 side.wait_stream(torch.cuda.current_stream(self.device))
@@ -898,6 +951,7 @@ class RolloutEngine:
         toks = self.out_tok[idx].cpu()
         lps = self.out_lp[idx].cpu()
         routed = self.out_routed[idx].cpu() if self.record_routing else None
+        record = [t[idx].cpu() for t in (self.out_top_ids, self.out_top_lp, self.out_ent)] if self.n_top else None
         for j, s in enumerate(done_slots):
             r = self.running.pop(s)
             n = int(gen[s])
@@ -911,6 +965,8 @@ class RolloutEngine:
             else:
                 reason = "length"
             extra = {}
+            if record is not None:  # per generated token: [n, top_logprobs] and [n]
+                extra["top_token_ids"], extra["top_logprobs"], extra["entropy"] = (t[j, :n].clone() for t in record)
             if routed is not None:
                 # prompt tokens, then every generated token that was fed back (all but the last one)
                 extra["routed_experts"] = torch.cat([r.routed_prompt, routed[j, : max(n - 1, 0)]], 0)
@@ -955,13 +1011,14 @@ class RolloutEngine:
             assert need <= len(self.free_blocks) + len(self._idle_cached), "the cache is full"
             q.blocks += [self._take_block() for _ in range(need)]
             (singles if len(tokens) == 1 and q.length > 0 else prompts).append(j)
-        table = lambda js: torch.stack([torch.nn.functional.pad(torch.tensor(self.sequences[entries[j][0]].blocks, dtype=torch.int32),
-                                                                (0, self.max_blocks_per_seq - len(self.sequences[entries[j][0]].blocks))) for j in js])
+        open_ = [self.sequences[key] for key, _, _ in entries]
+        if entries:
+            self._write_tables([q.slot for q in open_], [q.blocks for q in open_])
         if prompts:
             seqs = [self.sequences[entries[j][0]] for j in prompts]
             n = [len(entries[j][1]) for j in prompts]
             ids = torch.tensor([int(t) for j in prompts for t in entries[j][1]], dtype=torch.int64)
-            h, _ = self._run_portions(ids, [q.length for q in seqs], [q.length + c for q, c in zip(seqs, n)], table(prompts), [q.slot for q in seqs])
+            h, _ = self._run_portions(ids, [q.length for q in seqs], [q.length + c for q, c in zip(seqs, n)], [q.slot for q in seqs])
             rows, row0 = [], 0
             for j, c in zip(prompts, n):
                 rows += [row0 + int(w) for w in entries[j][2]]
@@ -976,7 +1033,6 @@ class RolloutEngine:
             seqs = [self.sequences[entries[j][0]] for j in singles]
             slots = torch.tensor([q.slot for q in seqs], dtype=torch.int64, device=self.device)
             pos = torch.tensor([q.length for q in seqs], dtype=torch.int32, device=self.device)
-            self.block_table[slots] = table(singles).to(self.device)
             self.tok[slots] = torch.tensor([int(entries[j][1][0]) for j in singles], dtype=torch.int64, device=self.device)
             self.pos[slots] = pos
             self.ctx[slots] = pos + 1
