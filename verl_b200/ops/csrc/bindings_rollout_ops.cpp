@@ -6,6 +6,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <tuple>
 
 #include "rollout_ops.h"
@@ -19,16 +20,22 @@ inline cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().strea
 inline long long* lptr(const Tensor& t) { return reinterpret_cast<long long*>(t.data_ptr<int64_t>()); }
 #define CHECK_RC(rc, what) TORCH_CHECK((rc) == 0, what " failed with code ", (rc))
 
+// What the host form refuses with a ValueError is refused alike here; what only a GPU cannot take (a type, another device) is a RuntimeError.
+
 // A vector of n whole numbers on the device of `like`.
 void check_vec(const Tensor& t, at::ScalarType type, int64_t n, const Tensor& like, const char* what) {
-  TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.scalar_type() == type && t.dim() == 1 && t.size(0) == n && t.is_contiguous(), what,
-              ": expected a contiguous ", type, " vector of ", n, " on ", like.device(), ", got ", t.scalar_type(), " ", t.sizes(), " on ", t.device());
+  TORCH_CHECK_VALUE(t.scalar_type() == type && t.dim() == 1 && t.size(0) == n, what, ": expected a ", type, " vector of ", n, ", got ", t.scalar_type(), " ",
+                    t.sizes());
+  TORCH_CHECK(t.device() == like.device() && t.is_contiguous(), what, ": expected a contiguous vector on ", like.device(), ", got one on ", t.device());
 }
+int64_t length(const Tensor& t) { return t.dim() == 1 ? t.size(0) : -1; }
 void check_table(const Tensor& t, const char* what) {
-  TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kInt && t.dim() == 2 && t.stride(1) == 1 && t.size(0) <= INT_MAX && t.size(1) <= INT_MAX, what,
-              ": block_table must be a CUDA int32 matrix with contiguous rows");
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kInt && t.dim() == 2, what, ": block_table must be an int32 matrix [rows, blocks], got ", t.scalar_type(), " ", t.sizes());
+  TORCH_CHECK(t.is_cuda() && (t.stride(1) == 1 || t.size(1) <= 1) && t.size(0) <= INT_MAX && t.size(1) <= INT_MAX, what,
+              ": block_table must be a CUDA matrix with contiguous rows");
 }
 int type_of(const Tensor& t, bool f32, const char* what) {
+  TORCH_CHECK_VALUE(at::isFloatingType(t.scalar_type()), what, ": expected floating numbers, got ", t.scalar_type());
   TORCH_CHECK(t.is_cuda(), what, ": expected a CUDA tensor");
   if (t.scalar_type() == at::kBFloat16) return 0;
   if (t.scalar_type() == at::kHalf) return 1;
@@ -54,11 +61,11 @@ std::tuple<Tensor, Tensor, Tensor> decode_slot_map(const Tensor& table, const Te
 
 Tensor extend_block_tables_(Tensor table, const Tensor& rows, const Tensor& have, const Tensor& lengths, const Tensor& pool, int64_t bs) {
   check_table(table, "extend_block_tables_");
-  const int64_t B = rows.size(0);
+  const int64_t B = length(rows);
   check_vec(rows, at::kInt, B, table, "extend_block_tables_: rows");
   check_vec(have, at::kInt, B, table, "extend_block_tables_: have");
   check_vec(lengths, at::kInt, B, table, "extend_block_tables_: lengths");
-  check_vec(pool, at::kInt, pool.size(0), table, "extend_block_tables_: pool");
+  check_vec(pool, at::kInt, length(pool), table, "extend_block_tables_: pool");
   TORCH_CHECK(bs > 0 && bs <= (1 << 20) && table.size(1) <= (1 << 20) && B <= (1 << 20) && pool.size(0) <= INT_MAX,
               "extend_block_tables_: at most 2^20 rows of at most 2^20 blocks");
   const c10::cuda::CUDAGuard guard(table.device());
@@ -75,12 +82,13 @@ Tensor extend_block_tables_(Tensor table, const Tensor& rows, const Tensor& have
 std::tuple<Tensor, Tensor, Tensor> build_slot_map(const Tensor& table, const Tensor& rows, const Tensor& starts, const Tensor& ends, int64_t bs,
                                                   int64_t total) {
   check_table(table, "build_slot_map");
-  const int64_t B = rows.size(0);
+  const int64_t B = length(rows);
   check_vec(rows, at::kInt, B, table, "build_slot_map: rows");
   check_vec(starts, at::kInt, B, table, "build_slot_map: starts");
   check_vec(ends, at::kInt, B, table, "build_slot_map: ends");
   TORCH_CHECK(bs > 0 && bs <= (1 << 20), "build_slot_map: block_size");
-  TORCH_CHECK(total >= 0 && total <= (1 << 22) && B <= 8192, "build_slot_map: at most 2^22 tokens of at most 8192 sequences, got ", total, " of ", B);
+  TORCH_CHECK_VALUE(total >= 0, "build_slot_map: total must not be negative, got ", total);
+  TORCH_CHECK(total <= (1 << 22) && B <= 8192, "build_slot_map: at most 2^22 tokens of at most 8192 sequences, got ", total, " of ", B);
   const c10::cuda::CUDAGuard guard(table.device());
   Tensor cu = at::empty({B + 1}, table.options()), positions = at::empty({total}, table.options()),
          slots = at::empty({total}, table.options().dtype(at::kLong));
@@ -94,23 +102,26 @@ std::tuple<Tensor, Tensor, Tensor> build_slot_map(const Tensor& table, const Ten
 
 // Block size of a 4-bit pool [blocks, heads, bytes of a page] for heads of hd channels.
 int64_t kv4_block(const Tensor& pages, int64_t hd, const char* what) {
-  TORCH_CHECK(pages.is_cuda() && pages.scalar_type() == at::kByte && pages.dim() == 3 && pages.is_contiguous() &&
-              reinterpret_cast<uintptr_t>(pages.data_ptr()) % 16 == 0, what, ": pages must be a contiguous CUDA uint8 tensor [blocks, heads, page bytes]");
-  TORCH_CHECK(hd > 0 && hd % 32 == 0 && hd <= 1024, what, ": heads of a multiple of 32 channels, got ", hd);
+  TORCH_CHECK_VALUE(pages.scalar_type() == at::kByte && pages.dim() == 3 && pages.is_contiguous(), what,
+                    ": pages must be a contiguous uint8 tensor [blocks, kv_heads, page bytes], got ", pages.scalar_type(), " ", pages.sizes());
+  TORCH_CHECK_VALUE(hd > 0 && hd % 32 == 0 && hd <= 1024, what, ": heads of a multiple of 32 channels, at most 1024, got ", hd);
   const int64_t bs = pages.size(2) * 4 / (5 * hd);
-  TORCH_CHECK(bs > 0 && bs * hd * 5 == pages.size(2) * 4 && bs % 16 == 0, what, ": pages of ", pages.size(2),
-              " bytes hold no multiple of 16 tokens of a head of ", hd);
-  TORCH_CHECK(bs <= 1024, what, ": blocks of at most 1024 tokens");
+  TORCH_CHECK_VALUE(bs > 0 && bs * hd * 5 == pages.size(2) * 4 && bs % 16 == 0 && bs <= 1024, what, ": pages of ", pages.size(2),
+                    " bytes hold no multiple of 16 tokens, at most 1024, of a head of ", hd);
+  TORCH_CHECK(pages.is_cuda() && reinterpret_cast<uintptr_t>(pages.data_ptr()) % 16 == 0 && pages.size(0) * bs <= INT_MAX, what,
+              ": pages must lie on a CUDA device and hold fewer than 2^31 tokens");
   return bs;
 }
 
 void kv4_append_(const Tensor& k, const Tensor& v, const Tensor& slots, Tensor pages) {
+  TORCH_CHECK_VALUE(v.scalar_type() == k.scalar_type() && k.dim() == 3 && v.sizes() == k.sizes(),
+                    "kv4_append_: k and v must be [tokens, heads, channels] of one floating type, got ", k.scalar_type(), " ", k.sizes(), ", ", v.scalar_type(), " ",
+                    v.sizes());
   const int type = type_of(k, false, "kv4_append_");
-  TORCH_CHECK(v.scalar_type() == k.scalar_type() && v.device() == k.device() && k.device() == pages.device() && k.dim() == 3 && v.sizes() == k.sizes(),
-              "kv4_append_: k and v [tokens, heads, channels] of one type on the device of the pages");
   const int64_t T = k.size(0), nkv = k.size(1), hd = k.size(2);
   const int64_t bs = kv4_block(pages, hd, "kv4_append_");
-  TORCH_CHECK(pages.size(1) == nkv, "kv4_append_: the pages hold ", pages.size(1), " heads, k has ", nkv);
+  TORCH_CHECK_VALUE(pages.size(1) == nkv, "kv4_append_: the pool holds ", pages.size(1), " heads, k has ", nkv);
+  TORCH_CHECK(v.device() == k.device() && pages.device() == k.device() && T <= INT_MAX, "kv4_append_: k, v and the pages on one device");
   check_vec(slots, at::kLong, T, k, "kv4_append_: slots");
   if (T == 0 || nkv == 0 || pages.size(0) == 0) return;
   for (const Tensor* t : {&k, &v})
@@ -124,7 +135,7 @@ void kv4_append_(const Tensor& k, const Tensor& v, const Tensor& slots, Tensor p
 }
 
 std::tuple<Tensor, Tensor> kv4_gather(const Tensor& pages, const Tensor& slots, int64_t hd, at::ScalarType dtype) {
-  const int64_t bs = kv4_block(pages, hd, "kv4_gather"), T = slots.size(0), nkv = pages.size(1);
+  const int64_t bs = kv4_block(pages, hd, "kv4_gather"), T = length(slots), nkv = pages.size(1);
   TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kHalf, "kv4_gather: bf16 or fp16");
   check_vec(slots, at::kLong, T, pages, "kv4_gather: slots");
   const c10::cuda::CUDAGuard guard(pages.device());
@@ -139,24 +150,27 @@ std::tuple<Tensor, Tensor> kv4_gather(const Tensor& pages, const Tensor& slots, 
 
 Tensor paged_decode_kv4(const Tensor& q, const Tensor& pages, const Tensor& table, const Tensor& ctx, const OptTensor& plan, double scale) {
   VbKv4Decode a{};
-  a.type = type_of(q, false, "paged_decode_kv4");
-  TORCH_CHECK(q.dim() == 3 && (q.size(2) == 64 || q.size(2) == 128), "paged_decode_kv4: q [sequences, heads, 64 or 128 channels]");
-  const int64_t B = q.size(0), nh = q.size(1), hd = q.size(2), bs = kv4_block(pages, hd, "paged_decode_kv4"), nkv = pages.size(1);
-  TORCH_CHECK(pages.device() == q.device() && table.device() == q.device(), "paged_decode_kv4: tensors on several devices");
-  TORCH_CHECK(nkv > 0 && nh > 0 && nh % nkv == 0 && nh / nkv <= 16, "paged_decode_kv4: at most 16 query heads to a key head, got ", nh, " / ", nkv);
-  TORCH_CHECK((bs & (bs - 1)) == 0 && bs <= 256, "paged_decode_kv4: blocks of 16, 32, 64, 128 or 256 tokens, got ", bs);
-  check_table(table, "paged_decode_kv4");
-  TORCH_CHECK(table.size(0) == B && pages.size(0) <= INT_MAX && B <= 65535, "paged_decode_kv4: one table row for each of at most 65535 sequences");
-  TORCH_CHECK(table.size(1) * bs <= (1LL << 30) && (table.size(1) * bs + 63) / 64 * B * nkv <= (1LL << 30) - 1, "paged_decode_kv4: a table of ", B, " x ",
+  TORCH_CHECK_VALUE(q.dim() == 3, "paged_decode_attention_kv4: q must be [sequences, heads, channels], got ", q.sizes());
+  a.type = type_of(q, false, "paged_decode_attention_kv4");
+  const int64_t B = q.size(0), nh = q.size(1), hd = q.size(2), bs = kv4_block(pages, hd, "paged_decode_attention_kv4"), nkv = pages.size(1);
+  check_table(table, "paged_decode_attention_kv4");
+  TORCH_CHECK_VALUE(nkv > 0 && nh > 0 && nh % nkv == 0 && table.size(0) == B, "paged_decode_attention_kv4: ", B, " sequences of ", nh, " heads against tables of ",
+                    table.size(0), " rows and ", nkv, " KV heads");
+  check_vec(ctx, at::kInt, B, q, "paged_decode_attention_kv4: ctx_len");
+  if (plan.has_value()) check_vec(*plan, at::kInt, B + 1, q, "paged_decode_attention_kv4: plan");
+  TORCH_CHECK(pages.device() == q.device() && table.device() == q.device(), "paged_decode_attention_kv4: tensors on several devices");
+  TORCH_CHECK((hd == 64 || hd == 128) && nh / nkv <= 16, "paged_decode_attention_kv4: heads of 64 or 128 channels, at most 16 to a KV head, got ", nh, " / ", nkv,
+              " of ", hd);
+  TORCH_CHECK((bs & (bs - 1)) == 0 && bs <= 256, "paged_decode_attention_kv4: blocks of 16, 32, 64, 128 or 256 tokens, got ", bs);
+  TORCH_CHECK(B <= 65535, "paged_decode_attention_kv4: at most 65535 sequences, got ", B);
+  TORCH_CHECK(table.size(1) * bs <= (1LL << 30) && (table.size(1) * bs + 63) / 64 * B * nkv <= (1LL << 30) - 1, "paged_decode_attention_kv4: a table of ", B, " x ",
               table.size(1), " blocks of ", bs, " is more than the kernel counts in 30 bits");
-  check_vec(ctx, at::kInt, B, q, "paged_decode_kv4: ctx_len");
-  if (plan.has_value()) check_vec(*plan, at::kInt, B + 1, q, "paged_decode_kv4: plan");
   const c10::cuda::CUDAGuard guard(q.device());
   Tensor out = at::empty({B, nh, hd}, q.options());
   if (B == 0) return out;
   if (pages.size(0) == 0 || table.size(1) == 0) return out.zero_();
   TORCH_CHECK(q.stride(2) == 1 && q.stride(1) == hd && (B == 1 || q.stride(0) % 8 == 0) && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
-              "paged_decode_kv4: heads of a sequence side by side, sequences on 16-byte boundaries");
+              "paged_decode_attention_kv4: heads of a sequence side by side, sequences on 16-byte boundaries");
   a.q = q.data_ptr(); a.ldq = B == 1 ? 0 : q.stride(0);
   a.pages = pages.data_ptr<uint8_t>(); a.num_blocks = (int)pages.size(0); a.block_size = (int)bs;
   a.table = table.data_ptr<int>(); a.width = (int)table.size(1); a.ldt = table.stride(0);
@@ -178,25 +192,29 @@ Tensor paged_decode_kv4(const Tensor& q, const Tensor& pages, const Tensor& tabl
   return out;
 }
 
+// Logits with contiguous rows, and what the kernels are told about them. `valid` 0: all columns.
 VbScores scores_of(const Tensor& x, const Tensor& ids, double temperature, int64_t valid, const char* what) {
   VbScores a{};
+  TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) > 0, what, ": logits must be [rows, vocabulary], got ", x.sizes());
+  TORCH_CHECK_VALUE(ids.scalar_type() == at::kLong && (ids.dim() == 1 || ids.dim() == 2) && ids.size(0) == x.size(0), what, ": ids must be int64 [", x.size(0),
+                    "] or [", x.size(0), ", n], got ", ids.scalar_type(), " ", ids.sizes());
+  TORCH_CHECK_VALUE(ids.dim() == 1 || ids.size(1) <= 4096, what, ": at most 4096 given tokens a row, got ", ids.size(1));
+  TORCH_CHECK_VALUE(temperature > 0, what, ": temperature must be positive, got ", temperature);
+  TORCH_CHECK_VALUE(valid >= 0 && valid <= x.size(1), what, ": valid_vocab must lie in 0 .. ", x.size(1), ", got ", valid);
   a.type = type_of(x, true, what);
-  TORCH_CHECK(x.dim() == 2 && (x.stride(1) == 1 || x.size(1) <= 1) && x.size(1) > 0 && x.size(1) < INT_MAX && x.size(0) <= INT_MAX, what,
-              ": logits [rows, vocabulary] with contiguous rows");
-  TORCH_CHECK(valid > 0 && valid <= x.size(1), what, ": valid_vocab must lie in 1 .. ", x.size(1), ", got ", valid);
-  TORCH_CHECK(temperature > 0, what, ": temperature must be positive");
-  TORCH_CHECK(ids.device() == x.device() && ids.scalar_type() == at::kLong && (ids.dim() == 1 || ids.dim() == 2) && ids.size(0) == x.size(0) &&
-              ids.is_contiguous(), what, ": ids must be a contiguous int64 tensor on ", x.device(), " with an entry or a row for each row of logits");
-  TORCH_CHECK(ids.dim() == 1 || ids.size(1) <= 4096, what, ": at most 4096 given tokens a row");
-  a.x = x.data_ptr(); a.ldx = x.size(0) <= 1 ? 0 : x.stride(0); a.T = (int)x.size(0); a.V = (int)valid;
+  TORCH_CHECK(x.size(1) < INT_MAX && x.size(0) <= INT_MAX && (x.stride(1) == 1 || x.size(1) == 1) && ids.device() == x.device() && ids.is_contiguous(), what,
+              ": logits and ids on one device, with contiguous rows");
+  a.x = x.data_ptr(); a.ldx = x.size(0) <= 1 ? 0 : x.stride(0); a.T = (int)x.size(0); a.V = (int)(valid ? valid : x.size(1));
   a.inv_temp = (float)(1.0 / temperature);
   a.ids = lptr(ids); a.K = ids.dim() == 1 ? 1 : (int)ids.size(1);
   return a;
 }
+Tensor by_rows(const Tensor& x) { return x.dim() == 2 && x.stride(1) != 1 && x.size(1) > 1 ? x.contiguous() : x; }
 
-std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_scores(const Tensor& x, const Tensor& ids, int64_t top, double temperature, int64_t valid) {
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_scores(const Tensor& logits, const Tensor& given, int64_t top, double temperature, int64_t valid) {
+  const Tensor x = by_rows(logits), ids = given.contiguous();
   VbScores a = scores_of(x, ids, temperature, valid, "token_scores");
-  TORCH_CHECK(top >= 0 && top <= 128 && top <= valid, "token_scores: top_k must lie in 0 .. min(128, valid_vocab), got ", top);
+  TORCH_CHECK_VALUE(top >= 0 && top <= std::min(128, a.V), "token_scores: top_k must lie in 0 .. ", std::min(128, a.V), ", got ", top);
   const c10::cuda::CUDAGuard guard(x.device());
   const auto f32 = x.options().dtype(at::kFloat);
   Tensor lp = at::empty(ids.sizes(), f32), ent = at::empty({x.size(0)}, f32), lse = at::empty({x.size(0)}, f32);
@@ -208,14 +226,15 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_scores(const Tensor& x,
   return {lp, ent, lse, top_ids, top_lp};
 }
 
-Tensor token_scores_bwd(const Tensor& x, const Tensor& ids, const Tensor& lse, const Tensor& ent, const Tensor& g_lp, const OptTensor& g_ent,
+Tensor token_scores_bwd(const Tensor& logits, const Tensor& given, const Tensor& lse, const Tensor& ent, const Tensor& g_lp, const OptTensor& g_ent,
                         double temperature, int64_t valid) {
+  const Tensor x = by_rows(logits), ids = given.contiguous();
   VbScores a = scores_of(x, ids, temperature, valid, "token_scores_bwd");
   const int64_t T = x.size(0);
   check_vec(lse, at::kFloat, T, x, "token_scores_bwd: lse");
   check_vec(ent, at::kFloat, T, x, "token_scores_bwd: entropy");
-  TORCH_CHECK(g_lp.device() == x.device() && g_lp.scalar_type() == at::kFloat && g_lp.sizes() == ids.sizes() && g_lp.is_contiguous(),
-              "token_scores_bwd: g_logprob must be a contiguous fp32 tensor of the shape of ids");
+  TORCH_CHECK_VALUE(g_lp.scalar_type() == at::kFloat && g_lp.sizes() == ids.sizes(), "token_scores_bwd: g_logprob must be fp32, of the shape of ids");
+  TORCH_CHECK(g_lp.device() == x.device() && g_lp.is_contiguous(), "token_scores_bwd: g_logprob must be contiguous and on the device of the logits");
   if (g_ent.has_value()) check_vec(*g_ent, at::kFloat, T, x, "token_scores_bwd: g_entropy");
   const c10::cuda::CUDAGuard guard(x.device());
   Tensor dx = at::empty({T, x.size(1)}, x.options());
@@ -257,7 +276,8 @@ struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
   }
 };
 
-std::tuple<Tensor, Tensor> token_logprobs(const Tensor& x, const Tensor& ids, double temperature, int64_t valid) {
+std::tuple<Tensor, Tensor> token_logprobs(const Tensor& logits, const Tensor& given, double temperature, int64_t valid) {
+  const Tensor x = by_rows(logits), ids = given.contiguous();
   if (at::GradMode::is_enabled() && x.requires_grad()) {
     auto out = TokenLogprobs::apply(x, ids, temperature, valid);
     return {out[0], out[1]};

@@ -105,10 +105,11 @@ extend_block_tables_kernel(int* __restrict__ table, long long ldt, int S, int wi
 
 constexpr int SM_THREADS = 256;
 constexpr int SM_TOKENS = 4;  // consecutive tokens of a thread: 16 and 32 bytes of output
+constexpr int SM_TURNS = 4;   // times that a block goes on: its sums over the batch are made once for 4096 tokens
 
 __global__ void __launch_bounds__(SM_THREADS)
 build_slot_map_kernel(const int* __restrict__ table, long long ldt, int S, int width, const int* __restrict__ rows, const int* __restrict__ starts,
-                      const int* __restrict__ ends, int B, int bs, int total, int* __restrict__ cu_out, int* __restrict__ positions,
+                      const int* __restrict__ ends, int B, int bs, int shift, int total, int* __restrict__ cu_out, int* __restrict__ positions,
                       long long* __restrict__ slots) {
   extern __shared__ int cu[];  // [B + 1]
   __shared__ int red[32];
@@ -117,7 +118,7 @@ build_slot_map_kernel(const int* __restrict__ table, long long ldt, int S, int w
   for (int base = 0; base < B; base += blockDim.x) {
     const int i = base + threadIdx.x;
     const int n = i < B ? min(max(ends[i] - max(starts[i], 0), 0), total) : 0;
-    int sum;  // at most 256 x 2^22 (SM_MAX_TOTAL)
+    int sum;  // at most 256 x 2^22, the most tokens that the launcher takes
     const int inc = pm_scan(n, red, sum);
     if (i < B) cu[i + 1] = min(carry + inc, total);
     carry = min(carry + sum, total);
@@ -126,37 +127,43 @@ build_slot_map_kernel(const int* __restrict__ table, long long ldt, int S, int w
   if (blockIdx.x == 0)
     for (int i = threadIdx.x; i <= B; i += blockDim.x) cu_out[i] = cu[i];
   const int end = cu[B];
-  const int t0 = (blockIdx.x * SM_THREADS + threadIdx.x) * SM_TOKENS;
-  if (t0 >= total) return;
-  int lo = 0, hi = B;  // the sequence of t0: the last i with cu[i] <= t0, as far as there is one
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= t0) lo = mid; else hi = mid;
-  }
-  int at[SM_TOKENS];
-  long long slot[SM_TOKENS];
+  for (int turn = 0; turn < SM_TURNS; ++turn) {
+    const int t0 = ((blockIdx.x * SM_TURNS + turn) * SM_THREADS + threadIdx.x) * SM_TOKENS;
+    if (t0 >= total) return;
+    int lo = 0, hi = B;  // the sequence of t0: the last i with cu[i] <= t0, as far as there is one
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (cu[mid] <= t0) lo = mid; else hi = mid;
+    }
+    int at[SM_TOKENS];
+    long long slot[SM_TOKENS];
+    int last_lo = -1, last_j = -1, blk = -1;
 #pragma unroll
-  for (int u = 0; u < SM_TOKENS; ++u) {
-    const int t = t0 + u;
-    at[u] = 0;
-    slot[u] = -1;
-    if (t >= end) continue;
-    while (cu[lo + 1] <= t) ++lo;
-    const int p = max(starts[lo], 0) + t - cu[lo], r = rows[lo], j = p / bs;
-    at[u] = p;
-    if (p >= 0 && r >= 0 && r < S && j < width) {
-      const int blk = table[r * ldt + j];
+    for (int u = 0; u < SM_TOKENS; ++u) {
+      const int t = t0 + u;
+      at[u] = 0;
+      slot[u] = -1;
+      if (t >= end) continue;
+      while (cu[lo + 1] <= t) ++lo;
+      const int p = max(starts[lo], 0) + t - cu[lo], j = shift >= 0 ? p >> shift : p / bs;
+      at[u] = p;
+      if (lo != last_lo || j != last_j) {
+        const int r = rows[lo];
+        blk = p >= 0 && r >= 0 && r < S && j < width ? table[r * ldt + j] : -1;
+        last_lo = lo;
+        last_j = j;
+      }
       if (blk >= 0) slot[u] = static_cast<long long>(blk) * bs + (p - j * bs);
     }
-  }
-  if (t0 + SM_TOKENS <= total) {
-    *reinterpret_cast<int4*>(positions + t0) = make_int4(at[0], at[1], at[2], at[3]);
-    *reinterpret_cast<longlong2*>(slots + t0) = make_longlong2(slot[0], slot[1]);
-    *reinterpret_cast<longlong2*>(slots + t0 + 2) = make_longlong2(slot[2], slot[3]);
-  } else {
-    for (int u = 0; u < SM_TOKENS && t0 + u < total; ++u) {
-      positions[t0 + u] = at[u];
-      slots[t0 + u] = slot[u];
+    if (t0 + SM_TOKENS <= total) {
+      *reinterpret_cast<int4*>(positions + t0) = make_int4(at[0], at[1], at[2], at[3]);
+      *reinterpret_cast<longlong2*>(slots + t0) = make_longlong2(slot[0], slot[1]);
+      *reinterpret_cast<longlong2*>(slots + t0 + 2) = make_longlong2(slot[2], slot[3]);
+    } else {
+      for (int u = 0; u < SM_TOKENS && t0 + u < total; ++u) {
+        positions[t0 + u] = at[u];
+        slots[t0 + u] = slot[u];
+      }
     }
   }
 }
@@ -180,9 +187,9 @@ extern "C" int vb_extend_block_tables(int* table, long long ldt, int S, int widt
 
 extern "C" int vb_build_slot_map(const int* table, long long ldt, int S, int width, const int* rows, const int* starts, const int* ends, int B,
                                  int block_size, int total, int* cu, int* positions, long long* slots, cudaStream_t s) {
-  const int per = SM_THREADS * SM_TOKENS;
+  const int per = SM_THREADS * SM_TOKENS * SM_TURNS, shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(static_cast<unsigned>(block_size)) : -1;
   const int blocks = total > 0 ? (total + per - 1) / per : 1;
-  build_slot_map_kernel<<<blocks, SM_THREADS, (B + 1) * sizeof(int), s>>>(table, ldt, S, width, rows, starts, ends, B, block_size, total, cu, positions,
+  build_slot_map_kernel<<<blocks, SM_THREADS, (B + 1) * sizeof(int), s>>>(table, ldt, S, width, rows, starts, ends, B, block_size, shift, total, cu, positions,
                                                                          slots);
   return static_cast<int>(cudaGetLastError());
 }

@@ -64,7 +64,7 @@ __device__ __forceinline__ float ts_max_nan(float a, float b) {
 // 16 bytes of a row as floats
 template <typename T> struct Lane;
 template <> struct Lane<float> {
-  static constexpr int N = 4, LOW = 0;  // values in 16 bytes, bits of a value as a float that are always zero
+  static constexpr int N = 4, LOW = 16;  // values in 16 bytes, low bits of their keys that the bound leaves out (zero, or of little use)
   static __device__ __forceinline__ uint4 none() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
   static __device__ __forceinline__ void open(const uint4& v, float (&f)[N]) {
     f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
@@ -422,7 +422,7 @@ token_scores_kernel(const VbScores p, int* status) {
     uint32_t bound = 0;
     const uint32_t mine = any ? order_key(most) : 0u;
     if (p.top > 0)
-      for (int bit = 31; bit >= L::LOW; --bit) {  // below, all keys of one sign are alike
+      for (int bit = 31; bit >= L::LOW; --bit) {
         const uint32_t want = bound | (1u << bit);
         if (ts_count(mine >= want) >= p.top) bound = want;
       }

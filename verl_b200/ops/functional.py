@@ -717,10 +717,10 @@ def extend_block_tables_(block_table: torch.Tensor, rows: torch.Tensor, have: to
     ``ceil(lengths[i] / block_size)``; the blocks that it lacks are taken from ``pool`` in the order of the sequences. All int32. Returns
     how many blocks of ``pool`` were taken, an int32 tensor [1]; -1 where the pool or a row is too small or a row is out of range: nothing
     was written then."""
-    _check_i32("extend_block_tables_", block_table, rows=rows, have=have, lengths=lengths)
-    _check_i32("extend_block_tables_", block_table, pool=pool)
     if block_table.is_cuda:
         return _ops().extend_block_tables_(block_table, rows, have, lengths, pool, int(block_size))
+    _check_i32("extend_block_tables_", block_table, rows=rows, have=have, lengths=lengths)
+    _check_i32("extend_block_tables_", block_table, pool=pool)
     R, width = block_table.shape
     need = (lengths.clamp(min=0).long() + block_size - 1) // block_size
     new = (need - have).clamp(min=0)
@@ -738,11 +738,11 @@ def build_slot_map(block_table: torch.Tensor, rows: torch.Tensor, starts: torch.
     sequence behind the other. Returns ``(cu_seqlens int32 [n + 1], positions int32 [total], slots int64 [total])``, a slot being
     ``block * block_size + offset``. ``total`` is the number of tokens (the sum of the lengths, known to the host); places behind the
     last token, and tokens without a valid row or block, get slot -1."""
+    if block_table.is_cuda:
+        return _ops().build_slot_map(block_table, rows, starts, ends, int(block_size), int(total))
     _check_i32("build_slot_map", block_table, rows=rows, starts=starts, ends=ends)
     if total < 0:
         raise ValueError(f"build_slot_map: total must not be negative, got {total}")
-    if block_table.is_cuda:
-        return _ops().build_slot_map(block_table, rows, starts, ends, int(block_size), int(total))
     R, width = block_table.shape
     a = starts.clamp(min=0).long()
     cu = torch.cat([a.new_zeros(1), (ends - a).clamp(min=0).cumsum(0)]).clamp(max=total)
@@ -765,12 +765,12 @@ def decode_slot_map(block_table: torch.Tensor, pos: torch.Tensor, ctx: torch.Ten
     (-1: inactive, or no block there), the context lengths with those of inactive rows zeroed, and the plan of
     :func:`paged_decode_attention_kv4`: the 64-token pieces of the contexts summed up in front of every row (int32 [S + 1]). Returns
     ``(slots int64 [S], ctx int32 [S], plan)``. One launch."""
+    if block_table.is_cuda:
+        return _ops().decode_slot_map(block_table, pos, ctx, active, int(block_size))
     _check_i32("decode_slot_map", block_table, pos=pos, ctx=ctx)
     S, width = block_table.shape
     if pos.shape[0] != S or active.shape != (S,) or active.dtype != torch.bool:
         raise ValueError(f"decode_slot_map: pos, ctx (int32) and active (bool) must have an entry for each of the {S} rows")
-    if block_table.is_cuda:
-        return _ops().decode_slot_map(block_table, pos, ctx, active, int(block_size))
     p = pos.long()
     ok = active & (p >= 0) & (p // block_size < width)
     blk = block_table.gather(1, (p // block_size).clamp(0, max(width - 1, 0))[:, None])[:, 0].long() if width and S else torch.full_like(p, -1)
@@ -829,6 +829,9 @@ def kv4_append_(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, pages: to
     """Quantise keys and values [T, kv_heads, head_dim] into a 4-bit pool (:func:`kv4_page_bytes`) at ``slots`` int64 [T]; negative slots
     are skipped, and a slot may occur once. A group of 32 channels is held as ``least + code * scale``, ``code`` in 0 .. 15 between its
     least and largest value. Values beyond +-7600 are held as that, a NaN makes its group NaN. bf16 or fp16 on a GPU."""
+    if k.is_cuda and not audit.enabled():
+        _ops().kv4_append_(k, v, slots, pages)
+        return
     if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype or not k.is_floating_point():
         raise ValueError(f"kv4_append_: k and v must be [tokens, heads, channels] of one floating type, got {k.dtype} {tuple(k.shape)}, "
                          f"{v.dtype} {tuple(v.shape)}")
@@ -856,6 +859,8 @@ def kv4_append_(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, pages: to
 def kv4_gather(pages: torch.Tensor, slots: torch.Tensor, head_dim: int, dtype: torch.dtype = torch.bfloat16):
     """Keys and values [T, kv_heads, head_dim] of the tokens at ``slots`` int64 [T] of a 4-bit pool, rounded once to ``dtype`` (bf16 or fp16
     on a GPU); zeros for negative slots."""
+    if pages.is_cuda and not audit.enabled():
+        return _ops().kv4_gather(pages, slots, int(head_dim), dtype)
     bs = _kv4_block_size("kv4_gather", pages, head_dim)
     if slots.dtype != torch.int64 or slots.dim() != 1:
         raise ValueError(f"kv4_gather: slots must be an int64 vector, got {slots.dtype} {tuple(slots.shape)}")
@@ -879,6 +884,8 @@ def paged_decode_attention_kv4(q: torch.Tensor, pages: torch.Tensor, block_table
     or fp16, heads of 64 or 128 channels, blocks of 16 to 256 tokens (a power of two), at most 16 query heads to a KV head.
 
     ``plan`` (third result of :func:`decode_slot_map` for the same contexts) saves a launch when it is made once for all layers of a step."""
+    if q.is_cuda and not audit.enabled():
+        return _ops().paged_decode_kv4(q, pages, block_table, ctx_len, plan, float(scale) if scale is not None else 1.0 / math.sqrt(max(q.shape[-1], 1)))
     if q.dim() != 3 or not q.is_floating_point():
         raise ValueError(f"paged_decode_attention_kv4: q must be [sequences, heads, channels], got {q.dtype} {tuple(q.shape)}")
     B, nh, hd = q.shape
@@ -940,12 +947,11 @@ def token_scores(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0, temper
 
     A logit of -inf has probability 0; a row that has nothing else scores -inf, with entropy 0. A NaN or +inf makes its row's scores NaN;
     among the most likely tokens a NaN counts as the largest value."""
+    if logits.is_cuda:
+        return TokenScores._make(_ops().token_scores(logits, ids, int(top_k), float(temperature), int(valid_vocab)))
     V = _scores_args("token_scores", logits, ids, temperature, valid_vocab)
     if not 0 <= top_k <= min(TOP_K_LIMIT, V):
         raise ValueError(f"token_scores: top_k must lie in 0 .. {min(TOP_K_LIMIT, V)}, got {top_k}")
-    if logits.is_cuda:
-        x = logits if logits.stride(1) == 1 else logits.contiguous()
-        return TokenScores._make(_ops().token_scores(x, ids.contiguous(), int(top_k), float(temperature), V))
     flat = ids if ids.dim() == 2 else ids[:, None]
     x = logits[:, :V].float()
     z = x * (1.0 / float(temperature))
@@ -965,23 +971,20 @@ def token_scores(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0, temper
 def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, temperature: float = 1.0, valid_vocab: int = 0):
     """``logprob`` and ``entropy`` of :func:`token_scores` with their gradient, on a GPU (``utils.kernel.token_logprobs`` is the form for any device
     and leading shape)."""
-    V = _scores_args("token_logprobs", logits, ids, temperature, valid_vocab)
-    x = logits if logits.stride(1) == 1 else logits.contiguous()
-    return _ops().token_logprobs(x, ids.contiguous(), float(temperature), V)
+    return _ops().token_logprobs(logits, ids, float(temperature), int(valid_vocab))
 
 
 def token_scores_bwd(logits: torch.Tensor, ids: torch.Tensor, lse: torch.Tensor, entropy: torch.Tensor, g_logprob: torch.Tensor,
                      g_entropy: Optional[torch.Tensor], temperature: float = 1.0, valid_vocab: int = 0) -> torch.Tensor:
     """Gradient of the logits, in their type, from those of ``logprob`` and ``entropy`` (None: none) of :func:`token_scores`. A token that is given
     several times gathers all its gradients; ids outside the vocabulary and columns behind ``valid_vocab`` have none."""
+    if logits.is_cuda:
+        return _ops().token_scores_bwd(logits, ids, lse.contiguous(), entropy.contiguous(), g_logprob.float().contiguous(),
+                                       g_entropy.float().contiguous() if g_entropy is not None else None, float(temperature), int(valid_vocab))
     V = _scores_args("token_scores_bwd", logits, ids, temperature, valid_vocab)
     T = logits.shape[0]
     if g_logprob.shape != ids.shape or (g_entropy is not None and g_entropy.shape != (T,)) or lse.shape != (T,) or entropy.shape != (T,):
         raise ValueError("token_scores_bwd: g_logprob has the shape of ids; lse, entropy and g_entropy have an entry for each row")
-    if logits.is_cuda:
-        x = logits if logits.stride(1) == 1 else logits.contiguous()
-        return _ops().token_scores_bwd(x, ids.contiguous(), lse.contiguous(), entropy.contiguous(), g_logprob.float().contiguous(),
-                                       g_entropy.float().contiguous() if g_entropy is not None else None, float(temperature), V)
     flat, g = (t if t.dim() == 2 else t[:, None] for t in (ids, g_logprob.float()))
     inv = 1.0 / float(temperature)
     logp = torch.log_softmax(logits[:, :V].float() * inv, -1)
