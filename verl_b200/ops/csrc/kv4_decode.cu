@@ -34,8 +34,8 @@ constexpr int KD_PIECE = 64;                     // tokens that the plan counts 
 constexpr int KD_WARPS = 4;
 constexpr int KD_THREADS = KD_WARPS * 32;
 constexpr int KD_TILES = KD_PIECE / 16;
-__host__ __device__ constexpr int kd_ctas(int nt) { return nt == 1 ? 4 : 3; }  // CTAs of an SM: what registers and shared memory hold
-constexpr int KD_MIN_PIECES = 2;                 // shortest run of a warp
+constexpr int KD_CTAS = 3;                       // CTAs of an SM: 168 registers a thread (four of 128: 129 us where three take 127)
+constexpr int KD_MIN_PIECES = 1;                 // shortest run of a warp
 
 __device__ int g_kv4_status[4];
 
@@ -159,7 +159,7 @@ __device__ __forceinline__ bool kd_wait(uint64_t* full, uint32_t parity) {
 }
 
 template <int HD, int NT, typename T>
-__global__ void __launch_bounds__(KD_THREADS, kd_ctas(NT))
+__global__ void __launch_bounds__(KD_THREADS, KD_CTAS)
 kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
   using L = KDSmem<HD, NT>;
   constexpr int CPR = HD / 4, VPR = HD / 8, KW = CPR / 8, VW = VPR / 8;  // channels of a thread's run, and words of them
@@ -205,16 +205,21 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
     if (!missing)
       src = p.pages + (static_cast<long long>(blk) * p.nkv + ahead.kvh) * kv4_page_bytes(bs, HD) + src_off + (tok & (bs - 1)) * row;
   };
+  uint32_t there = 0, gone = 0;  // lanes that fetch, and that miss a page
+  const auto look_all = [&](int u) {
+    look(u);
+    there = __ballot_sync(0xffffffffu, src != nullptr);
+    gone = __ballot_sync(0xffffffffu, missing);
+  };
   const auto load = [&](int j, int value) {  // keys or values of the j-th of the two; returns the pages of it that do not exist (bits 0, 4, 8, 12)
-    const bool mine = (lane >> 4) == j && (what & 1) == value;
-    const uint32_t copies = __ballot_sync(0xffffffffu, mine && src != nullptr && what < 2), gone = __ballot_sync(0xffffffffu, mine && missing && what < 2);
-    if (lane == 0) mbar_expect_tx(&full[value], __popc(copies) * tokens * (HD / 2 + HD / 8));
+    const uint32_t codes = 0x1111u << (16 * j + value);  // the lanes of its codes
+    if (lane == 0) mbar_expect_tx(&full[value], __popc(there & codes) * tokens * (HD / 2 + HD / 8));
     __syncwarp();
-    if (mine && src != nullptr) bulk_load(stage + dst_off, src, bytes, &full[value]);
-    return (gone >> (16 * j)) >> value;
+    if ((lane >> 4) == j && (what & 1) == value && src != nullptr) bulk_load(stage + dst_off, src, bytes, &full[value]);
+    return (gone >> (16 * j + value)) & 0x1111u;
   };
   uint32_t lost = 0, lost_next = 0;
-  look(u0);
+  look_all(u0);
   lost_next = load(0, 0);
   load(0, 1);
   int looked = 1;  // the next of the two
@@ -285,7 +290,7 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
       const int next = u + 1;
       if (looked == 2) {
         looked = 0;
-        if (next < u1) look(next);
+        if (next < u1) look_all(next);
       }
       lost = lost_next;
       if (ok) {
@@ -485,65 +490,65 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
 }
 
 // Joins the runs of every (sequence, head) that more than one warp worked on, and writes zeros for contexts of no tokens. A block takes
-// `heads` query heads of a (sequence, KV head), four channels a thread; what threads are left share the runs and meet in shared memory.
+// `heads` query heads of a (sequence, KV head), eight channels a thread; what threads are left share the runs and meet in shared memory.
 struct KDSum {
-  float m, s;
-  float4 x;
-  __device__ __forceinline__ void add(float mo, float so, float4 v) {
+  float m, s, x[8];
+  __device__ __forceinline__ void add(float mo, float so, const float (&v)[8]) {
     const float M = fmaxf(m, mo), mu = M == -INFINITY ? 0.f : M, fa = fast_exp2(m - mu), fb = fast_exp2(mo - mu);
     m = M;
     s = s * fa + so * fb;
-    x.x = x.x * fa + v.x * fb;
-    x.y = x.y * fa + v.y * fb;
-    x.z = x.z * fa + v.z * fb;
-    x.w = x.w * fa + v.w * fb;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = x[i] * fa + v[i] * fb;
   }
 };
 
 template <int HD, typename T>
-__global__ void __launch_bounds__(1024)
+__global__ void __launch_bounds__(512)
 kv4_join_kernel(const VbKv4Decode p, int runs, int heads) {
   extern __shared__ __align__(16) KDSum sums[];  // one a thread
   const int b = blockIdx.y, h0 = blockIdx.x * heads, G = p.nh / p.nkv, kvh = h0 / G, g0 = h0 % G;
   const int total = kd_total(p), per = kd_per(total, runs), n = p.plan[b + 1] - p.plan[b], len = kd_len(p, b);
   T* out = static_cast<T*>(p.out) + (static_cast<long long>(b) * p.nh + h0) * HD;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the runs' sums, and what came before them
-  const auto store = [&](int at, float4 v) {
-    T e[4] = {static_cast<T>(v.x), static_cast<T>(v.y), static_cast<T>(v.z), static_cast<T>(v.w)};
-    *reinterpret_cast<uint2*>(out + at * 4) = *reinterpret_cast<const uint2*>(e);
+  const auto store = [&](int at, const float (&v)[8], float f) {
+    uint4 o;
+    T* e = reinterpret_cast<T*>(&o);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = static_cast<T>(v[i] * f);
+    *reinterpret_cast<uint4*>(out + at * 8) = o;
   };
-  const int lanes = heads * HD / 4, groups = max(1, static_cast<int>(blockDim.x) / lanes), group = threadIdx.x / lanes;
+  const int lanes = heads * HD / 8, groups = max(1, static_cast<int>(blockDim.x) / lanes), group = threadIdx.x / lanes;
+  KDSum a{-INFINITY, 0.f, {}};
   if (n <= 0 || len == 0) {
-    for (int at = threadIdx.x; at < lanes; at += blockDim.x) store(at, make_float4(0.f, 0.f, 0.f, 0.f));
+    for (int at = threadIdx.x; at < lanes; at += blockDim.x) store(at, a.x, 0.f);
     return;
   }
   const int base = p.plan[b] * p.nkv + kvh * n, i0 = max(base, 0) / per, i1 = min((base + n - 1) / per, runs - 1);
   if (i0 >= i1) return;
   for (int at0 = 0; at0 < lanes; at0 += blockDim.x) {  // more than once for more channels than threads, with one group then
-    const int at = at0 + static_cast<int>(threadIdx.x) - (groups > 1 ? group * lanes : 0), head = at / (HD / 4), d = at % (HD / 4) * 4;
-    KDSum a{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+    const int at = at0 + static_cast<int>(threadIdx.x) - (groups > 1 ? group * lanes : 0), head = at / (HD / 8), d = at % (HD / 8) * 8;
+    a = KDSum{-INFINITY, 0.f, {}};
     if (group < groups && at < lanes) {
-      const auto slot = [&](int i) { return p.part + ((2LL * i + (i * per >= base ? 0 : 1)) * G + g0 + head) * (HD + 4); };
-#pragma unroll 4
+#pragma unroll 2
       for (int i = i0 + (groups > 1 ? group : 0); i <= i1; i += groups) {
-        const float* s = slot(i);
+        const float* s = p.part + ((2LL * i + (i * per >= base ? 0 : 1)) * G + g0 + head) * (HD + 4);
         const float2 ms = *reinterpret_cast<const float2*>(s + HD);
-        a.add(ms.x, ms.y, *reinterpret_cast<const float4*>(s + d));
+        const float4 lo = *reinterpret_cast<const float4*>(s + d), hi = *reinterpret_cast<const float4*>(s + d + 4);
+        const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        a.add(ms.x, ms.y, v);
       }
     }
-    if (groups > 1) {
-      sums[threadIdx.x] = a;
+    const int used = min(groups, i1 - i0 + 1);
+    for (int k = 1; k < used; k *= 2) {  // group g takes over group g + k's sums
+      if (group < used) sums[threadIdx.x] = a;
       __syncthreads();
-      if (group == 0)
-        for (int k = 1; k < groups; ++k) {
-          const KDSum o = sums[threadIdx.x + k * lanes];
-          a.add(o.m, o.s, o.x);
-        }
+      if (group % (2 * k) == 0 && group + k < used) {
+        const KDSum o = sums[threadIdx.x + k * lanes];
+        a.add(o.m, o.s, o.x);
+      }
+      __syncthreads();
     }
-    if (at < lanes && (groups == 1 || group == 0)) {
-      const float inv = a.s == 0.f ? 0.f : 1.f / a.s;
-      store(at, make_float4(a.x.x * inv, a.x.y * inv, a.x.z * inv, a.x.w * inv));
-    }
+    if (at < lanes && (groups == 1 || group == 0)) store(at, a.x, a.s == 0.f ? 0.f : 1.f / a.s);
   }
 }
 
@@ -582,7 +587,7 @@ static cudaError_t kd_launch(const VbKv4Decode& p, int* status, cudaStream_t s) 
   constexpr int smem = KDSmem<HD, NT>::TOTAL;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  const int ctas = num_sms() * kd_ctas(NT);
+  const int ctas = num_sms() * KD_CTAS;
   kern<<<ctas, KD_THREADS, smem, s>>>(p, __builtin_ctz(static_cast<unsigned>(p.block_size)), status);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
@@ -592,7 +597,7 @@ static cudaError_t kd_launch(const VbKv4Decode& p, int* status, cudaStream_t s) 
   cudaLaunchConfig_t cfg{};
   // A block per (sequence, KV head), or where each has many runs (few sequences with long contexts) one per query head with threads that share
   // the runs: one sequence of 131072 tokens (296 runs a head) 24 us and 6 us; 320 sequences (3 runs a head) 10.5 us.
-  const int runs = ctas * KD_WARPS, many = runs / (p.B * p.nkv) >= 16, heads = many ? 1 : p.nh / p.nkv, threads = many ? 512 : 256;
+  const int runs = ctas * KD_WARPS, many = runs / (p.B * p.nkv) >= 16, heads = many ? 1 : p.nh / p.nkv, threads = many ? 512 : 128;
   cfg.gridDim = dim3(p.nh / heads, p.B);
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = threads * sizeof(KDSum);
@@ -615,7 +620,7 @@ using namespace vb;
 
 extern "C" long long vb_kv4_decode_scratch(int B, int nh, int nkv, int hd) {
   const int G = nh / nkv;
-  return 2LL * num_sms() * kd_ctas(G <= 8 ? 1 : 2) * KD_WARPS * G * (hd + 4);
+  return 2LL * num_sms() * KD_CTAS * KD_WARPS * G * (hd + 4);
 }
 
 extern "C" int vb_kv4_status() {
