@@ -450,6 +450,32 @@ def test_rows_of_the_type_s_lowest_value_are_uniform(dev, V):
         assert ((d[0] - want).abs() <= want.abs() * (HALF[dtype] + 64 * U32)).all() and (d[1] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [2000, 50257, 300000])
+def test_alternatives_among_many_equal_values(dev, V, dtype):
+    """More values at the k-th largest one than the kernel keeps: those above it, then the first of its equals."""
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(8, V, generator=g)
+    few = torch.randint(0, V, (5,), generator=g)
+    x[0, :] = float("-inf")
+    x[0, few] = torch.arange(5.0)                                   # a mask that leaves five
+    x[1] = 0.1                                                      # no short number in 32 bits
+    x[2] = torch.randint(0, 4, (V,), generator=g) * 0.3 - 5.1       # four values, all negative
+    x[3] = (torch.rand(V, generator=g) < 0.01) * 2.0                # one in a hundred
+    x[4] = -0.1
+    x[4, V - 1], x[4, V // 2] = 0.3, 0.2
+    x[5] = torch.arange(V).flip(0) // 1000                          # equal ones side by side
+    x[6, :] = -1e-30
+    x[7, :] = float("-inf")
+    x = x.to(dtype).to(dev)
+    for k in (1, 20, 128):
+        out = F.token_scores(x, torch.zeros(8, dtype=torch.int64, device=dev), k)
+        _, _, _, order, top_lp = scores_64(x, torch.zeros(8, dtype=torch.int64), k, 1.0, V)
+        assert torch.equal(out.top_ids.cpu(), order)
+        got, tol = out.top_logprob.double().cpu(), 2 * slack(x, V, 1.0)[:, None]
+        assert ((got == top_lp) | ((got - top_lp).abs() <= tol))[:7].all() and (got[7] == float("-inf")).all()
+
+
 def grad_64(logits, ids, g_lp, g_ent, temperature, valid):
     z = (logits[:, :valid].double().cpu() / temperature).requires_grad_(True)
     logp = torch.log_softmax(z, -1)

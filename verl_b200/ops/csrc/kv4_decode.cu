@@ -34,7 +34,9 @@ constexpr int KD_PIECE = 64;                     // tokens that the plan counts 
 constexpr int KD_WARPS = 4;
 constexpr int KD_THREADS = KD_WARPS * 32;
 constexpr int KD_TILES = KD_PIECE / 16;
-constexpr int KD_CTAS = 3;                       // CTAs of an SM: 168 registers a thread (four of 128: 129 us where three take 127)
+// CTAs of an SM: three leave 168 registers a thread (four of 128: 129 us where three take 127); 16 heads of 128 channels need more (three: 68 us,
+// with spills, where two take 59)
+__host__ __device__ constexpr int kd_ctas(int hd, int nt) { return hd == 128 && nt == 2 ? 2 : 3; }
 constexpr int KD_MIN_PIECES = 1;                 // shortest run of a warp
 
 __device__ int g_kv4_status[4];
@@ -159,7 +161,7 @@ __device__ __forceinline__ bool kd_wait(uint64_t* full, uint32_t parity) {
 }
 
 template <int HD, int NT, typename T>
-__global__ void __launch_bounds__(KD_THREADS, KD_CTAS)
+__global__ void __launch_bounds__(KD_THREADS, kd_ctas(HD, NT))
 kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
   using L = KDSmem<HD, NT>;
   constexpr int CPR = HD / 4, VPR = HD / 8, KW = CPR / 8, VW = VPR / 8;  // channels of a thread's run, and words of them
@@ -587,7 +589,7 @@ static cudaError_t kd_launch(const VbKv4Decode& p, int* status, cudaStream_t s) 
   constexpr int smem = KDSmem<HD, NT>::TOTAL;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  const int ctas = num_sms() * KD_CTAS;
+  const int ctas = num_sms() * kd_ctas(HD, NT);
   kern<<<ctas, KD_THREADS, smem, s>>>(p, __builtin_ctz(static_cast<unsigned>(p.block_size)), status);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
@@ -620,7 +622,7 @@ using namespace vb;
 
 extern "C" long long vb_kv4_decode_scratch(int B, int nh, int nkv, int hd) {
   const int G = nh / nkv;
-  return 2LL * num_sms() * KD_CTAS * KD_WARPS * G * (hd + 4);
+  return 2LL * num_sms() * kd_ctas(hd, G <= 8 ? 1 : 2) * KD_WARPS * G * (hd + 4);
 }
 
 extern "C" int vb_kv4_status() {

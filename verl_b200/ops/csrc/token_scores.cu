@@ -7,8 +7,8 @@
 // The most likely tokens come with the same pass: every thread also keeps the largest value that it met, and the k-th largest of those of a
 // block is a bound that at least k values of the row reach. The largest value of each group of 32 (16 of 32 bits) stays in shared memory, and
 // only groups that reach the bound are looked at again (hardly more than k, from L2); what reaches it there is again hardly more than k
-// values, which are ranked by counting. Rows that this does not fit (over 768 values at the bound: few different values) and rows with NaN,
-// +inf or nothing above -1e30 take a slow path, right for any values.
+// values, which are ranked by counting. Where over 768 values reach it (few different values, or a mask that leaves fewer than k), the row is
+// gone over again for what is above the bound and for the first values that equal it; rows with NaN or +inf are searched k times over.
 //
 // Blocks stay for many rows. One warp of a block brings the rows into a ring of shared memory by bulk copies, so that the next row is on its way
 // while the block ranks the last one. Where rows are few, a row belongs to a cluster of up to 8 blocks, which exchange their sums, bounds and
@@ -277,6 +277,82 @@ __device__ void top_any(const VbScores& p, long long t, const T* x, Shared& sh, 
   }
 }
 
+// Writes the tokens of the list, which holds `found` values, at their ranks: four lanes a candidate count the larger ones.
+template <typename F>
+__device__ void write_ranked(const VbScores& p, long long t, const Shared& sh, int found, const F& logprob) {
+  for (int i0 = 0; i0 < found; i0 += TS_THREADS / 4) {
+    const int i = i0 + (threadIdx.x >> 2), quarter = threadIdx.x & 3;
+    const unsigned long long key = sh.list[min(i, found - 1)];
+    int rank = 0;
+#pragma unroll 4
+    for (int j = quarter; j < found; j += 4) rank += sh.list[j] > key;
+    rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+    rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+    if (i >= found || quarter != 0 || rank >= p.top) continue;
+    const long long at = t * p.top + rank;
+    p.top_ids[at] = 0xffffffffu - static_cast<uint32_t>(key);
+    p.top_lp[at] = logprob(key_value(static_cast<uint32_t>(key >> 32)));
+  }
+}
+
+// The most likely tokens of a row without NaN in three passes of one block: the `top`-th largest of the threads' largest values, what is above
+// it, and as many of the first values that equal it as are missing. False where over TS_CANDIDATES values are above it.
+template <typename T, typename F>
+__device__ bool top_ties(const VbScores& p, long long t, const T* x, Shared& sh, const F& logprob) {
+  float most = -INFINITY;
+  for (int v = threadIdx.x; v < p.V; v += TS_THREADS) most = fmaxf(most, static_cast<float>(x[v]));
+  const uint32_t mine = static_cast<int>(threadIdx.x) < p.V ? order_key(most) : 0u;
+  uint32_t bound = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t want = bound | (1u << bit);
+    if (ts_count(mine >= want) >= min(p.top, TS_THREADS)) bound = want;
+  }
+  const float limit = bound <= order_key(-INFINITY) ? -INFINITY : key_value(bound);
+  if (threadIdx.x == 0) sh.found = 0;
+  ts_sync();
+  for (int v = threadIdx.x; v < p.V; v += TS_THREADS) {
+    const float f = static_cast<float>(x[v]);
+    if (f > limit) {
+      const int k = atomicAdd(&sh.found, 1);
+      if (k < TS_CANDIDATES) sh.list[k] = (static_cast<unsigned long long>(order_key(f)) << 32) | (0xffffffffu - v);
+    }
+  }
+  ts_sync();
+  int found = sh.found;
+  if (found > TS_CANDIDATES) return false;
+  constexpr int EACH = 8;  // consecutive values of a thread
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int v0 = 0; v0 < p.V && found < p.top; v0 += TS_THREADS * EACH) {
+    const int v = v0 + threadIdx.x * EACH;
+    uint32_t equal = 0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+      if (v + i < p.V && static_cast<float>(x[v + i]) == limit) equal |= 1u << i;
+    int before = __popc(equal);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int n = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += n;
+    }
+    ts_sync();
+    if (lane == 31) sh.red[warp] = static_cast<float>(before);  // whole numbers below 2^24
+    ts_sync();
+    int all = 0;
+    for (int w = 0; w < TS_THREADS / 32; ++w) {
+      const int n = static_cast<int>(sh.red[w]);
+      if (w < warp) before += n;
+      all += n;
+    }
+    before -= __popc(equal);
+    for (uint32_t e = equal; e != 0 && found + before < p.top; e &= e - 1, ++before)
+      sh.list[found + before] = (static_cast<unsigned long long>(order_key(limit)) << 32) | (0xffffffffu - (v + __ffs(e) - 1));
+    found = min(found + all, p.top);
+  }
+  ts_sync();
+  write_ranked(p, t, sh, found, logprob);
+  return true;
+}
+
 template <typename T>
 __device__ __forceinline__ void bulk_row(void* dst, const T* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
@@ -452,6 +528,7 @@ token_scores_kernel(const VbScores p, int* status) {
       const float limit = bound <= order_key(-INFINITY) ? -INFINITY : key_value(bound);
       const int chunks = (n + TS_CHUNK - 1) / TS_CHUNK, low = static_cast<int>(bound >> 16);
       if (mine >= bound)
+#pragma unroll 8
         for (int slot = 0; slot < min(chunks, TS_SLOTS); ++slot)
           if (sh.top[slot][threadIdx.x] >= low) {
             const int k = atomicAdd(&sh.groups, 1);
@@ -465,15 +542,23 @@ token_scores_kernel(const VbScores p, int* status) {
         if (k < TS_CANDIDATES) first->list[k] = (static_cast<unsigned long long>(order_key(f)) << 32) | (0xffffffffu - at);
       };
       // item i: vector i % TS_PER of group i / TS_PER, and for rows of more stages than slots the same place some stages on
-      for (int i = threadIdx.x; i < items; i += TS_THREADS) {
-        const int turn = i / (groups * TS_PER), k = i - turn * groups * TS_PER, g = sh.group[k / TS_PER];
-        const int at = ((turn * TS_SLOTS + g / TS_THREADS) * TS_PER + k % TS_PER) * TS_THREADS + g % TS_THREADS;
-        if (at >= n) continue;
-        float f[L::N];
-        L::open(__ldg(vec + at), f);
+      for (int i0 = threadIdx.x; i0 < items; i0 += 2 * TS_THREADS) {
+        uint4 raw[2];
+        int at[2];
 #pragma unroll
-        for (int j = 0; j < L::N; ++j)
-          if (f[j] >= limit) put(f[j], row.head + (v0 + at) * L::N + j);
+        for (int u = 0; u < 2; ++u) {
+          const int i = i0 + u * TS_THREADS, turn = i / (groups * TS_PER), k = i - turn * groups * TS_PER, g = i < items ? sh.group[k / TS_PER] : 0;
+          at[u] = i < items ? ((turn * TS_SLOTS + g / TS_THREADS) * TS_PER + k % TS_PER) * TS_THREADS + g % TS_THREADS : n;
+          raw[u] = at[u] < n ? __ldg(vec + at[u]) : L::none();
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float f[L::N];
+          L::open(raw[u], f);
+#pragma unroll
+          for (int j = 0; j < L::N; ++j)
+            if (f[j] >= limit && at[u] < n) put(f[j], row.head + (v0 + at[u]) * L::N + j);
+        }
       }
       if (has_loose && loose >= limit) put(loose, loose_at);
     }
@@ -485,7 +570,10 @@ token_scores_kernel(const VbScores p, int* status) {
       ts_sync();
       if (p.top > 0) {
         const Stat b = any_stat(x, p.V, p.inv_temp, sh.red);
-        top_any(p, t, x, sh, b.m, logf(b.s), false);
+        const float bls = logf(b.s);
+        const bool wild = !(b.s >= 0.f) || b.m == INFINITY;  // NaN or +inf in it
+        if (wild || !top_ties(p, t, x, sh, [&](float f) { return b.m == -INFINITY ? -INFINITY : f * p.inv_temp - b.m - bls; }))
+          top_any(p, t, x, sh, b.m, bls, false);
       }
       ts_sync();
       continue;
@@ -502,26 +590,11 @@ token_scores_kernel(const VbScores p, int* status) {
     }
     if (p.top > 0) {
       const int found = sh.found;
-      if (found > TS_CANDIDATES || found < p.top) {
+      const auto logprob = [&](float f) { return scaled_logprob(f, p.inv_temp, a.m, ls); };
+      if (found >= p.top && found <= TS_CANDIDATES)
+        write_ranked(p, t, sh, found, logprob);
+      else if (!top_ties(p, t, x, sh, logprob))
         top_any(p, t, x, sh, a.m, ls, true);
-      } else {
-        // four lanes a candidate count the larger ones
-        for (int i0 = 0; i0 < found; i0 += TS_THREADS / 4) {
-          const int i = i0 + (threadIdx.x >> 2), quarter = threadIdx.x & 3;
-          const unsigned long long key = sh.list[min(i, found - 1)];
-          int rank = 0;
-#pragma unroll 4
-          for (int j = quarter; j < found; j += 4) rank += sh.list[j] > key;
-          rank += __shfl_xor_sync(0xffffffffu, rank, 1);
-          rank += __shfl_xor_sync(0xffffffffu, rank, 2);
-          if (i >= found || quarter != 0) continue;
-          if (rank < p.top) {
-            const long long at = static_cast<long long>(t) * p.top + rank;
-            p.top_ids[at] = 0xffffffffu - static_cast<uint32_t>(key);
-            p.top_lp[at] = scaled_logprob(key_value(static_cast<uint32_t>(key >> 32)), p.inv_temp, a.m, ls);
-          }
-        }
-      }
     }
     ts_sync();  // the next row starts with an empty list
   }
@@ -605,9 +678,10 @@ token_scores_bwd_kernel(const VbScores p, const float* __restrict__ g_lp, const 
 
 template <typename T>
 static cudaError_t ts_forward(const VbScores& a, cudaStream_t s) {
-  // as many blocks to a row as the card holds at once, with at least 1024 vectors for each; with more rows than that, blocks that stay
+  // A row to several blocks while there are at most three to an SM then (64 rows of 128256 in 32 bits: 17 us in 256 blocks, 19 us in 512; 100 rows of
+  // 152064: 19 us in 400, 23 us in 100), with at least 1024 vectors for each. With more rows than the card holds blocks, blocks that stay.
   int parts = 1;
-  while (parts < 8 && 2LL * parts * a.T <= TS_BLOCKS * num_sms() && a.V / Lane<T>::N >= 2048 * parts) parts *= 2;
+  while (parts < 8 && 2LL * parts * a.T <= 3 * num_sms() && a.V / Lane<T>::N >= 2048 * parts) parts *= 2;
   constexpr int smem = TS_STAGES * TS_CHUNK * 16;
   auto kern = token_scores_kernel<T>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
