@@ -259,7 +259,7 @@ def attention_64(q, pages, table, lens, bs, scale):
         # Sums of products are fp32 (their length times U32). A score is off by at most ds, a weight by 2 ds and by the rounding of
         # e^(s - reference) to fp16 (U16, and 2^-25 of the largest where it is small), which acts on the whole value.
         dot = lambda x: np.einsum("hgd,htd->hgt", np.abs(q[b]), np.abs(x))
-        ds = scale * (U16 * dot(2 * kp + 3 * ks) + 2.0**-21 * np.abs(q[b]).sum(-1, keepdims=True) + (2.0**-22 + (hd + 8) * U32) * dot(np.abs(kk) + 3 * kp))
+        ds = abs(scale) * (U16 * dot(2 * kp + 3 * ks) + 2.0**-21 * np.abs(q[b]).sum(-1, keepdims=True) + (2.0**-22 + (hd + 8) * U32) * dot(np.abs(kk) + 3 * kp))
         ds = ds.max(-1, keepdims=True)
         size, codes_size = (np.einsum("hgt,htd->hgd", w, np.abs(x)) for x in (vv, vp + 2 * vs))
         off[b] = ((2 * ds + 2 * U16) * size + U16 * codes_size + 2.0**-21 + (n + 64) * U32 * (size + 3 * codes_size)
@@ -301,6 +301,40 @@ def test_attention_with_queries_of_any_size(dev, factor):
     out = F.paged_decode_attention_kv4(q, pages, table, ctx, scale=scale)
     want, off = attention_64(q, pages, table, [100, 30], 64, scale)
     assert (np.abs(out.double().cpu().numpy() - want) <= off + 2.0**-8 * np.abs(want) + 2.0**-24).all()
+
+
+def test_attention_with_a_scale_of_any_sign(dev):
+    rs = np.random.RandomState(8)
+    pages, table, ctx = make_pool(rs, [90, 1], 2, 64, 64, 2, dev)
+    q = torch.from_numpy(rs.randn(2, 6, 64)).to(torch.bfloat16).to(dev)
+    for scale in (-0.125, 0.0):
+        out = F.paged_decode_attention_kv4(q, pages, table, ctx, scale=scale)
+        want, off = attention_64(q, pages, table, [90, 1], 64, scale)
+        assert (np.abs(out.double().cpu().numpy() - want) <= np.abs(off) + 2.0**-8 * np.abs(want) + 2.0**-20).all()
+
+
+@pytest.mark.gpu
+def test_attention_of_two_streams_and_of_a_wrong_plan():
+    """Calls on two streams at once keep apart; a plan for other contexts gives other numbers, and nothing outside its tensors is touched."""
+    rs = np.random.RandomState(9)
+    pages, table, ctx = make_pool(rs, [700, 300, 0, 64], 2, 64, 64, 12, "cuda")
+    q = torch.from_numpy(rs.randn(4, 6, 64)).to(torch.bfloat16).cuda()
+    want = F.paged_decode_attention_kv4(q, pages, table, ctx)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(20):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(F.paged_decode_attention_kv4(q, pages, table, ctx))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+    for plan in ([0, 0, 0, 0, 0], [0, 40, 80, 120, 160], [5, 3, 9, 2, 7], [0, -5, 3, 2, 1], [0, 2**30, 0, 0, 2**31 - 1]):
+        F.paged_decode_attention_kv4(q, pages, table, ctx, plan=i32(plan, "cuda"))
+    torch.cuda.synchronize()
+    assert torch.equal(F.paged_decode_attention_kv4(q, pages, table, ctx), want)
+    from verl_b200.ops import native
+
+    native.check_status()
 
 
 def test_blocks_that_do_not_exist_are_skipped(dev):
@@ -574,6 +608,49 @@ def test_log_probs_are_differentiated_once(dev):
         lp.sum().backward()
     with torch.no_grad():
         assert not token_logprobs(x, torch.zeros(3, dtype=torch.int64, device=dev))[0].requires_grad
+
+
+def test_entropy_changed_in_place_before_the_backward_pass(dev):
+    """The gradient needs the entropy as it was: it has it, or says that it was changed."""
+    x = torch.randn(3, 20, device=dev, requires_grad=True)
+    ids = torch.zeros(3, dtype=torch.int64, device=dev)
+    want = torch.autograd.grad(sum(t.sum() for t in token_logprobs(x, ids)), x)[0]
+    lp, ent = token_logprobs(x, ids)
+    total = lp.sum() + ent.sum()
+    with torch.no_grad():
+        ent.mul_(2.0)
+    try:
+        assert torch.equal(torch.autograd.grad(total, x)[0], want)
+    except RuntimeError as e:
+        assert "modified by an inplace operation" in str(e)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,V", [(3, 1003), (2, 70000)])
+def test_scores_and_their_gradient_captured_and_replayed(T, V):
+    x = torch.randn(T, V, device="cuda", requires_grad=True)
+    ids = torch.randint(0, V, (T, 2), device="cuda")
+    g_lp, g_ent = torch.randn(T, 2, device="cuda"), torch.randn(T, device="cuda")
+
+    def step():
+        lp, ent = token_logprobs(x, ids)
+        return lp, ent, torch.autograd.grad((lp, ent), x, (g_lp, g_ent))[0], F.token_scores(x.detach(), ids, 9)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for _ in range(2):
+        with torch.no_grad():
+            x.copy_(torch.randn(T, V))
+        graph.replay()
+        eager = step()
+        for a, b in zip((*captured[:3], *captured[3]), (*eager[:3], *eager[3])):
+            assert torch.equal(a, b)
 
 
 def test_refusals_of_the_scores(dev):

@@ -251,7 +251,7 @@ struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& ids, double temperature, int64_t valid) {
     at::AutoDispatchBelowADInplaceOrView below;
     auto [lp, ent, lse, top, top_lp] = token_scores(x, ids, 0, temperature, valid);
-    ctx->save_for_backward({x, ids, lse, ent.detach()});
+    ctx->save_for_backward({x, ids, lse, ent});
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["valid"] = valid;
     ctx->set_materialize_grads(false);
@@ -267,7 +267,7 @@ struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
         const Tensor g_lp = g[0].defined() ? g[0].contiguous() : at::zeros(saved[1].sizes(), saved[2].options());
         OptTensor g_ent;
         if (g[1].defined()) g_ent = g[1].contiguous();
-        dx = token_scores_bwd(saved[0].detach(), saved[1], saved[2], saved[3], g_lp, g_ent, ctx->saved_data["temperature"].toDouble(), ctx->saved_data["valid"].toInt());
+        dx = token_scores_bwd(saved[0].detach(), saved[1], saved[2], saved[3].detach(), g_lp, g_ent, ctx->saved_data["temperature"].toDouble(), ctx->saved_data["valid"].toInt());
       }
       if (again)  // a graph of the gradient is asked for: an error where it is used
         dx = std::make_shared<torch::autograd::DelayedError>("token_logprobs can be differentiated once", 2)->apply({dx, saved[0]})[0];

@@ -32,7 +32,7 @@ class TokenLogprobs(torch.autograd.Function):
     def forward(ctx, logits: torch.Tensor, ids: torch.Tensor, temperature: float, valid_vocab: int):
         out = F.token_scores(logits, ids, 0, temperature, valid_vocab)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(logits, ids, out.lse, out.entropy)
+        ctx.save_for_backward(logits, ids, out.lse, out.entropy.clone())
         ctx.meta = (temperature, valid_vocab)
         return out.logprob, out.entropy
 

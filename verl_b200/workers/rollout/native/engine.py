@@ -597,6 +597,7 @@ class RolloutEngine:
 
     def _write_tables(self, slots: Sequence[int], blocks: Sequence[Sequence[int]]) -> None:
         """The block tables of some sequence slots, from their block lists (one transfer and one launch)."""
+        assert all(len(b) <= self.max_blocks_per_seq for b in blocks), "a sequence holds more blocks than max_model_len has"
         i32 = lambda x: torch.tensor(x, dtype=torch.int32).to(self.device)
         F.extend_block_tables_(self.block_table, i32(list(slots)), torch.zeros(len(slots), dtype=torch.int32, device=self.device),
                                i32([len(b) * self.bs for b in blocks]), i32([b for row in blocks for b in row]), self.bs)
