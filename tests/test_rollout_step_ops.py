@@ -180,6 +180,25 @@ def test_append_and_gather(dev, T, nkv, hd, bs, dtype):
         assert got.dtype == dtype and (off <= np.abs(want) * (HALF[dtype] + 2 * U32) + 2.0**-24).all()   # one rounding to the type, one in fp32
 
 
+@pytest.mark.parametrize("T,nkv,bs", [(5001, 16, 48), (9999, 8, 64)])
+def test_append_of_many_tokens(dev, T, nkv, bs):
+    if dev == "cpu":
+        T //= 16
+    g = torch.Generator().manual_seed(T)
+    k, v = (torch.randn(T, nkv, 128, generator=g).bfloat16().to(dev) for _ in range(2))
+    blocks = -(-T // bs) + 1
+    slots = torch.randperm(blocks * bs, generator=g)[:T]
+    pages = torch.zeros(blocks, nkv, F.kv4_page_bytes(bs, 128), dtype=torch.uint8, device=dev)
+    F.kv4_append_(k, v, slots.to(dev), pages)
+    b, o = (slots // bs).numpy(), (slots % bs).numpy()
+    back = F.kv4_gather(pages, slots.to(dev), 128, torch.float16)
+    for x, got, c, s, m in zip((k, v), back, *unpacked(pages, bs, 128)):
+        wc, ws, wm = quantised(x.float().cpu().numpy())
+        assert np.array_equal(c[b, :, o], wc) and np.array_equal(s[b, :, o], ws) and np.array_equal(m[b, :, o], wm)
+        want = (wc * ws.astype(np.float64) + wm).reshape(T, nkv, 128)
+        assert (np.abs(got.double().cpu().numpy() - want) <= np.abs(want) * (U16 + 2 * U32) + 2.0**-24).all()   # as above
+
+
 def test_values_outside_the_range_of_the_cache(dev):
     x = torch.zeros(4, 1, 64, dtype=torch.bfloat16, device=dev)
     x[0, 0, 3], x[1, 0, 40], x[2, 0, 0], x[3, 0, 63] = float("nan"), float("inf"), -1e30, 1e-6
