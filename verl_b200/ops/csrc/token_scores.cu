@@ -46,6 +46,27 @@ __device__ __forceinline__ float ts_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Two fp32 numbers in one instruction, each rounded as alone
+__device__ __forceinline__ unsigned long long ts_two(float a, float b) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 ts_of(unsigned long long v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ unsigned long long ts_fma(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ unsigned long long ts_add(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ int g_ts_status[4];
 
 // barrier of the threads that compute
@@ -448,7 +469,8 @@ token_scores_kernel(const VbScores p, int* status) {
         *keep = slot < TS_SLOTS ? key : max(*keep, key);
       }
       if (big * c > a.m + 60.f) a.move(big * c);
-      float s0 = a.s, s1 = 0.f, w0 = a.w, w1 = 0.f;
+      unsigned long long s2 = ts_two(a.s, 0.f), w2 = ts_two(a.w, 0.f);
+      const unsigned long long c2 = ts_two(c, c), m2 = ts_two(-a.m, -a.m);
 #pragma unroll
       for (int u = 0; u < TS_PER; ++u) {
         if (left <= u * TS_THREADS) break;
@@ -456,16 +478,17 @@ token_scores_kernel(const VbScores p, int* status) {
         L::open(at[u * TS_THREADS], f);
 #pragma unroll
         for (int i = 0; i < L::N; i += 2) {
-          const float d0 = fmaf(f[i], c, -a.m), e0 = ts_exp2(d0), d1 = fmaf(f[i + 1], c, -a.m), e1 = ts_exp2(d1);
-          s0 += e0;
-          w0 = fmaf(e0, d0, w0);
-          s1 += e1;
-          w1 = fmaf(e1, d1, w1);
+          const unsigned long long d2 = ts_fma(ts_two(f[i], f[i + 1]), c2, m2);
+          const float2 d = ts_of(d2);
+          const unsigned long long e2 = ts_two(ts_exp2(d.x), ts_exp2(d.y));
+          s2 = ts_add(s2, e2);
+          w2 = ts_fma(e2, d2, w2);
         }
       }
-      if (w0 + w1 == w0 + w1) {
-        a.s = s0 + s1;
-        a.w = w0 + w1;
+      const float2 s = ts_of(s2), w = ts_of(w2);
+      if (w.x + w.y == w.x + w.y) {
+        a.s = s.x + s.y;
+        a.w = w.x + w.y;
       } else {  // 0 * -inf got into the sums: again with a floor under the exponents
 #pragma unroll 1
         for (int u = 0; u < TS_PER; ++u) {
