@@ -194,13 +194,13 @@ __device__ __forceinline__ Stat block_stat(Stat a, float* red) {
   if (lane == 0) { red[warp] = a.m; red[16 + warp] = a.s; red[32 + warp] = a.w; }
   ts_sync();
   constexpr int W = TS_THREADS / 32;
-  Stat b{lane < W ? red[lane] : -1e30f, lane < W ? red[16 + lane] : 0.f, lane < W ? red[32 + lane] : 0.f};
+  Stat b{red[lane % W], red[16 + lane % W], red[32 + lane % W]};
   m = b.m;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  for (int o = W / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   b.move(m);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
+  for (int o = W / 2; o > 0; o >>= 1) {
     b.s += __shfl_xor_sync(0xffffffffu, b.s, o);
     b.w += __shfl_xor_sync(0xffffffffu, b.w, o);
   }
@@ -249,6 +249,21 @@ __device__ Stat any_stat(const T* x, int V, float inv_temp, float* red) {
   a = block_stat(a, red);
   a.m = m;
   return a;
+}
+
+// A place for each of the n things of this thread, warp by warp: the counter goes up once for all 32 threads, which all take part.
+template <typename F>
+__device__ __forceinline__ int warp_places(int n, const F& count) {
+  const int lane = threadIdx.x & 31;
+  int upto = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int before = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += before;
+  }
+  int base = 0;
+  if (lane == 31 && upto > 0) base = count(upto);
+  return __shfl_sync(0xffffffffu, base, 31) + upto - n;
 }
 
 struct Shared {
@@ -303,6 +318,7 @@ template <typename F>
 __device__ void write_ranked(const VbScores& p, long long t, const Shared& sh, int found, const F& logprob) {
   for (int i0 = 0; i0 < found; i0 += TS_THREADS / 4) {
     const int i = i0 + (threadIdx.x >> 2), quarter = threadIdx.x & 3;
+    if ((i & ~7) >= found) break;  // the warp's eight
     const unsigned long long key = sh.list[min(i, found - 1)];
     int rank = 0;
 #pragma unroll 4
@@ -517,7 +533,7 @@ token_scores_kernel(const VbScores p, int* status) {
     }
     a = block_stat(a, sh.red);
 
-    // ---- the bound: bit by bit, the largest key that `top` threads' largest values reach
+    // ---- the bound: bit by bit, the largest key that `top` threads' largest values reach (100 cycles a bit; by one warp with eight keys a lane, 170)
     uint32_t bound = 0;
     const uint32_t mine = any ? order_key(most) : 0u;
     if (p.top > 0)
@@ -550,40 +566,56 @@ token_scores_kernel(const VbScores p, int* status) {
     if (p.top > 0 && !odd) {
       const float limit = bound <= order_key(-INFINITY) ? -INFINITY : key_value(bound);
       const int chunks = (n + TS_CHUNK - 1) / TS_CHUNK, low = static_cast<int>(bound >> 16);
+      uint32_t hits = 0;
       if (mine >= bound)
 #pragma unroll 8
-        for (int slot = 0; slot < min(chunks, TS_SLOTS); ++slot)
-          if (sh.top[slot][threadIdx.x] >= low) {
-            const int k = atomicAdd(&sh.groups, 1);
-            if (k < TS_CANDIDATES) sh.group[k] = static_cast<uint16_t>(slot * TS_THREADS + threadIdx.x);
-          }
+        for (int slot = 0; slot < min(chunks, TS_SLOTS); ++slot) hits |= static_cast<uint32_t>(sh.top[slot][threadIdx.x] >= low) << slot;
+      int k = warp_places(__popc(hits), [&](int n) { return atomicAdd(&sh.groups, n); });
+      for (; hits != 0; hits &= hits - 1, ++k)
+        if (k < TS_CANDIDATES) sh.group[k] = static_cast<uint16_t>((__ffs(hits) - 1) * TS_THREADS + threadIdx.x);
       ts_sync();
       const int groups = min(sh.groups, TS_CANDIDATES), turns = (chunks + TS_SLOTS - 1) / TS_SLOTS, items = groups * TS_PER * turns;
       if (sh.groups > TS_CANDIDATES && threadIdx.x == 0) atomicAdd(&first->found, TS_CANDIDATES + 1);  // too many: the slow path
-      const auto put = [&](float f, int at) {
-        const int k = atomicAdd(&first->found, 1);
+      const auto found = [&](int n) { return parts > 1 ? atomicAdd(&first->found, n) : atomicAdd(&sh.found, n); };
+      const auto put = [&](float f, int at, int k) {
         if (k < TS_CANDIDATES) first->list[k] = (static_cast<unsigned long long>(order_key(f)) << 32) | (0xffffffffu - at);
       };
       // item i: vector i % TS_PER of group i / TS_PER, and for rows of more stages than slots the same place some stages on
-      for (int i0 = threadIdx.x; i0 < items; i0 += 2 * TS_THREADS) {
+      for (int i0 = static_cast<int>(threadIdx.x) & ~31; i0 < items; i0 += 2 * TS_THREADS) {
         uint4 raw[2];
         int at[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const int i = i0 + u * TS_THREADS, turn = i / (groups * TS_PER), k = i - turn * groups * TS_PER, g = i < items ? sh.group[k / TS_PER] : 0;
+          const int i = i0 + (threadIdx.x & 31) + u * TS_THREADS, turn = turns == 1 ? 0 : i / (groups * TS_PER), k = i - turn * groups * TS_PER;
+          const int g = i < items ? sh.group[k / TS_PER] : 0;
           at[u] = i < items ? ((turn * TS_SLOTS + g / TS_THREADS) * TS_PER + k % TS_PER) * TS_THREADS + g % TS_THREADS : n;
           raw[u] = at[u] < n ? __ldg(vec + at[u]) : L::none();
         }
+        uint32_t reach = 0;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           float f[L::N];
           L::open(raw[u], f);
 #pragma unroll
           for (int j = 0; j < L::N; ++j)
-            if (f[j] >= limit && at[u] < n) put(f[j], row.head + (v0 + at[u]) * L::N + j);
+            if (f[j] >= limit && at[u] < n) reach |= 1u << (u * L::N + j);
         }
+        int k = warp_places(__popc(reach), found);
+        if (reach != 0)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            float f[L::N];
+            L::open(raw[u], f);
+#pragma unroll
+            for (int j = 0; j < L::N; ++j)
+              if (reach >> (u * L::N + j) & 1u) put(f[j], row.head + (v0 + at[u]) * L::N + j, k++);
+          }
       }
-      if (has_loose && loose >= limit) put(loose, loose_at);
+      if (row.loose() > 0) {
+        const bool reaches = has_loose && loose >= limit;
+        k = warp_places(reaches, found);
+        if (reaches) put(loose, loose_at, k);
+      }
     }
     if (parts > 1) cluster.sync(); else ts_sync();
     if (part != 0) return;
