@@ -106,6 +106,8 @@ extend_block_tables_kernel(int* __restrict__ table, long long ldt, int S, int wi
 constexpr int SM_THREADS = 256;
 constexpr int SM_TOKENS = 4;  // consecutive tokens of a thread: 16 and 32 bytes of output
 constexpr int SM_TURNS = 4;   // times that a block goes on: its sums over the batch are made once for 4096 tokens
+// 512 sequences of 2.3 million tokens: 15 us for 28 MB (1.9 TB/s; 4.5 us at the copy rate) in 568 blocks. A block's time is a chain: two sums over the
+// batch, the search for its sequences, row and start, page, stores. Look-ups token by token, of which a warp nearly always needs some, took 17 us.
 
 __global__ void __launch_bounds__(SM_THREADS)
 build_slot_map_kernel(const int* __restrict__ table, long long ldt, int S, int width, const int* __restrict__ rows, const int* __restrict__ starts,
@@ -127,43 +129,72 @@ build_slot_map_kernel(const int* __restrict__ table, long long ldt, int S, int w
   if (blockIdx.x == 0)
     for (int i = threadIdx.x; i <= B; i += blockDim.x) cu_out[i] = cu[i];
   const int end = cu[B];
+  // Four tokens of one sequence are on one page or two: those of all turns are looked up together. A warp's tokens always meet the end of a page.
+  int t0[SM_TURNS], p0[SM_TURNS], lo[SM_TURNS], row[SM_TURNS], blk[SM_TURNS], next[SM_TURNS];
+#pragma unroll
   for (int turn = 0; turn < SM_TURNS; ++turn) {
-    const int t0 = ((blockIdx.x * SM_TURNS + turn) * SM_THREADS + threadIdx.x) * SM_TOKENS;
-    if (t0 >= total) return;
-    int lo = 0, hi = B;  // the sequence of t0: the last i with cu[i] <= t0, as far as there is one
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (cu[mid] <= t0) lo = mid; else hi = mid;
+    t0[turn] = ((blockIdx.x * SM_TURNS + turn) * SM_THREADS + threadIdx.x) * SM_TOKENS;
+    int i = 0, hi = B;  // the sequence of t0: the last i with cu[i] <= t0, as far as there is one
+    if (t0[turn] < end)
+      while (hi - i > 1) {
+        const int mid = (i + hi) >> 1;
+        if (cu[mid] <= t0[turn]) i = mid; else hi = mid;
+      }
+    lo[turn] = i;
+    p0[turn] = row[turn] = -1;
+    if (t0[turn] < end) {
+      p0[turn] = max(starts[i], 0) + t0[turn] - cu[i];
+      row[turn] = rows[i];
     }
+  }
+#pragma unroll
+  for (int turn = 0; turn < SM_TURNS; ++turn) {
+    const int p = p0[turn], r = row[turn], j = shift >= 0 ? p >> shift : p / bs, k = j + (p - j * bs + SM_TOKENS > bs);
+    const bool there = p >= 0 && r >= 0 && r < S;
+    blk[turn] = there && j < width ? table[r * ldt + j] : -1;
+    next[turn] = there && k < width ? table[r * ldt + k] : -1;
+  }
+#pragma unroll
+  for (int turn = 0; turn < SM_TURNS; ++turn) {
+    if (t0[turn] >= total) return;
     int at[SM_TOKENS];
     long long slot[SM_TOKENS];
-    int last_lo = -1, last_j = -1, blk = -1;
+    const int p = p0[turn], off = shift >= 0 ? p & (bs - 1) : p % bs;
+    if (p >= 0 && t0[turn] + SM_TOKENS <= cu[lo[turn] + 1] && bs >= SM_TOKENS) {
+      const long long first = static_cast<long long>(blk[turn]) * bs + off, second = (static_cast<long long>(next[turn]) - 1) * bs + off;
 #pragma unroll
-    for (int u = 0; u < SM_TOKENS; ++u) {
-      const int t = t0 + u;
-      at[u] = 0;
-      slot[u] = -1;
-      if (t >= end) continue;
-      while (cu[lo + 1] <= t) ++lo;
-      const int p = max(starts[lo], 0) + t - cu[lo], j = shift >= 0 ? p >> shift : p / bs;
-      at[u] = p;
-      if (lo != last_lo || j != last_j) {
-        const int r = rows[lo];
-        blk = p >= 0 && r >= 0 && r < S && j < width ? table[r * ldt + j] : -1;
-        last_lo = lo;
-        last_j = j;
+      for (int u = 0; u < SM_TOKENS; ++u) {
+        const bool same = off + u < bs;
+        at[u] = p + u;
+        slot[u] = (same ? blk[turn] : next[turn]) >= 0 ? (same ? first : second) + u : -1;
       }
-      if (blk >= 0) slot[u] = static_cast<long long>(blk) * bs + (p - j * bs);
-    }
-    if (t0 + SM_TOKENS <= total) {
-      *reinterpret_cast<int4*>(positions + t0) = make_int4(at[0], at[1], at[2], at[3]);
-      *reinterpret_cast<longlong2*>(slots + t0) = make_longlong2(slot[0], slot[1]);
-      *reinterpret_cast<longlong2*>(slots + t0 + 2) = make_longlong2(slot[2], slot[3]);
     } else {
-      for (int u = 0; u < SM_TOKENS && t0 + u < total; ++u) {
-        positions[t0 + u] = at[u];
-        slots[t0 + u] = slot[u];
+      int i = lo[turn];
+#pragma unroll
+      for (int u = 0; u < SM_TOKENS; ++u) {
+        const int t = t0[turn] + u;
+        at[u] = 0;
+        slot[u] = -1;
+        if (t >= end) continue;
+        while (cu[i + 1] <= t) ++i;
+        const int q = max(starts[i], 0) + t - cu[i], j = shift >= 0 ? q >> shift : q / bs, r = rows[i];
+        at[u] = q;
+        if (q < 0 || r < 0 || r >= S || j >= width) continue;
+        const int page = table[r * ldt + j];
+        if (page >= 0) slot[u] = static_cast<long long>(page) * bs + (q - j * bs);
       }
+    }
+    if (t0[turn] + SM_TOKENS <= total) {
+      *reinterpret_cast<int4*>(positions + t0[turn]) = make_int4(at[0], at[1], at[2], at[3]);
+      *reinterpret_cast<longlong2*>(slots + t0[turn]) = make_longlong2(slot[0], slot[1]);
+      *reinterpret_cast<longlong2*>(slots + t0[turn] + 2) = make_longlong2(slot[2], slot[3]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < SM_TOKENS; ++u)
+        if (t0[turn] + u < total) {
+          positions[t0[turn] + u] = at[u];
+          slots[t0[turn] + u] = slot[u];
+        }
     }
   }
 }
