@@ -309,6 +309,18 @@ def test_attention_over_the_cache(dev, nh, nkv, hd, bs, lens, dtype):
     assert (np.abs(again.double().cpu().numpy() - want) <= off + HALF[dtype] * np.abs(want) + 2.0**-24).all()
 
 
+@pytest.mark.parametrize("nh,nkv,hd,bs,lens", [(28, 4, 128, 64, [700, 129, 1000]), (12, 1, 64, 16, [255, 33]), (16, 1, 128, 32, [1200, 31]), (14, 2, 64, 64, [5000])])
+def test_attention_in_fp16_is_rounded_once(dev, nh, nkv, hd, bs, lens):
+    """What the output's own rounding (at most 2^-11 of each value) does not explain is fp32 sums: scores below 2^4 from products whose magnitudes, with the
+    64 that a code is held on, sum to below 2^10; 2^5 roundings of random sign of 2^-24 of that, weighed by a softmax, are below 2^-14."""
+    rs = np.random.RandomState(nh + hd)
+    pages, table, ctx = make_pool(rs, lens, nkv, hd, bs, -(-max(lens) // bs), dev)
+    q = torch.from_numpy(rs.randn(len(lens), nh, hd)).half().to(dev)
+    out = F.paged_decode_attention_kv4(q, pages, table, ctx).double().cpu().numpy()
+    want, _ = attention_64(q, pages, table, lens, bs, 1.0 / math.sqrt(hd))
+    assert np.linalg.norm(out - want) <= (2.0**-11 + 2.0**-14) * np.linalg.norm(want)
+
+
 @pytest.mark.parametrize("factor", [1e-20, 1e-3, 300.0, 1e12])
 def test_attention_with_queries_of_any_size(dev, factor):
     """Queries are brought to a common power of two before they are rounded to fp16: tiny ones keep their bits, large ones do not overflow."""

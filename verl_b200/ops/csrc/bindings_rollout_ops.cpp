@@ -245,8 +245,8 @@ Tensor token_scores_bwd(const Tensor& logits, const Tensor& given, const Tensor&
   return dx;
 }
 
-// Log-probs and entropy with their gradient. In C++, because a function written in Python costs more on the host (146 us a step, 36 of them
-// forward) than the kernels of most batches on the device.
+// Log-probs and entropy with their gradient. In C++, because a function written in Python costs more on the host than the kernels of most
+// batches on the device: 146 us a step where this takes 68 (of which about 45 are any graph's).
 struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& ids, double temperature, int64_t valid) {
     at::AutoDispatchBelowADInplaceOrView below;

@@ -20,7 +20,16 @@
 //   S gains m (sum of q over the thread's channels), one more k step of an instruction that has m twice against that sum's two fp16 halves;
 //   O gains sum_t p_t m_t, the same for all channels of a thread: one accumulator more, added at the end.
 // 1.1 instructions an element. Queries are scaled by a power of two per head, into fp16's range; weights are e^(s - reference) <= 64 in fp16.
+// These roundings to 11 bits (6e-4 of the output's norm in all) are below those of a bf16 output (1.7e-3). For fp16 (2.1e-4 by its own rounding) there are
+// none: codes apart from each other, scales in two parts of at most seven bits, under which codes are exact, weights in two halves. That takes two and
+// three matrix instructions for one, and 1.65 times the time where instructions count.
+//
+// 320 sequences of 28 heads over 4 KV heads of 128 channels, 2048 tokens on average: 115 to 125 us for 525 MB with the join (0.65 to 0.7 of the copy
+// rate; fp16 190). Copies alone would take 98 us with the join, the instructions 106: both are near their limits, and warps that wait for one do not
+// always cover the other. One sequence of 131072 tokens, 8 KV heads: 47 us for 168 MB (fp16 70), 8 of them the join's. Four of 160 tokens: 12 us, two launches.
 #include <math.h>
+
+#include <type_traits>
 
 #include "kv4_common.cuh"
 #include "rollout_ops.h"
@@ -99,6 +108,37 @@ __device__ __forceinline__ void kd_numbers(uint32_t (&x)[4], uint32_t w, const S
   x[3] = fma2(high, f.s, f.n);
 }
 
+// For fp16 outputs, all of it exact: the codes apart from each other, and the scale in two parts of at most seven bits, under which a code is a
+// number of at most eleven.
+struct FineScales {
+  Scales hi, lo;
+  static __device__ __forceinline__ uint32_t rest(uint32_t v) {
+    uint32_t d;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(v), "r"(v & 0xfff0fff0u));
+    return d;
+  }
+  __device__ __forceinline__ explicit FineScales(uint32_t v) : hi(v & 0xfff0fff0u), lo(rest(v)) {}
+};
+// The pairs (0, 4), (1, 5), (2, 6), (3, 7) of a word, x[0..3] times the first part of their scales and x[4..7] times the second
+__device__ __forceinline__ void kd_numbers(uint32_t (&x)[8], uint32_t w, const FineScales& f, uint32_t magic) {
+  const uint32_t up = w << 4;
+  uint32_t c[4];
+  asm("lop3.b32 %0, %1, 0x00f000f0, %2, 0xea;" : "=r"(c[0]) : "r"(up), "r"(magic));
+  asm("lop3.b32 %0, %1, 0x00f000f0, %2, 0xea;" : "=r"(c[1]) : "r"(w), "r"(magic));
+  c[2] = __byte_perm(up, magic, 0x7351) & 0xfff0fff0u;
+  c[3] = __byte_perm(w, magic, 0x7351) & 0xfff0fff0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[i] = fma2(c[i], f.hi.s, f.hi.n);
+    x[4 + i] = fma2(c[i], f.lo.s, f.lo.n);
+  }
+}
+// What is left of two numbers behind their fp16 roundings
+__device__ __forceinline__ uint32_t pack2_rest(float lo, float hi, uint32_t rounded) {
+  const __half2 h = *reinterpret_cast<const __half2*>(&rounded);
+  return pack2(lo - __low2float(h), hi - __high2float(h));
+}
+
 template <int HD, int NT>
 struct KDSmem {
   static constexpr int CODES = KD_PIECE * HD / 2;             // of keys, or of values
@@ -164,6 +204,9 @@ template <int HD, int NT, typename T>
 __global__ void __launch_bounds__(KD_THREADS, kd_ctas(HD, NT))
 kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
   using L = KDSmem<HD, NT>;
+  constexpr bool FINE = std::is_same<T, __half>::value;  // numbers, queries and weights without a rounding that an output of 11 bits would show
+  using Sc = std::conditional_t<FINE, FineScales, Scales>;
+  constexpr int PARTS = FINE ? 2 : 1;
   constexpr int CPR = HD / 4, VPR = HD / 8, KW = CPR / 8, VW = VPR / 8;  // channels of a thread's run, and words of them
   extern __shared__ __align__(16) uint8_t smem[];  // 16 bytes are what bulk copies ask for
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.nh / p.nkv, bs = p.block_size;
@@ -273,7 +316,10 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
       for (int w = 0; w < KW; ++w)
 #pragma unroll
         for (int j = 0; j < 4; j += 2) {
-          qf[t][w][j] = pack2(fmaf(16.f, x[w * 8 + j], -x[w * 8 + j + 1]), fmaf(16.f, x[w * 8 + j + 4], -x[w * 8 + j + 5]));
+          if constexpr (FINE)
+            qf[t][w][j] = pack2(x[w * 8 + j], x[w * 8 + j + 4]);
+          else
+            qf[t][w][j] = pack2(fmaf(16.f, x[w * 8 + j], -x[w * 8 + j + 1]), fmaf(16.f, x[w * 8 + j + 4], -x[w * 8 + j + 5]));
           qf[t][w][j + 1] = pack2(x[w * 8 + j + 1], x[w * 8 + j + 5]);
         }
       const float hi = __half2float(__float2half_rn(sum));
@@ -303,7 +349,7 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
       const bool work = ok && left > 0, ragged = left < KD_PIECE || lost != 0;
       // does token i of the piece count?
       const auto counts = [&](int i) { return i < left && !((lost >> (4 * (i / tokens))) & 1u); };
-      uint32_t pb[NT][KD_TILES][2];
+      uint32_t pb[PARTS][NT][KD_TILES][2];
       if (work) {
         const uint8_t* kc = stage + krow * (HD / 2) + c * (CPR / 2);
         const uint8_t* kp = stage + L::OFF_PK + (krow * (HD / KV4_GROUP) + c * CPR / KV4_GROUP) * 4;
@@ -324,21 +370,20 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
             }
             par[h] = *reinterpret_cast<const uint32_t*>(kp + (i * 16 + h * 8) * (HD / KV4_GROUP) * 4);
           }
-          const Scales f0(__byte_perm(par[0], 0u, 0x1010)), f1(__byte_perm(par[1], 0u, 0x1010));
+          const Sc f0(__byte_perm(par[0], 0u, 0x1010)), f1(__byte_perm(par[1], 0u, 0x1010));
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             mma_f16_16816_from_zero(st[t][i], __byte_perm(par[0], 0u, 0x3232), __byte_perm(par[1], 0u, 0x3232), 0u, 0u, qs[t], 0u);
           }
 #pragma unroll
           for (int w = 0; w < KW; ++w) {
-            uint32_t a[4], b[4];
+            uint32_t a[4 * PARTS], b[4 * PARTS];
             kd_numbers(a, wk[0][w], f0, magic);
             kd_numbers(b, wk[1][w], f1, magic);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              mma_f16_16816(st[t][i], a[0], b[0], a[1], b[1], qf[t][w][0], qf[t][w][1]);
-              mma_f16_16816(st[t][i], a[2], b[2], a[3], b[3], qf[t][w][2], qf[t][w][3]);
-            }
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int k = 0; k < 4 * PARTS; k += 2) mma_f16_16816(st[t][i], a[k], b[k], a[k + 1], b[k + 1], qf[t][w][k & 3], qf[t][w][(k & 3) + 1]);
           }
         }
         __syncwarp();
@@ -391,8 +436,13 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
           }
 #pragma unroll
           for (int i = 0; i < KD_TILES; ++i) {
-            pb[t][i][0] = movmatrix_t(pack2(st[t][i][0], st[t][i][1]));
-            pb[t][i][1] = movmatrix_t(pack2(st[t][i][2], st[t][i][3]));
+            const uint32_t w0 = pack2(st[t][i][0], st[t][i][1]), w1 = pack2(st[t][i][2], st[t][i][3]);
+            pb[0][t][i][0] = movmatrix_t(w0);
+            pb[0][t][i][1] = movmatrix_t(w1);
+            if constexpr (FINE) {
+              pb[1][t][i][0] = movmatrix_t(pack2_rest(st[t][i][0], st[t][i][1], w0));
+              pb[1][t][i][1] = movmatrix_t(pack2_rest(st[t][i][2], st[t][i][3], w1));
+            }
           }
         }
       } else if (ok && next < u1) {
@@ -425,23 +475,31 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
             for (int j = 0; j < 4; ++j)
               if (!counts(i * 16 + j * 4 + c)) pv[j] = 0u;  // values of zero
           }
-          const Scales f01(__byte_perm(pv[0], pv[1], 0x5410)), f23(__byte_perm(pv[2], pv[3], 0x5410));
+          const Sc f01(__byte_perm(pv[0], pv[1], 0x5410)), f23(__byte_perm(pv[2], pv[3], 0x5410));
           const uint32_t m01 = __byte_perm(pv[0], pv[1], 0x7632), m23 = __byte_perm(pv[2], pv[3], 0x7632);
 #pragma unroll
-          for (int t = 0; t < NT; ++t) mma_f16_16816(z[t], m01, 0u, m23, 0u, pb[t][i][0], pb[t][i][1]);
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int k = 0; k < PARTS; ++k) mma_f16_16816(z[t], m01, 0u, m23, 0u, pb[k][t][i][0], pb[k][t][i][1]);
 #pragma unroll
           for (int w = 0; w < VW; ++w)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {  // channels 0..3 and 4..7 of the word: a pair of tokens side by side
               const uint32_t sel = half == 0 ? 0x5410 : 0x7632;
-              uint32_t x[4], y[4];
+              uint32_t x[4 * PARTS], y[4 * PARTS];
               kd_numbers(x, __byte_perm(wv[0][w], wv[1][w], sel), f01, magic);
               kd_numbers(y, __byte_perm(wv[2][w], wv[3][w], sel), f23, magic);
 #pragma unroll
-              for (int t = 0; t < NT; ++t) {
-                mma_f16_16816(o[t][w * 4 + half * 2], x[0], x[1], y[0], y[1], pb[t][i][0], pb[t][i][1]);
-                mma_f16_16816(o[t][w * 4 + half * 2 + 1], x[2], x[3], y[2], y[3], pb[t][i][0], pb[t][i][1]);
-              }
+              for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                  float (&to)[4] = o[t][w * 4 + half * 2 + k];
+                  mma_f16_16816(to, x[2 * k], x[2 * k + 1], y[2 * k], y[2 * k + 1], pb[0][t][i][0], pb[0][t][i][1]);
+                  if constexpr (FINE) {
+                    mma_f16_16816(to, x[4 + 2 * k], x[5 + 2 * k], y[4 + 2 * k], y[5 + 2 * k], pb[0][t][i][0], pb[0][t][i][1]);
+                    mma_f16_16816(to, x[2 * k], x[2 * k + 1], y[2 * k], y[2 * k + 1], pb[1][t][i][0], pb[1][t][i][1]);
+                  }
+                }
             }
         }
       }
@@ -466,8 +524,8 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
         float x[VPR];
 #pragma unroll
         for (int i = 0; i < HD / 16; ++i) {
-          x[2 * i] = fmaf(16.f, o[t][i][h], z[t][h]);
-          x[2 * i + 1] = o[t][i][2 + h] - o[t][i][h] + z[t][h];
+          x[2 * i] = fmaf(FINE ? 1.f : 16.f, o[t][i][h], z[t][h]);
+          x[2 * i + 1] = o[t][i][2 + h] - (FINE ? 0.f : o[t][i][h]) + z[t][h];
         }
         if (whole) {
           const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -598,7 +656,7 @@ static cudaError_t kd_launch(const VbKv4Decode& p, int* status, cudaStream_t s) 
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
   // A block per (sequence, KV head), or where each has many runs (few sequences with long contexts) one per query head with threads that share
-  // the runs: one sequence of 131072 tokens (296 runs a head) 24 us and 6 us; 320 sequences (3 runs a head) 10.5 us.
+  // the runs: one sequence of 131072 tokens (222 runs a head) 24 us and 8 us; 320 sequences (2 runs a head) 8.4 us.
   const int runs = ctas * KD_WARPS, many = runs / (p.B * p.nkv) >= 16, heads = many ? 1 : p.nh / p.nkv, threads = many ? 512 : 128;
   cfg.gridDim = dim3(p.nh / heads, p.B);
   cfg.blockDim = dim3(threads);
