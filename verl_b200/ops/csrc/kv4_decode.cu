@@ -24,7 +24,7 @@
 // none: codes apart from each other, scales in two parts of at most seven bits, under which codes are exact, weights in two halves. That takes two and
 // three matrix instructions for one, and 1.65 times the time where instructions count.
 //
-// 320 sequences of 28 heads over 4 KV heads of 128 channels, 2048 tokens on average: 115 to 125 us for 525 MB with the join (0.65 to 0.7 of the copy
+// 320 sequences of 28 heads over 4 KV heads of 128 channels, 2560 tokens on average: 115 to 125 us for 525 MB with the join (0.65 to 0.7 of the copy
 // rate; fp16 190). Copies alone would take 98 us with the join, the instructions 106: both are near their limits, and warps that wait for one do not
 // always cover the other. One sequence of 131072 tokens, 8 KV heads: 47 us for 168 MB (fp16 70), 8 of them the join's. Four of 160 tokens: 12 us, two launches.
 #include <math.h>
