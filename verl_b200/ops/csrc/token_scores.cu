@@ -2,7 +2,8 @@
 //
 // With y = x log2(e) / temperature and a reference M near the largest y, a row is read once for
 //   s = sum 2^(y - M),  w = sum 2^(y - M) (y - M):   lse = ln2 (M + log2 s),  H = ln2 (log2 s - w / s)
-// five instructions and one exponential a value. A thread keeps a reference of its own, which moves only when a value is 2^60 above it.
+// four instructions and one exponential a value. A thread keeps a reference of its own, the largest of its first values, which moves only when the sum
+// is 2^40 above it.
 //
 // The most likely tokens come with the same pass: every thread also keeps the largest value that it met, and the k-th largest of those of a
 // block is a bound that at least k values of the row reach. The largest value of each group of 32 (16 of 32 bits) stays in shared memory, and
@@ -404,7 +405,7 @@ __device__ __forceinline__ void bulk_row(void* dst, const T* src, uint32_t bytes
                : "memory");
 }
 
-template <typename T>
+template <typename T, bool TOP>
 __global__ void __launch_bounds__(TS_THREADS + 32, TS_BLOCKS)
 token_scores_kernel(const VbScores p, int* status) {
   using L = Lane<T>;
@@ -467,17 +468,8 @@ token_scores_kernel(const VbScores p, int* status) {
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], round & 1));
       const uint4* at = ring + stage * TS_CHUNK + threadIdx.x;
       const int left = n - v - static_cast<int>(threadIdx.x);
-      // The vectors are read from shared memory for the maximum and again for the sums: held in between, they would not fit the registers.
-      float big = -INFINITY;
-      if constexpr (sizeof(T) == 2) {
-        uint32_t top = 0x80008000u;
-#pragma unroll
-        for (int u = 0; u < TS_PER; ++u)
-          if (left > u * TS_THREADS) top = pair_max(top, pair_max(at[u * TS_THREADS]));
-        top = pair_max(top, top >> 16 | 0x80000000u) & 0xffffu;
-        if (top < 0x8000u) big = static_cast<float>(*reinterpret_cast<const T*>(&top));
-      }
-      if (big == -INFINITY)  // 32-bit values, or nothing that is not negative (NaN left aside)
+      const auto largest = [&]() {  // of this thread's values in the stage, NaN left aside
+        float big = -INFINITY;
 #pragma unroll
         for (int u = 0; u < TS_PER; ++u) {
           float f[L::N];
@@ -485,22 +477,26 @@ token_scores_kernel(const VbScores p, int* status) {
 #pragma unroll
           for (int i = 0; i < L::N; i += 2) big = fmaxf(big, fmaxf(f[i], f[i + 1]));
         }
-      most = fmaxf(most, big);
-      if (p.top > 0) {
-        uint16_t* keep = &sh.top[slot % TS_SLOTS][threadIdx.x];
-        const uint16_t key = static_cast<uint16_t>(order_key(big) >> 16);
-        *keep = slot < TS_SLOTS ? key : max(*keep, key);
+        return big;
+      };
+      if (slot == 0) {
+        const float big = largest();
+        if (big * c > a.m) a.move(big * c);
       }
-      if (big * c > a.m + 60.f) a.move(big * c);
       unsigned long long s2 = ts_two(a.s, 0.f), w2 = ts_two(a.w, 0.f);
       const unsigned long long c2 = ts_two(c, c), m2 = ts_two(-a.m, -a.m);
+      uint32_t pairs = 0x80008000u;
+      float big = -INFINITY;
 #pragma unroll
       for (int u = 0; u < TS_PER; ++u) {
         if (left <= u * TS_THREADS) break;
+        const uint4 v = at[u * TS_THREADS];
         float f[L::N];
-        L::open(at[u * TS_THREADS], f);
+        L::open(v, f);
+        if constexpr (TOP && sizeof(T) == 2) pairs = pair_max(pairs, pair_max(v));
 #pragma unroll
         for (int i = 0; i < L::N; i += 2) {
+          if constexpr (TOP && sizeof(T) == 4) big = fmaxf(big, fmaxf(f[i], f[i + 1]));
           const unsigned long long d2 = ts_fma(ts_two(f[i], f[i + 1]), c2, m2);
           const float2 d = ts_of(d2);
           const unsigned long long e2 = ts_two(ts_exp2(d.x), ts_exp2(d.y));
@@ -509,10 +505,12 @@ token_scores_kernel(const VbScores p, int* status) {
         }
       }
       const float2 s = ts_of(s2), w = ts_of(w2);
-      if (w.x + w.y == w.x + w.y) {
+      if (s.x + s.y < 0x1p40f && w.x + w.y == w.x + w.y) {
         a.s = s.x + s.y;
         a.w = w.x + w.y;
-      } else {  // 0 * -inf got into the sums: again with a floor under the exponents
+      } else {  // too far above the reference, or 0 * -inf got into the sums: again, with a floor under the exponents
+        const float up = fmaxf(largest() * c, a.s > 0.f ? a.m + log2f(a.s) : -INFINITY);
+        if (up > a.m + 20.f) a.move(up);
 #pragma unroll 1
         for (int u = 0; u < TS_PER; ++u) {
           if (left <= u * TS_THREADS) break;
@@ -521,6 +519,16 @@ token_scores_kernel(const VbScores p, int* status) {
 #pragma unroll
           for (int i = 0; i < L::N; ++i) a.add(fmaf(f[i], c, 0.f));
         }
+      }
+      if constexpr (TOP) {
+        if constexpr (sizeof(T) == 2) {
+          pairs = pair_max(pairs, pairs >> 16 | 0x80000000u) & 0xffffu;
+          big = pairs < 0x8000u ? static_cast<float>(*reinterpret_cast<const T*>(&pairs)) : largest();  // nothing that is not negative
+        }
+        most = fmaxf(most, big);
+        uint16_t* keep = &sh.top[slot % TS_SLOTS][threadIdx.x];
+        const uint16_t key = static_cast<uint16_t>(order_key(big) >> 16);
+        *keep = slot < TS_SLOTS ? key : max(*keep, key);
       }
       __syncwarp();
       if ((threadIdx.x & 31) == 0) mbar_arrive(&empty[stage]);
@@ -543,7 +551,7 @@ token_scores_kernel(const VbScores p, int* status) {
     // ---- the bound: bit by bit, the largest key that `top` threads' largest values reach (100 cycles a bit; by one warp with eight keys a lane, 170)
     uint32_t bound = 0;
     const uint32_t mine = any ? order_key(most) : 0u;
-    if (p.top > 0)
+    if constexpr (TOP)
       for (int bit = 31; bit >= L::LOW; --bit) {
         const uint32_t want = bound | (1u << bit);
         if (ts_count(mine >= want) >= p.top) bound = want;
@@ -570,7 +578,7 @@ token_scores_kernel(const VbScores p, int* status) {
 
     // ---- what reaches the bound, into the first block's list
     Shared* first = parts > 1 ? cluster.map_shared_rank(&sh, 0) : &sh;
-    if (p.top > 0 && !odd) {
+    if (TOP && !odd) {
       const float limit = bound <= order_key(-INFINITY) ? -INFINITY : key_value(bound);
       const int chunks = (n + TS_CHUNK - 1) / TS_CHUNK, low = static_cast<int>(bound >> 16);
       uint32_t hits = 0;
@@ -745,7 +753,7 @@ static cudaError_t ts_forward(const VbScores& a, cudaStream_t s) {
   int parts = 1;
   while (parts < 8 && 2LL * parts * a.T <= 3 * num_sms() && a.V / Lane<T>::N >= 2048 * parts) parts *= 2;
   constexpr int smem = TS_STAGES * TS_CHUNK * 16;
-  auto kern = token_scores_kernel<T>;
+  auto kern = a.top > 0 ? token_scores_kernel<T, true> : token_scores_kernel<T, false>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   int* status = nullptr;
   if (e == cudaSuccess) e = cudaGetSymbolAddress(reinterpret_cast<void**>(&status), g_ts_status);
