@@ -458,6 +458,37 @@ def test_scores(dev, T, V, valid, n, top, temperature, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("top", [0, 20])
+@pytest.mark.parametrize("V", [9000, 70000, 200000])
+def test_scores_of_rows_that_grow(dev, V, top, dtype):
+    """The first values of a row say nothing about the others: slopes, steps and single values far above what was there before, and all of it below zero."""
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(8, V, generator=g)
+    slope = torch.linspace(-1, 1, V)
+    x[0] += slope * 300
+    x[1] -= slope * 300
+    x[2, : V // 2] -= 5e4
+    x[3, V - 3] = 80.0
+    x[4, V // 2 :] += 45.0
+    x[5] += slope * 20
+    x[6] = x[6] - 1e3 + (torch.arange(V) // 3000) * 25.0
+    x[7, : V - 100] = float("-inf")
+    x = x.to(dtype).to(dev)
+    ids = torch.full((8,), V - 3, device=dev)
+    out = F.token_scores(x, ids, top)
+    lp, ent, lse, order, top_lp = scores_64(x, ids, top, 1.0, V)
+    tol = slack(x, V, 1.0)
+    assert torch.equal(out.top_ids.cpu(), order)
+    assert ((out.lse.double().cpu() - lse).abs() <= tol).all() and ((out.logprob.double().cpu() - lp).abs() <= 2 * tol).all()
+    assert ((out.top_logprob.double().cpu() - top_lp).abs() <= 2 * tol[:, None]).all()
+    # log s - w / s, with the terms of w up to 40 ln 2 (the least distance at which a reference moves) and the spread of the row larger than those of s
+    z = x.double().cpu()
+    p = torch.softmax(z, -1)
+    spread = torch.where(p > 0, p * (z.amax(-1, keepdim=True) - z), 0.0).sum(-1)
+    assert ((out.entropy.double().cpu() - ent).abs() <= tol * (2 + spread + 40 * math.log(2))).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("V", [40, 3001, 70000])
 def test_scores_of_masked_tied_and_undefined_rows(dev, V, dtype):
     g = torch.Generator().manual_seed(V)
