@@ -321,6 +321,36 @@ def test_attention_in_fp16_is_rounded_once(dev, nh, nkv, hd, bs, lens):
     assert np.linalg.norm(out - want) <= (2.0**-11 + 2.0**-14) * np.linalg.norm(want)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attention_over_long_contexts(dtype):
+    """Values of either sign cancel over a long context: what is left is small beside the codes, on which the sums must not lose it. The bound is the output's
+    rounding, at most HALF of each value, and for bf16 as much again for the fp16 roundings of codes and weights (together below 2^-10 of the norm)."""
+    B, nkv, G, hd, bs, n = 4, 2, 8, 64, 64, 80000
+    g = torch.Generator(device="cuda").manual_seed(3)
+    blocks = n // bs
+    pages = torch.randint(0, 256, (B * blocks, nkv, F.kv4_page_bytes(bs, hd)), dtype=torch.uint8, device="cuda", generator=g)
+    par = torch.empty(B * blocks, nkv, 2, bs, hd // 32, 2, dtype=torch.float16, device="cuda")
+    step = torch.rand(par.shape[:-1], device="cuda", generator=g) * 0.25 + 0.05
+    par[..., 0] = step
+    par[..., 1] = -7.5 * step + 0.2 * torch.randn(step.shape, device="cuda", generator=g)
+    pages[..., bs * hd :] = par.reshape(B * blocks, nkv, -1).view(torch.uint8)
+    table = torch.randperm(B * blocks, device="cuda", generator=g).to(torch.int32).view(B, blocks)
+    q = torch.randn(B, nkv * G, hd, device="cuda", generator=g).to(dtype)
+    out = F.paged_decode_attention_kv4(q, pages, table, torch.full((B,), n, dtype=torch.int32, device="cuda")).double()
+    want = torch.empty_like(out)
+    for b in range(B):
+        rows = table[b].long()
+        code = pages[rows, :, : bs * hd].view(blocks, nkv, 2, bs, hd // 2)
+        x = torch.stack([code & 15, code >> 4], -1).view(blocks, nkv, 2, bs, hd // 32, 32).double()
+        pr = par[rows].double()
+        k, v = (x * pr[..., :1] + pr[..., 1:]).permute(2, 1, 0, 3, 4, 5).reshape(2, nkv, n, hd)
+        w = torch.softmax(torch.einsum("hgd,htd->hgt", q[b].double().view(nkv, G, hd), k) / math.sqrt(hd), -1)
+        want[b] = torch.einsum("hgt,htd->hgd", w, v).view(nkv * G, hd)
+    bound = HALF[dtype] + (2.0**-10 if dtype == torch.bfloat16 else 2.0**-14)
+    assert float((out - want).norm() / want.norm()) <= bound
+
+
 @pytest.mark.parametrize("factor", [1e-20, 1e-3, 300.0, 1e12])
 def test_attention_with_queries_of_any_size(dev, factor):
     """Queries are brought to a common power of two before they are rounded to fp16: tiny ones keep their bits, large ones do not overflow."""

@@ -21,12 +21,13 @@
 //   O gains sum_t p_t m_t, the same for all channels of a thread: one accumulator more, added at the end.
 // 1.1 instructions an element. Queries are scaled by a power of two per head, into fp16's range; weights are e^(s - reference) <= 64 in fp16.
 // These roundings to 11 bits (6e-4 of the output's norm in all) are below those of a bf16 output (1.7e-3). For fp16 (2.1e-4 by its own rounding) there are
-// none: codes apart from each other, scales in two parts of at most seven bits, under which codes are exact, weights in two halves. That takes two and
-// three matrix instructions for one, and 1.65 times the time where instructions count.
+// none: codes apart from each other, scales in two parts of at most seven bits, under which codes are exact, weights in two halves; values count from
+// code 8, because the sum of codes and that of least values would each be hundreds of times their difference over a long context, and matrix
+// instructions add up by cutting off. That takes two and three matrix instructions for one, and 1.75 times the time where instructions count.
 //
 // 320 sequences of 28 heads over 4 KV heads of 128 channels, 2560 tokens on average: 115 to 125 us for 525 MB with the join (0.65 to 0.7 of the copy
-// rate; fp16 190). Copies alone would take 98 us with the join, the instructions 106: both are near their limits, and warps that wait for one do not
-// always cover the other. One sequence of 131072 tokens, 8 KV heads: 47 us for 168 MB (fp16 70), 8 of them the join's. Four of 160 tokens: 12 us, two launches.
+// rate; fp16 200). Copies alone would take 98 us with the join, the instructions 106: both are near their limits, and warps that wait for one do not
+// always cover the other. One sequence of 131072 tokens, 8 KV heads: 47 us for 168 MB (fp16 72), 8 of them the join's. Four of 160 tokens: 12 us, two launches.
 #include <math.h>
 
 #include <type_traits>
@@ -119,7 +120,15 @@ struct FineScales {
   }
   __device__ __forceinline__ explicit FineScales(uint32_t v) : hi(v & 0xfff0fff0u), lo(rest(v)) {}
 };
-// The pairs (0, 4), (1, 5), (2, 6), (3, 7) of a word, x[0..3] times the first part of their scales and x[4..7] times the second
+__device__ __forceinline__ uint32_t add2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t minus2(uint32_t a) { return a ^ 0x80008000u; }
+// The pairs (0, 4), (1, 5), (2, 6), (3, 7) of a word, x[0..3] times the first part of their scales and x[4..7] times the second. EIGHT: codes - 8, as
+// products that a long sum does not take away from each other again.
+template <bool EIGHT = false>
 __device__ __forceinline__ void kd_numbers(uint32_t (&x)[8], uint32_t w, const FineScales& f, uint32_t magic) {
   const uint32_t up = w << 4;
   uint32_t c[4];
@@ -129,9 +138,25 @@ __device__ __forceinline__ void kd_numbers(uint32_t (&x)[8], uint32_t w, const F
   c[3] = __byte_perm(w, magic, 0x7351) & 0xfff0fff0u;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    x[i] = fma2(c[i], f.hi.s, f.hi.n);
-    x[4 + i] = fma2(c[i], f.lo.s, f.lo.n);
+    if constexpr (EIGHT) {
+      c[i] = add2(c[i], 0xd480d480u);  // -72; times it the scale could be infinite
+      x[i] = mul2(c[i], f.hi.s);
+      x[4 + i] = mul2(c[i], f.lo.s);
+    } else {
+      x[i] = fma2(c[i], f.hi.s, f.hi.n);
+      x[4 + i] = fma2(c[i], f.lo.s, f.lo.n);
+    }
   }
+}
+template <bool EIGHT>
+__device__ __forceinline__ void kd_numbers(uint32_t (&x)[4], uint32_t w, const Scales& f, uint32_t magic) {
+  kd_numbers(x, w, f, magic);
+}
+// Least values with 8 scales added, as a rounded sum and what it leaves, which is exact
+__device__ __forceinline__ void kd_least(uint32_t& m, uint32_t& rest, uint32_t scales) {
+  const uint32_t e = mul2(scales, 0x48004800u), sum = add2(m, e), part = add2(sum, minus2(m));
+  rest = add2(add2(m, minus2(add2(sum, minus2(part)))), add2(e, minus2(part)));
+  m = sum;
 }
 // What is left of two numbers behind their fp16 roundings
 __device__ __forceinline__ uint32_t pack2_rest(float lo, float hi, uint32_t rounded) {
@@ -417,6 +442,7 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
               m[t][h] = mx;
               l[t][h] *= alpha[h];
               z[t][h] *= alpha[h];
+              z[t][2 + h] *= alpha[h];
             }
 #pragma unroll
             for (int i = 0; i < HD / 16; ++i) {
@@ -476,19 +502,23 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
               if (!counts(i * 16 + j * 4 + c)) pv[j] = 0u;  // values of zero
           }
           const Sc f01(__byte_perm(pv[0], pv[1], 0x5410)), f23(__byte_perm(pv[2], pv[3], 0x5410));
-          const uint32_t m01 = __byte_perm(pv[0], pv[1], 0x7632), m23 = __byte_perm(pv[2], pv[3], 0x7632);
+          uint32_t m01 = __byte_perm(pv[0], pv[1], 0x7632), m23 = __byte_perm(pv[2], pv[3], 0x7632), r01 = 0u, r23 = 0u;
+          if constexpr (FINE) {
+            kd_least(m01, r01, __byte_perm(pv[0], pv[1], 0x5410));
+            kd_least(m23, r23, __byte_perm(pv[2], pv[3], 0x5410));
+          }
 #pragma unroll
           for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int k = 0; k < PARTS; ++k) mma_f16_16816(z[t], m01, 0u, m23, 0u, pb[k][t][i][0], pb[k][t][i][1]);
+            for (int k = 0; k < PARTS; ++k) mma_f16_16816(z[t], m01, r01, m23, r23, pb[k][t][i][0], pb[k][t][i][1]);
 #pragma unroll
           for (int w = 0; w < VW; ++w)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {  // channels 0..3 and 4..7 of the word: a pair of tokens side by side
               const uint32_t sel = half == 0 ? 0x5410 : 0x7632;
               uint32_t x[4 * PARTS], y[4 * PARTS];
-              kd_numbers(x, __byte_perm(wv[0][w], wv[1][w], sel), f01, magic);
-              kd_numbers(y, __byte_perm(wv[2][w], wv[3][w], sel), f23, magic);
+              kd_numbers<FINE>(x, __byte_perm(wv[0][w], wv[1][w], sel), f01, magic);
+              kd_numbers<FINE>(y, __byte_perm(wv[2][w], wv[3][w], sel), f23, magic);
 #pragma unroll
               for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -522,10 +552,11 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
         const int head = t * 8 + 2 * c + h;
         if (head >= G) continue;
         float x[VPR];
+        const float least = FINE ? z[t][h] + z[t][2 + h] : z[t][h];
 #pragma unroll
         for (int i = 0; i < HD / 16; ++i) {
-          x[2 * i] = fmaf(FINE ? 1.f : 16.f, o[t][i][h], z[t][h]);
-          x[2 * i + 1] = o[t][i][2 + h] - (FINE ? 0.f : o[t][i][h]) + z[t][h];
+          x[2 * i] = fmaf(FINE ? 1.f : 16.f, o[t][i][h], least);
+          x[2 * i + 1] = o[t][i][2 + h] - (FINE ? 0.f : o[t][i][h]) + least;
         }
         if (whole) {
           const float inv = sum == 0.f ? 0.f : 1.f / sum;
