@@ -20,9 +20,10 @@
 // Measured, rows of 152064: 2048 of bf16 without alternatives 104 us (6.0 TB/s, 0.93 of the copy rate), with 64 of them 135 us, with 128 161 us; the same in
 // fp32 219 us with 64 (0.88); their gradient, which reads once and writes once, 205 us in bf16 (0.94). One row of 151936: 12 us. What bounds the bf16
 // forward is HBM beside its exponentials (70 us at the 16 a cycle that an SM has), and with alternatives the end of a row (15000 cycles of 75000:
-// the bound 2300, the groups 2300, their values from memory 6600, ranks 4200), which blocks that started together reach together. 256 threads
-// and four blocks an SM: with fewer blocks nothing covers that end, with more the registers do not hold a vector's work. 24 slots, because a row of
-// 152064 has 19 stages; the keys of larger groups bring more values to look at.
+// the bound 2300, the groups 2300, their values from memory 6600, ranks 4200), a chain that an SM's three other blocks do not cover: blocks that
+// start a part of a row apart take as long. 256 threads and four blocks an SM: with fewer blocks less covers that end, with more the registers do not
+// hold a vector's work. 24 slots, because a row of 152064 has 19 stages; the keys of larger groups bring more values to look at. Stages of 16 KB: with
+// 8 KB, and as many bytes on their way or more, 137 us where they take 115, for what a stage costs beside its values.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
