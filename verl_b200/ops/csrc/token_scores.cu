@@ -180,8 +180,9 @@ struct Stat {
     s *= f;
     m = to;
   }
-  __device__ __forceinline__ void add(float y) {
-    const float d = ts_max_nan(y - m, TS_FLOOR), e = ts_exp2(d);
+  // a value f with y = f c, by the one rounding of f c - m that its log-prob has, so that a value that the sum consists of has a log-prob of 0
+  __device__ __forceinline__ void add(float f, float c) {
+    const float d = ts_max_nan(fmaf(f, c, -m), TS_FLOOR), e = ts_exp2(d);
     s += e;
     w = fmaf(e, d, w);
   }
@@ -518,7 +519,7 @@ token_scores_kernel(const VbScores p, int* status) {
           float f[L::N];
           L::open(at[u * TS_THREADS], f);
 #pragma unroll
-          for (int i = 0; i < L::N; ++i) a.add(fmaf(f[i], c, 0.f));
+          for (int i = 0; i < L::N; ++i) a.add(f[i], c);
         }
       }
       if constexpr (TOP) {
@@ -545,7 +546,7 @@ token_scores_kernel(const VbScores p, int* status) {
     if (has_loose) {
       most = fmaxf(most, loose);
       if (loose * c > a.m + 60.f) a.move(loose * c);
-      a.add(loose * c);
+      a.add(loose, c);
     }
     a = block_stat(a, sh.red);
 
