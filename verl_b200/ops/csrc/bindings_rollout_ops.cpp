@@ -211,7 +211,8 @@ VbScores scores_of(const Tensor& x, const Tensor& ids, double temperature, int64
 }
 Tensor by_rows(const Tensor& x) { return x.dim() == 2 && x.stride(1) != 1 && x.size(1) > 1 ? x.contiguous() : x; }
 
-std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_scores(const Tensor& logits, const Tensor& given, int64_t top, double temperature, int64_t valid) {
+// `stat`, where the gradient is to follow: [rows, 4] fp32, what it wants of the rows.
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> scores(const Tensor& logits, const Tensor& given, int64_t top, double temperature, int64_t valid, float* stat) {
   const Tensor x = by_rows(logits), ids = given.contiguous();
   VbScores a = scores_of(x, ids, temperature, valid, "token_scores");
   TORCH_CHECK_VALUE(top >= 0 && top <= std::min(128, a.V), "token_scores: top_k must lie in 0 .. ", std::min(128, a.V), ", got ", top);
@@ -222,12 +223,19 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_scores(const Tensor& lo
   a.top = (int)top;
   a.logprob = lp.data_ptr<float>(); a.entropy = ent.data_ptr<float>(); a.lse = lse.data_ptr<float>();
   a.top_ids = lptr(top_ids); a.top_lp = top_lp.data_ptr<float>();
+  a.stat = stat;
   CHECK_RC(vb_token_scores(&a, cur_stream()), "vb_token_scores");
   return {lp, ent, lse, top_ids, top_lp};
 }
+Tensor stat_of(const Tensor& logits) { return at::empty({logits.dim() == 2 ? logits.size(0) : 0, 4}, logits.options().dtype(at::kFloat)); }
 
-Tensor token_scores_bwd(const Tensor& logits, const Tensor& given, const Tensor& lse, const Tensor& ent, const Tensor& g_lp, const OptTensor& g_ent,
-                        double temperature, int64_t valid) {
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_scores(const Tensor& logits, const Tensor& given, int64_t top, double temperature, int64_t valid) {
+  return scores(logits, given, top, temperature, valid, nullptr);
+}
+
+// `kept`: the rows' stat as the forward pass left it, or nothing: the rows are gone over once more for it.
+Tensor scores_bwd(const Tensor& logits, const Tensor& given, const Tensor& lse, const Tensor& ent, const Tensor& kept, const Tensor& g_lp, const OptTensor& g_ent,
+                  double temperature, int64_t valid) {
   const Tensor x = by_rows(logits), ids = given.contiguous();
   VbScores a = scores_of(x, ids, temperature, valid, "token_scores_bwd");
   const int64_t T = x.size(0);
@@ -237,12 +245,22 @@ Tensor token_scores_bwd(const Tensor& logits, const Tensor& given, const Tensor&
   TORCH_CHECK(g_lp.device() == x.device() && g_lp.is_contiguous(), "token_scores_bwd: g_logprob must be contiguous and on the device of the logits");
   if (g_ent.has_value()) check_vec(*g_ent, at::kFloat, T, x, "token_scores_bwd: g_entropy");
   const c10::cuda::CUDAGuard guard(x.device());
+  Tensor stat = kept;
+  if (!stat.defined()) {
+    stat = stat_of(x);
+    scores(x, at::empty({T, 0}, ids.options()), 0, temperature, valid, stat.data_ptr<float>());
+  }
   Tensor dx = at::empty({T, x.size(1)}, x.options());
+  a.stat = stat.data_ptr<float>();
   a.lse = lse.data_ptr<float>(); a.entropy = ent.data_ptr<float>();
   CHECK_RC(vb_token_scores_bwd(&a, g_lp.data_ptr<float>(), g_ent.has_value() ? g_ent->data_ptr<float>() : nullptr, dx.data_ptr(), dx.stride(0),
                                (int)x.size(1), cur_stream()),
            "vb_token_scores_bwd");
   return dx;
+}
+Tensor token_scores_bwd(const Tensor& logits, const Tensor& given, const Tensor& lse, const Tensor& ent, const Tensor& g_lp, const OptTensor& g_ent,
+                        double temperature, int64_t valid) {
+  return scores_bwd(logits, given, lse, ent, Tensor(), g_lp, g_ent, temperature, valid);
 }
 
 // Log-probs and entropy with their gradient. In C++, because a function written in Python costs more on the host than the kernels of most
@@ -250,8 +268,9 @@ Tensor token_scores_bwd(const Tensor& logits, const Tensor& given, const Tensor&
 struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& ids, double temperature, int64_t valid) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [lp, ent, lse, top, top_lp] = token_scores(x, ids, 0, temperature, valid);
-    ctx->save_for_backward({x, ids, lse, ent});
+    const Tensor stat = stat_of(x);
+    auto [lp, ent, lse, top, top_lp] = scores(x, ids, 0, temperature, valid, x.is_cuda() ? stat.data_ptr<float>() : nullptr);
+    ctx->save_for_backward({x, ids, lse, ent, stat});
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["valid"] = valid;
     ctx->set_materialize_grads(false);
@@ -267,7 +286,7 @@ struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
         const Tensor g_lp = g[0].defined() ? g[0].contiguous() : at::zeros(saved[1].sizes(), saved[2].options());
         OptTensor g_ent;
         if (g[1].defined()) g_ent = g[1].contiguous();
-        dx = token_scores_bwd(saved[0].detach(), saved[1], saved[2], saved[3].detach(), g_lp, g_ent, ctx->saved_data["temperature"].toDouble(), ctx->saved_data["valid"].toInt());
+        dx = scores_bwd(saved[0].detach(), saved[1], saved[2], saved[3].detach(), saved[4], g_lp, g_ent, ctx->saved_data["temperature"].toDouble(), ctx->saved_data["valid"].toInt());
       }
       if (again)  // a graph of the gradient is asked for: an error where it is used
         dx = std::make_shared<torch::autograd::DelayedError>("token_logprobs can be differentiated once", 2)->apply({dx, saved[0]})[0];

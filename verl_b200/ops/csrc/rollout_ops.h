@@ -39,6 +39,7 @@ struct VbScores {
   int top;
   float* logprob; float* entropy; float* lse;
   long long* top_ids; float* top_lp;                   // [T, top]
+  float* stat;                                         // [T, 4], what the gradient wants of a row; forward: may be null
 };
 int vb_token_scores(const VbScores* a, cudaStream_t s);
 int vb_token_scores_bwd(const VbScores* a, const float* g_lp, const float* g_ent, void* dx, long long lddx, int columns, cudaStream_t s);

@@ -3,7 +3,7 @@
 // With y = x log2(e) / temperature and a reference M near the largest y, a row is read once for
 //   s = sum 2^(y - M),  w = sum 2^(y - M) (y - M):   lse = ln2 (M + log2 s),  H = ln2 (log2 s - w / s)
 // four instructions and one exponential a value. A thread keeps a reference of its own, the largest of its first values, which moves only when the sum
-// is 2^40 above it.
+// is 2^16 above it.
 //
 // The most likely tokens come with the same pass: every thread also keeps the largest value that it met, and the k-th largest of those of a
 // block is a bound that at least k values of the row reach. The largest value of each group of 32 (16 of 32 bits) stays in shared memory, and
@@ -15,7 +15,8 @@
 // while the block ranks the last one. Where rows are few, a row belongs to a cluster of up to 8 blocks, which exchange their sums, bounds and
 // candidates through distributed shared memory. The gradient needs no exchange:
 //   dL/dx_v = 1/T (sum_j g_j [v = id_j] - p_v (sum_j g_j + h (log p_v + H)))
-// is one more pass, 2^y (a + b y) a value, with the given tokens' columns written again behind it.
+// is one more pass, 2^y (a + b y) a value, with the given tokens' columns written again behind it. It takes log p from the reference and the
+// logarithm of the sum that the forward pass left, not from their sum, the log-sum-exp.
 //
 // Measured, rows of 152064: 2048 of bf16 without alternatives 104 us (6.0 TB/s, 0.93 of the copy rate), with 64 of them 135 us, with 128 161 us; the same in
 // fp32 219 us with 64 (0.88); their gradient, which reads once and writes once, 205 us in bf16 (0.94). One row of 151936: 12 us. What bounds the bf16
@@ -48,6 +49,8 @@ constexpr int TS_CHUNK = TS_PER * TS_THREADS;  // vectors of a stage: 16 KB
 constexpr int TS_CANDIDATES = 768;
 constexpr int TS_SLOTS = 24;       // groups of a thread that are told apart: stages of the row, modulo this
 constexpr float TS_LOG2E = 1.4426950408889634f, TS_LN2 = 0.6931471805599453f;
+// Exponents of 2 that a thread's sum, and so any of its terms, stays below: a term 2^d is off by the rounding of d, half a step of 2^-20 at 16.
+constexpr float TS_ABOVE = 16.f;
 constexpr float TS_FLOOR = -200.f;  // exponents below this are zeros: keeps 0 * inf out of the sums
 
 __device__ __forceinline__ float ts_exp2(float x) {
@@ -230,10 +233,23 @@ __device__ __forceinline__ unsigned long long block_max(unsigned long long v, un
   return v;
 }
 
-// Log-prob of value f of a row with reference m and ls = log2 s. A value near the type's lowest is its own log-prob: log2(e) times it is not finite.
-__device__ __forceinline__ float scaled_logprob(float f, float inv_temp, float m, float ls) {
-  const float d = fmaf(f, inv_temp * TS_LOG2E, -m);
-  return d == -INFINITY ? f * inv_temp : TS_LN2 * (d - ls);
+// What log2 p = y - m - log2 s takes of a row: the reference, and log2 s as a whole number and the logarithm of what is left, in [1, 2). Neither is
+// added to the reference, which would round off digits of p by the size of the logits (log-sum-exp 9e4: p off by 4e-3); and for the value that s
+// consists of, y - m and the whole number are close and their difference exact: 1 - p is off by at most 2e-6, in rows of 32000 by 4e-7.
+struct Norm {
+  float m, whole, part;
+  static __device__ __forceinline__ Norm of(const Stat& a) {
+    const int e = static_cast<int>(__float_as_uint(a.s) >> 23) - 127;  // s is a normal number: at least one term of it is
+    return {a.m, static_cast<float>(e), log2f(__uint_as_float((__float_as_uint(a.s) & 0x007fffffu) | 0x3f800000u))};
+  }
+  __device__ __forceinline__ float log2_s() const { return whole + part; }
+  __device__ __forceinline__ float log2_p(float f, float c) const { return fmaf(f, c, -m) - whole - part; }
+};
+
+// Log-prob of value f. A value near the type's lowest is its own log-prob: log2(e) times it is not finite.
+__device__ __forceinline__ float scaled_logprob(float f, float inv_temp, const Norm& n) {
+  const float y = n.log2_p(f, inv_temp * TS_LOG2E);
+  return y == -INFINITY ? f * inv_temp : TS_LN2 * y;
 }
 
 // Largest z = x / temperature and sum e^(z - m), sum e^(z - m) (z - m) of any row, by one block: for a row whose largest value is NaN or +inf
@@ -296,6 +312,7 @@ __device__ void scores_any(const VbScores& p, long long t, const T* x, Shared& s
   if (threadIdx.x == 0) {
     p.lse[t] = empty ? none : a.m + ls;
     p.entropy[t] = empty ? 0.f : ls - a.w / a.s;
+    if (p.stat != nullptr) reinterpret_cast<float4*>(p.stat)[t] = make_float4(NAN, 0.f, 0.f, 0.f);  // the gradient reads the row again
   }
   for (int j = threadIdx.x; j < p.K; j += TS_THREADS) {
     const long long id = p.ids[t * p.K + j];
@@ -304,8 +321,8 @@ __device__ void scores_any(const VbScores& p, long long t, const T* x, Shared& s
 }
 
 // The largest (value, lowest place) below the last one, `top` times over.
-template <typename T>
-__device__ void top_any(const VbScores& p, long long t, const T* x, Shared& sh, float m, float ls, bool scaled) {
+template <typename T, typename F>
+__device__ void top_any(const VbScores& p, long long t, const T* x, Shared& sh, const F& logprob) {
   unsigned long long last = ~0ull;
   for (int k = 0; k < p.top; ++k) {
     unsigned long long b = 0;
@@ -316,9 +333,8 @@ __device__ void top_any(const VbScores& p, long long t, const T* x, Shared& sh, 
     last = block_max(b, sh.wide);
     if (threadIdx.x == 0) {
       const uint32_t v = 0xffffffffu - static_cast<uint32_t>(last);
-      const float f = static_cast<float>(x[v]);
       p.top_ids[t * p.top + k] = v;
-      p.top_lp[t * p.top + k] = scaled ? scaled_logprob(f, p.inv_temp, m, ls) : m == -INFINITY ? -INFINITY : f * p.inv_temp - m - ls;
+      p.top_lp[t * p.top + k] = logprob(static_cast<float>(x[v]));
     }
   }
 }
@@ -507,12 +523,12 @@ token_scores_kernel(const VbScores p, int* status) {
         }
       }
       const float2 s = ts_of(s2), w = ts_of(w2);
-      if (s.x + s.y < 0x1p40f && w.x + w.y == w.x + w.y) {
+      if (s.x + s.y < 0x1p16f && w.x + w.y == w.x + w.y) {
         a.s = s.x + s.y;
         a.w = w.x + w.y;
       } else {  // too far above the reference, or 0 * -inf got into the sums: again, with a floor under the exponents
         const float up = fmaxf(largest() * c, a.s > 0.f ? a.m + log2f(a.s) : -INFINITY);
-        if (up > a.m + 20.f) a.move(up);
+        if (up > a.m + 0.5f * TS_ABOVE) a.move(up);
 #pragma unroll 1
         for (int u = 0; u < TS_PER; ++u) {
           if (left <= u * TS_THREADS) break;
@@ -545,7 +561,7 @@ token_scores_kernel(const VbScores p, int* status) {
     const bool any = has_loose || static_cast<int>(threadIdx.x) < n;
     if (has_loose) {
       most = fmaxf(most, loose);
-      if (loose * c > a.m + 60.f) a.move(loose * c);
+      if (loose * c > a.m + TS_ABOVE) a.move(loose * c);
       a.add(loose, c);
     }
     a = block_stat(a, sh.red);
@@ -643,30 +659,31 @@ token_scores_kernel(const VbScores p, int* status) {
       if (p.top > 0) {
         const Stat b = any_stat(x, p.V, p.inv_temp, sh.red);
         const float bls = logf(b.s);
+        const auto logprob = [&](float f) { return b.m == -INFINITY ? -INFINITY : f * p.inv_temp - b.m - bls; };
         const bool wild = !(b.s >= 0.f) || b.m == INFINITY;  // NaN or +inf in it
-        if (wild || !top_ties(p, t, x, sh, [&](float f) { return b.m == -INFINITY ? -INFINITY : f * p.inv_temp - b.m - bls; }))
-          top_any(p, t, x, sh, b.m, bls, false);
+        if (wild || !top_ties(p, t, x, sh, logprob)) top_any(p, t, x, sh, logprob);
       }
       ts_sync();
       continue;
     }
-    const float ls = log2f(a.s);
+    const Norm norm = Norm::of(a);
+    const auto logprob = [&](float f) { return scaled_logprob(f, p.inv_temp, norm); };
     if (threadIdx.x == 0) {
-      p.lse[t] = TS_LN2 * (a.m + ls);
-      p.entropy[t] = TS_LN2 * (ls - a.w / a.s);
+      p.lse[t] = TS_LN2 * (a.m + norm.log2_s());
+      p.entropy[t] = TS_LN2 * (norm.log2_s() - a.w / a.s);
+      if (!TOP && p.stat != nullptr) reinterpret_cast<float4*>(p.stat)[t] = make_float4(norm.m, norm.whole, norm.part, 0.f);
     }
     for (int j = threadIdx.x; j < p.K; j += TS_THREADS) {
       const long long at = static_cast<long long>(t) * p.K + j, id = j < TS_THREADS ? id0 : p.ids[at];
       const bool there = id >= 0 && id < p.V;
-      p.logprob[at] = there ? scaled_logprob(static_cast<float>(j < TS_THREADS ? given : x[id]), p.inv_temp, a.m, ls) : 0.f;
+      p.logprob[at] = there ? logprob(static_cast<float>(j < TS_THREADS ? given : x[id])) : 0.f;
     }
     if (p.top > 0) {
       const int found = sh.found;
-      const auto logprob = [&](float f) { return scaled_logprob(f, p.inv_temp, a.m, ls); };
       if (found >= p.top && found <= TS_CANDIDATES)
         write_ranked(p, t, sh, found, logprob);
       else if (!top_ties(p, t, x, sh, logprob))
-        top_any(p, t, x, sh, a.m, ls, true);
+        top_any(p, t, x, sh, logprob);
     }
     ts_sync();  // the next row starts with an empty list
   }
@@ -689,19 +706,22 @@ token_scores_bwd_kernel(const VbScores p, const float* __restrict__ g_lp, const 
   for (int j = threadIdx.x; j < p.K; j += TS_THREADS)
     if (ids[j] >= 0 && ids[j] < p.V) gs.s += gl[j];
   const float g = block_stat(gs, sh.red).s;
-  // log2 p = x c - m - ls
-  float m = lse * TS_LOG2E, ls = 0.f, c = p.inv_temp * TS_LOG2E;
-  bool apart = false;
-  if (fabsf(lse) > 1e5f && lse > -INFINITY) {  // too large to hold log s as well: both again, and the differences before they are scaled
+  // log2 p from the row's reference and sum as the forward pass had them: the log-sum-exp alone has lost log s in its own rounding
+  const float4 kept = reinterpret_cast<const float4*>(p.stat)[t];
+  const Norm norm{kept.x, kept.y, kept.z};
+  const float c = p.inv_temp * TS_LOG2E;
+  float m = 0.f, ls = 0.f;
+  const bool apart = norm.m != norm.m;  // a row that has no such reference: both again, and the differences before they are scaled
+  if (apart) {
     const Stat b = any_stat(x, p.V, p.inv_temp, sh.red);
     m = b.m;
     ls = logf(b.s) * TS_LOG2E;
-    apart = true;
   }
   const bool empty = lse == -INFINITY;
   const float a0 = -p.inv_temp * (g + h * H), a1 = -p.inv_temp * h * TS_LN2;
+  const auto log2_p = [&](float f) { return ts_max_nan(apart ? (f * p.inv_temp - m) * TS_LOG2E - ls : norm.log2_p(f, c), TS_FLOOR); };
   const auto slope = [&](float f) {
-    const float y = ts_max_nan(apart ? (f * p.inv_temp - m) * TS_LOG2E - ls : fmaf(f, c, -m), TS_FLOOR);
+    const float y = log2_p(f);
     return empty ? 0.f : ts_exp2(y) * fmaf(a1, y, a0);
   };
   // vectors where the row and its gradient lie alike
@@ -744,7 +764,11 @@ token_scores_bwd_kernel(const VbScores p, const float* __restrict__ g_lp, const 
         earlier |= i < j;
         sum += gl[i];
       }
-    if (!earlier && !empty) d[id] = static_cast<T>(fmaf(p.inv_temp, sum, slope(static_cast<float>(x[id]))));
+    if (earlier || empty) continue;
+    const float f = static_cast<float>(x[id]), y = log2_p(f);
+    // sum - p (g + h (log p + H)), and where p is above a half as (sum - g) + g (1 - p) - p h (log p + H): a token that is all but certain has a small
+    // difference, not two large terms
+    d[id] = static_cast<T>(y < -1.f ? fmaf(p.inv_temp, sum, slope(f)) : p.inv_temp * (sum - g - g * expm1f(TS_LN2 * y) - ts_exp2(y) * h * fmaf(TS_LN2, y, H)));
   }
 }
 

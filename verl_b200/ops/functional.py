@@ -977,7 +977,8 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, temperature: float =
 def token_scores_bwd(logits: torch.Tensor, ids: torch.Tensor, lse: torch.Tensor, entropy: torch.Tensor, g_logprob: torch.Tensor,
                      g_entropy: Optional[torch.Tensor], temperature: float = 1.0, valid_vocab: int = 0) -> torch.Tensor:
     """Gradient of the logits, in their type, from those of ``logprob`` and ``entropy`` (None: none) of :func:`token_scores`. A token that is given
-    several times gathers all its gradients; ids outside the vocabulary and columns behind ``valid_vocab`` have none."""
+    several times gathers all its gradients; ids outside the vocabulary and columns behind ``valid_vocab`` have none. A log-sum-exp in 32 bits does
+    not hold what the probabilities need, so the rows are read once more for it; ``token_logprobs`` keeps it from its forward pass."""
     if logits.is_cuda:
         return _ops().token_scores_bwd(logits, ids, lse.contiguous(), entropy.contiguous(), g_logprob.float().contiguous(),
                                        g_entropy.float().contiguous() if g_entropy is not None else None, float(temperature), int(valid_vocab))
