@@ -19,7 +19,7 @@
 // The least values m of the groups go through the matrix unit apart from the codes:
 //   S gains m (sum of q over the thread's channels), one more k step of an instruction that has m twice against that sum's two fp16 halves;
 //   O gains sum_t p_t m_t, the same for all channels of a thread: one accumulator more, added at the end.
-// 1.1 instructions an element. Queries are scaled by a power of two per head, into fp16's range; weights are e^(s - reference) <= 64 in fp16.
+// 1.1 instructions an element. Queries are scaled by a power of two per head, into fp16's range; weights are 2^(s - reference) <= 2^14 in fp16.
 // These roundings to 11 bits (6e-4 of the output's norm in all) are below those of a bf16 output (1.7e-3). For fp16 (2.1e-4 by its own rounding) there are
 // none: codes apart from each other, scales in two parts of at most seven bits, under which codes are exact, weights in two halves; values count from
 // code 8, because the sum of codes and that of least values would each be hundreds of times their difference over a long context, and matrix
@@ -48,6 +48,13 @@ constexpr int KD_TILES = KD_PIECE / 16;
 // with spills, where two take 59)
 __host__ __device__ constexpr int kd_ctas(int hd, int nt) { return hd == 128 && nt == 2 ? 2 : 3; }
 constexpr int KD_MIN_PIECES = 1;                 // shortest run of a warp
+// The reference of a head's weights lies 2^8 below the largest score of the piece that set it: weights of up to 2^14 are as exact in fp16 as those of
+// 1, and smaller ones keep 11 bits down to 2^-14. It is set again by a piece with a score 2^14 above it, and by one that has none above 2^-4: behind a
+// token that outweighs all others, as the first one of a sequence often does, the others would be left with no bits, and where that token's
+// value is small they are what the output consists of (a token of weight 0.9997 before 65536 others: bf16 and fp16 outputs off by 2e-2 with a reference
+// that only rises). The sums may then grow to 2^60, which fp32 holds. Weights below 2^-32 of the largest one of their own piece are lost.
+constexpr float KD_BELOW = 8.f, KD_HIGH = 14.f, KD_LOW = -4.f;
+constexpr int KD_ROOM = 60;
 
 __device__ int g_kv4_status[4];
 
@@ -430,16 +437,26 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
             for (int i = 1; i < KD_TILES; ++i) top[h] = fmaxf(top[h], fmaxf(st[t][i][h], st[t][i][2 + h]));
             top[h] *= sc[t][h];  // the factor is not negative: its sign is the query's
           }
-          // the reference stays until a score is 2^6 above it: weights up to 64 are as exact in fp16 as those up to 1
-          if (__any_sync(0xffffffffu, top[0] > m[t][0] + 6.f || top[1] > m[t][1] + 6.f)) {
+          const uint32_t column = 0x11111111u << c;  // the lanes of this thread's heads
+          const uint32_t near0 = __ballot_sync(0xffffffffu, top[0] >= m[t][0] + KD_LOW), near1 = __ballot_sync(0xffffffffu, top[1] >= m[t][1] + KD_LOW);
+          const bool high = top[0] > m[t][0] + KD_HIGH || top[1] > m[t][1] + KD_HIGH, low = (near0 & column) == 0u || (near1 & column) == 0u;
+          if (__any_sync(0xffffffffu, high || low)) {
             float alpha[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              float mx = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 4));
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-              mx = fmaxf(fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16)), m[t][h]);
-              alpha[h] = fast_exp2(m[t][h] - (mx == -INFINITY ? 0.f : mx));
-              m[t][h] = mx;
+              float mx = top[h], big = l[t][h], to = m[t][h];
+#pragma unroll
+              for (int step = 4; step < 32; step *= 2) {
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, step));
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, step));
+              }
+              const int room = KD_ROOM + 127 - static_cast<int>(__float_as_uint(big) >> 23);
+              if (mx > to + KD_HIGH)
+                to = mx - KD_BELOW;
+              else if (mx < to + KD_LOW && mx > -INFINITY && room > 0)
+                to = fmaxf(mx - KD_BELOW, to - static_cast<float>(room));
+              alpha[h] = to == m[t][h] ? 1.f : fast_exp2(m[t][h] - to);
+              m[t][h] = to;
               l[t][h] *= alpha[h];
               z[t][h] *= alpha[h];
               z[t][2 + h] *= alpha[h];
@@ -453,12 +470,14 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float mu = m[t][h] == -INFINITY ? 0.f : m[t][h];
+            float sum = 0.f;  // of the piece first: beside a sum that is far larger its parts would be lost
 #pragma unroll
             for (int i = 0; i < KD_TILES; ++i) {
               st[t][i][h] = fast_exp2(fmaf(st[t][i][h], sc[t][h], -mu));
               st[t][i][2 + h] = fast_exp2(fmaf(st[t][i][2 + h], sc[t][h], -mu));
-              l[t][h] += st[t][i][h] + st[t][i][2 + h];
+              sum += st[t][i][h] + st[t][i][2 + h];
             }
+            l[t][h] += sum;
           }
 #pragma unroll
           for (int i = 0; i < KD_TILES; ++i) {
