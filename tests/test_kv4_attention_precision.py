@@ -93,3 +93,23 @@ def test_a_token_that_outweighs_all_others(nh, nkv, hd, B, where, dtype):
     # the same token twice, the second time with a value: now it is all of the output
     F.kv4_append_(k, torch.ones_like(k), torch.full((1,), (where + 5000) % n, dtype=torch.int64, device="cuda"), pages)
     assert off(q[0], up)[0]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("nh,nkv,hd,n", [(8, 8, 64, 98304), (32, 8, 128, 32768), (20, 2, 128, 98304), (12, 1, 64, 131072), (8, 8, 128, 131071)])
+def test_contexts_that_one_warp_works_on_alone(nh, nkv, hd, n, dtype):
+    """As many (sequence, head) pairs as there are warps: thousands of tokens are added up in one place, and as their values are of either sign what is left is
+    small beside the codes that it comes from. The sequences share their pages, weights are nearly equal."""
+    bs = 64
+    B = -(-1776 // nkv)
+    gen = torch.Generator(device="cuda").manual_seed(hd + n)
+    pages = pool_of(-(-n // bs), nkv, hd, bs, gen)
+    q = (torch.randn(nh, hd, device="cuda", generator=gen) * 0.05).to(dtype)
+    table = torch.randperm(len(pages), device="cuda", generator=gen).to(torch.int32)
+    out = F.paged_decode_attention_kv4(q.expand(B, -1, -1).contiguous(), pages, table.expand(B, -1).contiguous(), torch.full((B,), n, dtype=torch.int32, device="cuda"))
+    k, v = rows_of(pages[table.long()], hd, bs)
+    w = torch.softmax(torch.einsum("hgd,htd->hgt", q.double().view(nkv, -1, hd), k[:, :n]) / math.sqrt(hd), -1)
+    want = torch.einsum("hgt,htd->hgd", w, v[:, :n]).reshape(-1, hd)
+    off = max(beside_rounding(o, want) for o in out[:: B // 12])
+    print(f"beside rounding {off:.2e}")
+    assert off <= BOUND[dtype]

@@ -20,14 +20,16 @@
 //   S gains m (sum of q over the thread's channels), one more k step of an instruction that has m twice against that sum's two fp16 halves;
 //   O gains sum_t p_t m_t, the same for all channels of a thread: one accumulator more, added at the end.
 // 1.1 instructions an element. Queries are scaled by a power of two per head, into fp16's range; weights are 2^(s - reference) <= 2^14 in fp16.
-// These roundings to 11 bits (6e-4 of the output's norm in all) are below those of a bf16 output (1.7e-3). For fp16 (2.1e-4 by its own rounding) there are
+// These roundings to 11 bits (6e-4 of the output's norm in all) are below those of a bf16 output (1.7e-3); what one channel adds to a score is off by up
+// to 2^-11 of itself, and the token's weight with it (a score of 14 from one channel: 7e-3). For fp16 (2.1e-4 by its own rounding) there are
 // none: codes apart from each other, scales in two parts of at most seven bits, under which codes are exact, weights in two halves; values count from
 // code 8, because the sum of codes and that of least values would each be hundreds of times their difference over a long context, and matrix
 // instructions add up by cutting off. That takes two and three matrix instructions for one, and 1.75 times the time where instructions count.
 //
-// 320 sequences of 28 heads over 4 KV heads of 128 channels, 2560 tokens on average: 115 to 125 us for 525 MB with the join (0.65 to 0.7 of the copy
-// rate; fp16 200). Copies alone would take 98 us with the join, the instructions 106: both are near their limits, and warps that wait for one do not
-// always cover the other. One sequence of 131072 tokens, 8 KV heads: 47 us for 168 MB (fp16 72), 8 of them the join's. Four of 160 tokens: 12 us, two launches.
+// 320 sequences of 28 heads over 4 KV heads of 128 channels, 2560 tokens on average: 130 us for 525 MB with the join (0.62 of the copy rate; fp16 200),
+// 5 of them for the reference that follows the scores and the sums that are folded. Neither HBM (57 %) nor the schedulers (0.53 instructions a cycle) are
+// full: three warps to a scheduler, each of which goes through keys, softmax and values one behind the other, do not cover what they wait for. One
+// sequence of 131072 tokens, 8 KV heads: 49 us for 168 MB (fp16 72), 8 of them the join's. Four of 160 tokens: 12 us, two launches.
 #include <math.h>
 
 #include <type_traits>
@@ -55,6 +57,7 @@ constexpr int KD_MIN_PIECES = 1;                 // shortest run of a warp
 // that only rises). The sums may then grow to 2^60, which fp32 holds. Weights below 2^-32 of the largest one of their own piece are lost.
 constexpr float KD_BELOW = 8.f, KD_HIGH = 14.f, KD_LOW = -4.f;
 constexpr int KD_ROOM = 60;
+constexpr int KD_FOLD = 32;                      // pieces after which a warp's sums of products go to shared memory
 
 __device__ int g_kv4_status[4];
 
@@ -177,7 +180,9 @@ struct KDSmem {
   static constexpr int PARAMS = KD_PIECE * (HD / KV4_GROUP) * 4;
   static constexpr int OFF_PK = 2 * CODES;
   static constexpr int STAGE = 2 * CODES + 2 * PARAMS;        // of a warp, a multiple of 128 bytes
-  static constexpr int OFF_BAR = KD_WARPS * STAGE;
+  static constexpr int SUMS = NT * (HD / 16 + 2) * 512;       // of a warp: four numbers a thread and sum, and the references that they are under
+  static constexpr int OFF_SUMS = KD_WARPS * STAGE;
+  static constexpr int OFF_BAR = OFF_SUMS + KD_WARPS * SUMS;
   static constexpr int TOTAL = OFF_BAR + KD_WARPS * 2 * 8;
 };
 
@@ -243,6 +248,7 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
   extern __shared__ __align__(16) uint8_t smem[];  // 16 bytes are what bulk copies ask for
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.nh / p.nkv, bs = p.block_size;
   uint8_t* stage = smem + warp * L::STAGE;
+  float4* sums = reinterpret_cast<float4*>(smem + L::OFF_SUMS + warp * L::SUMS) + lane;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR) + warp * 2;  // keys are there, values are there
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int run = blockIdx.x * KD_WARPS + warp, total = kd_total(p), per = kd_per(total, gridDim.x * KD_WARPS);
@@ -366,8 +372,41 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
 #pragma unroll
       for (int i = 0; i < HD / 16; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
     }
+    // Matrix instructions add up by cutting off, always towards zero: over thousands of tokens that is far more than what is left where values of either
+    // sign cancel (131072 tokens a warp: outputs off by 1.6e-2 of their norm in bf16 and 2.8e-3 in fp16 beside their own rounding). So sums of KD_FOLD
+    // pieces are added up here, rounded to nearest: 2.5e-4 and 3e-6; with 8 pieces 2.1e-4 and 4e-6, in the same time. Every thread
+    // has a place of its own in shared memory. `keep`: what is there is taken along; `back`: it comes back into the registers.
+    const auto fold = [&](bool keep, bool back) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float4* at = sums + t * (HD / 16 + 2) * 32;
+        float f[2] = {0.f, 0.f};
+        if (keep) {
+          const float4 old = at[(HD / 16 + 1) * 32];
+          f[0] = old.x == m[t][0] ? 1.f : fast_exp2(old.x - m[t][0]);
+          f[1] = old.y == m[t][1] ? 1.f : fast_exp2(old.y - m[t][1]);
+        }
+#pragma unroll
+        for (int i = 0; i <= HD / 16; ++i) {
+          float (&a)[4] = i < HD / 16 ? o[t][i < HD / 16 ? i : 0] : z[t];
+          if (keep) {
+            const float4 old = at[i * 32];
+            a[0] = fmaf(old.x, f[0], a[0]);
+            a[1] = fmaf(old.y, f[1], a[1]);
+            a[2] = fmaf(old.z, f[0], a[2]);
+            a[3] = fmaf(old.w, f[1], a[3]);
+          }
+          if (!back) {
+            at[i * 32] = make_float4(a[0], a[1], a[2], a[3]);
+            a[0] = a[1] = a[2] = a[3] = 0.f;
+          }
+        }
+        if (!back) at[(HD / 16 + 1) * 32] = make_float4(m[t][0], m[t][1], 0.f, 0.f);
+      }
+    };
     for (; u < seg_end; ++u, ++round) {
-      const int next = u + 1;
+      const int next = u + 1, done = u - seg;
+      if (done > 0 && done % KD_FOLD == 0) fold(done > KD_FOLD, false);
       if (looked == 2) {
         looked = 0;
         if (next < u1) look_all(next);
@@ -557,6 +596,7 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
       ++looked;
     }
 
+    if (seg_end - seg > KD_FOLD) fold(true, true);
     // ---- end of a segment. O^T[channel r VPR + 2 i, head] = 16 o + z, and the channel behind it o' - o + z
     const bool whole = seg == g.base && seg_end == g.end;
     float* part = p.part + (2LL * run + (seg == u0 ? 0 : 1)) * G * (HD + 4);
