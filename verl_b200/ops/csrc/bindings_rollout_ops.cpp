@@ -88,7 +88,7 @@ std::tuple<Tensor, Tensor, Tensor> build_slot_map(const Tensor& table, const Ten
   check_vec(ends, at::kInt, B, table, "build_slot_map: ends");
   TORCH_CHECK(bs > 0 && bs <= (1 << 20), "build_slot_map: block_size");
   TORCH_CHECK_VALUE(total >= 0, "build_slot_map: total must not be negative, got ", total);
-  TORCH_CHECK(total <= (1 << 22) && B <= 8192, "build_slot_map: at most 2^22 tokens of at most 8192 sequences, got ", total, " of ", B);
+  TORCH_CHECK(total <= (1LL << 31) - (1 << 13) && B <= (1 << 30), "build_slot_map: fewer than 2^31 - 2^13 tokens of at most 2^30 sequences, got ", total, " of ", B);
   const c10::cuda::CUDAGuard guard(table.device());
   Tensor cu = at::empty({B + 1}, table.options()), positions = at::empty({total}, table.options()),
          slots = at::empty({total}, table.options().dtype(at::kLong));

@@ -3,8 +3,8 @@
 //
 // need_i = ceil(length_i / block), new_i = max(need_i - have_i, 0), and sequence i takes pool[sum of new_j over j < i ...]; token t of a packed
 // batch belongs to the sequence i with cu_i <= t < cu_{i+1} and lies at position starts_i + t - cu_i. Both are exclusive sums over the batch,
-// which every block of a launch takes for itself (a batch is at most some thousand sequences, read from L2): one launch, no block waits
-// for another. Nothing out of range is read or written whatever the tensors hold: a token whose row, position or page is none gets slot -1.
+// which every block of a launch takes for itself (a batch is mostly some hundred sequences, read from L2): one launch, no block waits
+// for another. Slots of more than 8192 sequences take a launch more, for the sums. Nothing out of range is read or written whatever the tensors hold: a token whose row, position or page is none gets slot -1.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -14,13 +14,25 @@ namespace vb {
 
 constexpr int PM_THREADS = 1024;
 
+// Sums of counts, and sums of which no more than `most` is wanted or held: two of those fit 32 bits without a sign.
+struct Sum {
+  __device__ __forceinline__ int operator()(int a, int b) const { return a + b; }
+};
+struct SumUpTo {
+  int most;
+  __device__ __forceinline__ int operator()(int a, int b) const {
+    return static_cast<int>(min(static_cast<unsigned>(a) + static_cast<unsigned>(b), static_cast<unsigned>(most)));
+  }
+};
+
 // inclusive sum over the block; `red` holds 32 ints. Every thread also gets the block's total.
-__device__ __forceinline__ int pm_scan(int v, int* red, int& total) {
+template <typename Add = Sum>
+__device__ __forceinline__ int pm_scan(int v, int* red, int& total, const Add& add = Add()) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int u = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += u;
+    if (lane >= o) v = add(v, u);
   }
   __syncthreads();
   if (lane == 31) red[warp] = v;
@@ -29,11 +41,11 @@ __device__ __forceinline__ int pm_scan(int v, int* red, int& total) {
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int u = __shfl_up_sync(0xffffffffu, w, o);
-    if (lane >= o) w += u;
+    if (lane >= o) w = add(w, u);
   }
   total = __shfl_sync(0xffffffffu, w, 31);
   const int before = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
-  return v + (warp > 0 ? before : 0);
+  return add(v, warp > 0 ? before : 0);
 }
 
 // One block over all slots. The plan counts the 64-token pieces of the contexts in front of every sequence: what the attention over the
@@ -105,29 +117,46 @@ extend_block_tables_kernel(int* __restrict__ table, long long ldt, int S, int wi
 
 constexpr int SM_THREADS = 256;
 constexpr int SM_TOKENS = 4;  // consecutive tokens of a thread: 16 and 32 bytes of output
+constexpr int SM_OWN_SUMS = 8192;  // sequences whose sums fit the shared memory that every launch has
 constexpr int SM_TURNS = 4;   // times that a block goes on: its sums over the batch are made once for 4096 tokens
 // 512 sequences of 2.3 million tokens: 15 us for 28 MB (1.9 TB/s; 4.5 us at the copy rate) in 568 blocks. A block's time is a chain: two sums over the
 // batch, the search for its sequences, row and start, page, stores. Look-ups token by token, of which a warp nearly always needs some, took 17 us.
 
-__global__ void __launch_bounds__(SM_THREADS)
-build_slot_map_kernel(const int* __restrict__ table, long long ldt, int S, int width, const int* __restrict__ rows, const int* __restrict__ starts,
-                      const int* __restrict__ ends, int B, int bs, int shift, int total, int* __restrict__ cu_out, int* __restrict__ positions,
-                      long long* __restrict__ slots) {
-  extern __shared__ int cu[];  // [B + 1]
-  __shared__ int red[32];
+// cu[i + 1]: the tokens up to and with sequence i, no more than `total` of them.
+__device__ __forceinline__ void sum_lengths(int* cu, const int* __restrict__ starts, const int* __restrict__ ends, int B, int total, int* red) {
+  const SumUpTo add{total};
   int carry = 0;
   if (threadIdx.x == 0) cu[0] = 0;
   for (int base = 0; base < B; base += blockDim.x) {
-    const int i = base + threadIdx.x;
-    const int n = i < B ? min(max(ends[i] - max(starts[i], 0), 0), total) : 0;
-    int sum;  // at most 256 x 2^22, the most tokens that the launcher takes
-    const int inc = pm_scan(n, red, sum);
-    if (i < B) cu[i + 1] = min(carry + inc, total);
-    carry = min(carry + sum, total);
+    const int i = base + threadIdx.x, from = i < B ? max(starts[i], 0) : 0, to = i < B ? ends[i] : 0;
+    int sum;
+    const int inc = pm_scan(to > from ? min(to - from, total) : 0, red, sum, add);
+    if (i < B) cu[i + 1] = add(carry, inc);
+    carry = add(carry, sum);
   }
-  __syncthreads();
-  if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i <= B; i += blockDim.x) cu_out[i] = cu[i];
+}
+
+// For more sequences than a block's shared memory holds the sums of: they are taken once, by one block, and then read from memory.
+__global__ void __launch_bounds__(PM_THREADS)
+sum_lengths_kernel(const int* __restrict__ starts, const int* __restrict__ ends, int B, int total, int* __restrict__ cu) {
+  __shared__ int red[32];
+  sum_lengths(cu, starts, ends, B, total, red);
+}
+
+template <bool SUMMED>  // cu_out holds the sums already
+__global__ void __launch_bounds__(SM_THREADS)
+build_slot_map_kernel(const int* __restrict__ table, long long ldt, int S, int width, const int* __restrict__ rows, const int* __restrict__ starts,
+                      const int* __restrict__ ends, int B, int bs, int shift, int total, int* cu_out, int* __restrict__ positions,
+                      long long* __restrict__ slots) {
+  extern __shared__ int own_cu[];  // [B + 1]
+  __shared__ int red[32];
+  const int* cu = SUMMED ? cu_out : own_cu;
+  if constexpr (!SUMMED) {
+    sum_lengths(own_cu, starts, ends, B, total, red);
+    __syncthreads();
+    if (blockIdx.x == 0)
+      for (int i = threadIdx.x; i <= B; i += blockDim.x) cu_out[i] = own_cu[i];
+  }
   const int end = cu[B];
   // Four tokens of one sequence are on one page or two: those of all turns are looked up together. A warp's tokens always meet the end of a page.
   int t0[SM_TURNS], p0[SM_TURNS], lo[SM_TURNS], row[SM_TURNS], blk[SM_TURNS], next[SM_TURNS];
@@ -219,8 +248,15 @@ extern "C" int vb_extend_block_tables(int* table, long long ldt, int S, int widt
 extern "C" int vb_build_slot_map(const int* table, long long ldt, int S, int width, const int* rows, const int* starts, const int* ends, int B,
                                  int block_size, int total, int* cu, int* positions, long long* slots, cudaStream_t s) {
   const int per = SM_THREADS * SM_TOKENS * SM_TURNS, shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(static_cast<unsigned>(block_size)) : -1;
+  if (total > 0x7fffffff - per) return -2;  // places of the last block are counted in 31 bits
   const int blocks = total > 0 ? (total + per - 1) / per : 1;
-  build_slot_map_kernel<<<blocks, SM_THREADS, (B + 1) * sizeof(int), s>>>(table, ldt, S, width, rows, starts, ends, B, block_size, shift, total, cu, positions,
-                                                                         slots);
+  if (B <= SM_OWN_SUMS) {
+    build_slot_map_kernel<false><<<blocks, SM_THREADS, (B + 1) * sizeof(int), s>>>(table, ldt, S, width, rows, starts, ends, B, block_size, shift, total, cu,
+                                                                                  positions, slots);
+  } else {
+    verl_count_launches(1);
+    sum_lengths_kernel<<<1, PM_THREADS, 0, s>>>(starts, ends, B, total, cu);
+    build_slot_map_kernel<true><<<blocks, SM_THREADS, 0, s>>>(table, ldt, S, width, rows, starts, ends, B, block_size, shift, total, cu, positions, slots);
+  }
   return static_cast<int>(cudaGetLastError());
 }
