@@ -296,6 +296,7 @@ struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
 };
 
 std::tuple<Tensor, Tensor> token_logprobs(const Tensor& logits, const Tensor& given, double temperature, int64_t valid) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!logits._fw_grad(0).defined(), "token_logprobs: logits with a tangent (forward-mode derivatives)");
   const Tensor x = by_rows(logits), ids = given.contiguous();
   if (at::GradMode::is_enabled() && x.requires_grad()) {
     auto out = TokenLogprobs::apply(x, ids, temperature, valid);
