@@ -125,7 +125,13 @@ def student_topk_log_probs(hidden: torch.Tensor, weight: torch.Tensor, ids: torc
 def compute_forward_kl_topk(student_logits: Optional[torch.Tensor], teacher_topk_log_probs: torch.Tensor, teacher_topk_ids: torch.Tensor,
                             config: DistillationLossConfig, student_topk_logp: Optional[torch.Tensor] = None) -> dict:
     """Per-token forward KL on the teacher's support. Give either full ``student_logits`` [..., V] or the already
-    gathered ``student_topk_logp`` [..., k]. Returns ``distillation_losses``, ``student_mass``, ``teacher_mass``."""
+    gathered ``student_topk_logp`` [..., k]. Returns ``distillation_losses``, ``student_mass``, ``teacher_mass``.
+
+    Ids that ``student_logits`` has no column for (a teacher with a larger vocabulary, a filler of -1) count in none of the three."""
+    there = None
+    if student_topk_logp is None:
+        there = (teacher_topk_ids >= 0) & (teacher_topk_ids < student_logits.size(-1))
+        teacher_topk_ids = torch.where(there, teacher_topk_ids, 0)
     if student_topk_logp is None and student_logits.is_cuda and student_logits.dtype in (torch.float32, torch.bfloat16, torch.float16):
         from ...utils.kernel import token_logprobs
 
@@ -137,8 +143,10 @@ def compute_forward_kl_topk(student_logits: Optional[torch.Tensor], teacher_topk
     if config.log_prob_min_clamp is not None:
         lq_s = lq_s.clamp_min(config.log_prob_min_clamp)
         lp_t = lp_t.clamp_min(config.log_prob_min_clamp)
-    loss = kl_divergence(lq_s, lp_t)
-    t_mass, s_mass = lp_t.exp().sum(-1), lq_s.exp().sum(-1)
+    counted = lambda x: x.sum(-1) if there is None else torch.where(there, x, 0.0).sum(-1)
+    t, s = lp_t.exp(), lq_s.exp()
+    loss = counted(t * (lp_t - lq_s))
+    t_mass, s_mass = counted(t), counted(s)
     if config.use_tail_term:
         eps = 1e-6
         tt, ts = (1 - t_mass).clamp(eps, 1.0), (1 - s_mass).clamp(eps, 1.0)
