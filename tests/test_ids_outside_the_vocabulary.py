@@ -3,6 +3,8 @@
 import pytest
 import torch
 
+from verl_b200.models.generic import _logprob_entropy_from_logits
+from verl_b200.ops import audit
 from verl_b200.trainer.distillation.losses import DistillationLossConfig, compute_forward_kl_topk
 
 
@@ -48,3 +50,17 @@ def test_a_teacher_s_ids_that_the_student_does_not_have_do_not_count(dev, config
         assert (got.double().cpu().view(-1) - torch.stack(ref).detach()).abs().max() < 16 * 2.0**-20
     assert (grad.double().cpu() - want).abs().max() < 16 * 2.0**-20 and (grad[1, 0] == 0).all()
     assert out["student_mass"][1, 0] == 0 and out["teacher_mass"][1, 0] == 0
+
+
+def test_labels_outside_the_vocabulary_have_no_log_prob(dev):
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(4, 30, generator=g).to(dev).requires_grad_(True)
+    labels = torch.tensor([3, -100, 30, 29], device=dev)
+    lp, ent = _logprob_entropy_from_logits(x, labels)
+    (grad,) = torch.autograd.grad(lp.sum(), x)
+    ref = torch.log_softmax(x.detach().double().cpu(), -1)
+    assert lp[1] == 0 and lp[2] == 0 and (grad[1:3] == 0).all() and (grad[[0, 3]] != 0).all()
+    assert abs(float(lp[0]) - float(ref[0, 3])) < 2.0**-18 and abs(float(lp[3]) - float(ref[3, 29])) < 2.0**-18
+    assert (ent.double().cpu() + (ref.exp() * ref).sum(-1)).abs().max() < 2.0**-18
+    with audit.scope(), pytest.raises(audit.AuditError, match="labels"):
+        _logprob_entropy_from_logits(x, labels)

@@ -22,6 +22,7 @@ from typing import Iterator, Optional
 
 import torch
 
+from ..ops import audit
 from .config import ModelConfig
 from .weights import ALIGN, ParamSpec
 
@@ -180,12 +181,16 @@ class ModuleFlatParams:
 
 
 def _logprob_entropy_from_logits(logits: torch.Tensor, labels: torch.Tensor):
+    """(log-prob of ``labels``, entropy), fp32, of rows of logits. A label outside the vocabulary (padding) has log-prob 0 and no gradient."""
+    audit.check_index("log-probs of a library module", "labels", labels, logits.shape[-1])
     if logits.is_cuda:
         from ..utils.kernel import token_logprobs
 
         return token_logprobs(logits.float(), labels.long())
     logp = torch.log_softmax(logits.float(), -1)
-    lp = logp.gather(-1, labels.long()[:, None]).squeeze(-1)
+    at = labels.long()
+    there = (at >= 0) & (at < logp.shape[-1])
+    lp = torch.where(there, logp.gather(-1, torch.where(there, at, 0)[:, None]).squeeze(-1), 0.0)
     ent = -(logp.exp() * logp).sum(-1)
     return lp, ent
 
