@@ -183,16 +183,9 @@ class ModuleFlatParams:
 def _logprob_entropy_from_logits(logits: torch.Tensor, labels: torch.Tensor):
     """(log-prob of ``labels``, entropy), fp32, of rows of logits. A label outside the vocabulary (padding) has log-prob 0 and no gradient."""
     audit.check_index("log-probs of a library module", "labels", labels, logits.shape[-1])
-    if logits.is_cuda:
-        from ..utils.kernel import token_logprobs
+    from ..utils.kernel import logprobs_of_logits
 
-        return token_logprobs(logits.float(), labels.long())
-    logp = torch.log_softmax(logits.float(), -1)
-    at = labels.long()
-    there = (at >= 0) & (at < logp.shape[-1])
-    lp = torch.where(there, logp.gather(-1, torch.where(there, at, 0)[:, None]).squeeze(-1), 0.0)
-    ent = -(logp.exp() * logp).sum(-1)
-    return lp, ent
+    return logprobs_of_logits(logits.float(), labels.long())
 
 
 class GenericCausalLM:

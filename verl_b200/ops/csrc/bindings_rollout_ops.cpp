@@ -259,8 +259,20 @@ Tensor scores_bwd(const Tensor& logits, const Tensor& given, const Tensor& lse, 
   return dx;
 }
 Tensor token_scores_bwd(const Tensor& logits, const Tensor& given, const Tensor& lse, const Tensor& ent, const Tensor& g_lp, const OptTensor& g_ent,
-                        double temperature, int64_t valid) {
-  return scores_bwd(logits, given, lse, ent, Tensor(), g_lp, g_ent, temperature, valid);
+                        double temperature, int64_t valid, const OptTensor& stat) {
+  if (stat.has_value())
+    TORCH_CHECK(stat->scalar_type() == at::kFloat && stat->dim() == 2 && stat->size(0) == logits.size(0) && stat->size(1) == 4 && stat->is_contiguous() &&
+                stat->device() == logits.device() && reinterpret_cast<uintptr_t>(stat->data_ptr()) % 16 == 0,
+                "token_scores_bwd: stat must be what token_scores_kept returned for these logits");
+  return scores_bwd(logits, given, lse, ent, stat.has_value() ? *stat : Tensor(), g_lp, g_ent, temperature, valid);
+}
+
+// Log-probs, entropy and log-sum-exp with what their gradient wants, for an autograd function that is written elsewhere.
+std::tuple<Tensor, Tensor, Tensor, Tensor> token_scores_kept(const Tensor& logits, const Tensor& given, double temperature, int64_t valid) {
+  TORCH_CHECK(logits.is_cuda(), "token_scores_kept: expected a CUDA tensor");
+  const Tensor stat = stat_of(logits);
+  auto [lp, ent, lse, top, top_lp] = scores(logits, given, 0, temperature, valid, stat.data_ptr<float>());
+  return {lp, ent, lse, stat};
 }
 
 // Log-probs and entropy with their gradient. In C++, because a function written in Python costs more on the host than the kernels of most
@@ -317,5 +329,6 @@ TORCH_LIBRARY_FRAGMENT(verl_b200, m) {
   m.def("paged_decode_kv4", &paged_decode_kv4);
   m.def("token_scores", &token_scores);
   m.def("token_scores_bwd", &token_scores_bwd);
+  m.def("token_scores_kept", &token_scores_kept);
   m.def("token_logprobs", &token_logprobs);
 }

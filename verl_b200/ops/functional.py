@@ -48,6 +48,7 @@ __all__ = [
     "TokenScores",
     "token_scores",
     "token_logprobs",
+    "token_scores_kept",
     "token_scores_bwd",
     "sample_tokens",
     "grpo_advantage",
@@ -974,14 +975,20 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, temperature: float =
     return _ops().token_logprobs(logits, ids, float(temperature), int(valid_vocab))
 
 
+def token_scores_kept(logits: torch.Tensor, ids: torch.Tensor, temperature: float = 1.0, valid_vocab: int = 0):
+    """``(logprob, entropy, lse, stat)`` on a GPU: those of :func:`token_scores` and what :func:`token_scores_bwd` wants of each row, fp32 [T, 4]."""
+    return _ops().token_scores_kept(logits, ids, float(temperature), int(valid_vocab))
+
+
 def token_scores_bwd(logits: torch.Tensor, ids: torch.Tensor, lse: torch.Tensor, entropy: torch.Tensor, g_logprob: torch.Tensor,
-                     g_entropy: Optional[torch.Tensor], temperature: float = 1.0, valid_vocab: int = 0) -> torch.Tensor:
+                     g_entropy: Optional[torch.Tensor], temperature: float = 1.0, valid_vocab: int = 0,
+                     stat: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Gradient of the logits, in their type, from those of ``logprob`` and ``entropy`` (None: none) of :func:`token_scores`. A token that is given
     several times gathers all its gradients; ids outside the vocabulary and columns behind ``valid_vocab`` have none. A log-sum-exp in 32 bits does
-    not hold what the probabilities need, so the rows are read once more for it; ``token_logprobs`` keeps it from its forward pass."""
+    not hold what the probabilities need: ``stat`` does (last result of :func:`token_scores_kept`, GPU), without which the rows are read once more."""
     if logits.is_cuda:
         return _ops().token_scores_bwd(logits, ids, lse.contiguous(), entropy.contiguous(), g_logprob.float().contiguous(),
-                                       g_entropy.float().contiguous() if g_entropy is not None else None, float(temperature), int(valid_vocab))
+                                       g_entropy.float().contiguous() if g_entropy is not None else None, float(temperature), int(valid_vocab), stat)
     V = _scores_args("token_scores_bwd", logits, ids, temperature, valid_vocab)
     T = logits.shape[0]
     if g_logprob.shape != ids.shape or (g_entropy is not None and g_entropy.shape != (T,)) or lse.shape != (T,) or entropy.shape != (T,):

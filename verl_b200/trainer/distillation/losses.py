@@ -132,12 +132,9 @@ def compute_forward_kl_topk(student_logits: Optional[torch.Tensor], teacher_topk
     if student_topk_logp is None:
         there = (teacher_topk_ids >= 0) & (teacher_topk_ids < student_logits.size(-1))
         teacher_topk_ids = torch.where(there, teacher_topk_ids, 0)
-    if student_topk_logp is None and student_logits.is_cuda and student_logits.dtype in (torch.float32, torch.bfloat16, torch.float16):
-        from ...utils.kernel import token_logprobs
+        from ...utils.kernel import logprobs_of_logits
 
-        student_topk_logp = token_logprobs(student_logits, teacher_topk_ids)[0]   # logits read once forward and once backward
-    if student_topk_logp is None:
-        student_topk_logp = torch.log_softmax(student_logits.float(), -1).gather(-1, teacher_topk_ids)
+        student_topk_logp = logprobs_of_logits(student_logits, teacher_topk_ids, entropy=False)[0]   # on a GPU logits read once forward and once backward
     lp_t = teacher_topk_log_probs.float()
     lq_s = student_topk_logp.float()
     if config.log_prob_min_clamp is not None:
