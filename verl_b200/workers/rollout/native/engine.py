@@ -596,11 +596,17 @@ class RolloutEngine:
             self.running[r.slot] = r
 
     def _write_tables(self, slots: Sequence[int], blocks: Sequence[Sequence[int]]) -> None:
-        """The block tables of some sequence slots, from their block lists (one transfer and one launch)."""
+        """The block tables of some sequence slots, from their block lists: one transfer, for which the host does not wait, and one launch. What the
+        launch would refuse without a word is refused here."""
+        n = len(slots)
+        assert len(blocks) == n and all(0 <= s < self.S for s in slots), f"sequence slots {list(slots)} of {self.S}"
         assert all(len(b) <= self.max_blocks_per_seq for b in blocks), "a sequence holds more blocks than max_model_len has"
-        i32 = lambda x: torch.tensor(x, dtype=torch.int32).to(self.device)
-        F.extend_block_tables_(self.block_table, i32(list(slots)), torch.zeros(len(slots), dtype=torch.int32, device=self.device),
-                               i32([len(b) * self.bs for b in blocks]), i32([b for row in blocks for b in row]), self.bs)
+        packed = self._to_device([*slots, *[0] * n, *(len(b) * self.bs for b in blocks), *(b for row in blocks for b in row)])
+        F.extend_block_tables_(self.block_table, packed[:n], packed[n : 2 * n], packed[2 * n : 3 * n], packed[3 * n :], self.bs)
+
+    def _to_device(self, numbers: list[int]) -> torch.Tensor:
+        t = torch.tensor(numbers, dtype=torch.int32)
+        return t.pin_memory().to(self.device, non_blocking=True) if self.is_cuda else t
 
     @torch.no_grad()
     def _run_portions(self, ids: torch.Tensor, starts: list[int], ends: list[int], slots: list[int]):
@@ -611,7 +617,7 @@ class RolloutEngine:
         if self.is_cuda:
             ids = ids.pin_memory().to(dev, non_blocking=True)
         batch = PackedBatch.from_lengths(ids, [b - a for a, b in zip(starts, ends)], device=dev)
-        rows, a, b, zero = torch.tensor([list(slots), list(starts), list(ends), [0] * len(slots)], dtype=torch.int32).to(dev)
+        rows, a, b, zero = self._to_device([*slots, *starts, *ends, *[0] * len(slots)]).view(4, -1)
         _, positions, slot_map = F.build_slot_map(self.block_table, rows, a, b, self.bs, sum(ends) - sum(starts))
         if any(starts):
             batch.positions = positions
