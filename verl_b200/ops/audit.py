@@ -17,7 +17,7 @@ from typing import Optional
 
 import torch
 
-__all__ = ["AuditError", "enabled", "enable", "scope", "check_index", "check_aligned", "check_paged_cache"]
+__all__ = ["AuditError", "enabled", "enable", "scope", "check_index", "check_aligned", "check_paged_cache", "check_kv4_scales"]
 
 _ON = os.environ.get("VERL_B200_AUDIT", "0") == "1"
 
@@ -84,3 +84,14 @@ def check_paged_cache(op: str, block_table: torch.Tensor, ctx_len: torch.Tensor,
     used = (torch.arange(block_table.shape[1], device=block_table.device)[None, :] * block_size) < ctx_len.reshape(-1, 1)
     vals = torch.where(used, block_table, torch.zeros_like(block_table))
     check_index(op, "block_table (entries within each sequence's context)", vals, num_blocks)
+
+
+def check_kv4_scales(op: str, scales: torch.Tensor, block_table: torch.Tensor, ctx_len: torch.Tensor, block_size: int, limit: float) -> None:
+    """Scales [blocks, heads, block_size, groups] of a 4-bit pool lie below ``limit`` (a NaN passes) for the tokens of every sequence's context."""
+    if not _ON or block_table.numel() == 0 or _capturing(block_table):
+        return
+    for b, n in enumerate(ctx_len.tolist()):
+        blocks = block_table[b, : -(-n // block_size)].long()
+        far = (scales[blocks].abs() >= limit).any(-1).any(1).flatten()[:n]
+        if bool(far.any()):
+            raise AuditError(f"{op}: token {int(torch.nonzero(far)[0])} of sequence {b} has a scale of {limit:g} or more, beyond those that kv4_append_ writes")

@@ -788,12 +788,14 @@ def _kv4_plan(ctx: torch.Tensor, most: int) -> torch.Tensor:
 # ----------------------------------------------------------------------------------------------- 4-bit cache
 KV4_GROUP = 32        # channels of a head of a token that share a scale and a least value
 KV4_LIMIT = 7600.0    # largest magnitude that is kept
+KV4_SCALE_LIMIT = 1024.0   # scales lie below it: the attention takes 64 times one in fp16
 
 
 def kv4_page_bytes(block_size: int, head_dim: int) -> int:
     """Bytes of a page of the 4-bit cache: ``block_size`` tokens of one KV head, keys and values. A pool is a uint8 tensor
     [blocks, kv_heads, kv4_page_bytes]; a page holds the codes of the keys [block_size, head_dim / 2], those of the values, then
-    (scale, least value) in fp16 for each group of 32 channels of the keys and of the values: 0.625 bytes an element."""
+    (scale, least value) in fp16 for each group of 32 channels of the keys and of the values: 0.625 bytes an element. Scales lie below 1024, as those
+    that :func:`kv4_append_` writes do."""
     if head_dim <= 0 or head_dim % KV4_GROUP:
         raise ValueError(f"kv4: heads of a multiple of {KV4_GROUP} channels, got {head_dim}")
     if block_size <= 0 or block_size % 16 or block_size > 1024:
@@ -882,7 +884,8 @@ def paged_decode_attention_kv4(q: torch.Tensor, pages: torch.Tensor, block_table
                                scale: Optional[float] = None, plan: Optional[torch.Tensor] = None) -> torch.Tensor:
     """One query token per sequence, ``q`` [B, heads, head_dim], against the first ``ctx_len[b]`` tokens of its row of ``block_table`` [B, blocks]
     in a 4-bit pool: as :func:`paged_decode_attention` over the values that the pool holds; zeros for a context of zero tokens. On a GPU: bf16
-    or fp16, heads of 64 or 128 channels, blocks of 16 to 256 tokens (a power of two), at most 16 query heads to a KV head.
+    or fp16, heads of 64 or 128 channels, blocks of 16 to 256 tokens (a power of two), at most 16 query heads to a KV head. Scales in the pool lie below
+    1024 (audit mode looks at them); beyond that the GPU's numbers are not finite.
 
     ``plan`` (third result of :func:`decode_slot_map` for the same contexts) saves a launch when it is made once for all layers of a step."""
     if q.is_cuda and not audit.enabled():
@@ -899,6 +902,9 @@ def paged_decode_attention_kv4(q: torch.Tensor, pages: torch.Tensor, block_table
         raise ValueError(f"paged_decode_attention_kv4: plan must be int32 [{B + 1}], got {plan.dtype} {tuple(plan.shape)}")
     scale = scale if scale is not None else 1.0 / math.sqrt(hd)
     audit.check_paged_cache("paged_decode_attention_kv4", block_table, ctx_len, pages.shape[0], bs)
+    if audit.enabled():
+        for _, params in _kv4_views(pages, bs, hd):
+            audit.check_kv4_scales("paged_decode_attention_kv4", params[..., 0], block_table, ctx_len, bs, KV4_SCALE_LIMIT)
     if q.is_cuda:
         return _ops().paged_decode_kv4(q, pages, block_table, ctx_len, plan, float(scale))
     out = torch.zeros_like(q)
