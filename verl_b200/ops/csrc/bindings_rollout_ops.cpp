@@ -46,6 +46,7 @@ int type_of(const Tensor& t, bool f32, const char* what) {
 std::tuple<Tensor, Tensor, Tensor> decode_slot_map(const Tensor& table, const Tensor& pos, const Tensor& ctx, const Tensor& active, int64_t bs) {
   check_table(table, "decode_slot_map");
   const int64_t S = table.size(0);
+  TORCH_CHECK(S <= (1 << 30), "decode_slot_map: at most 2^30 rows, got ", S);
   check_vec(pos, at::kInt, S, table, "decode_slot_map: pos");
   check_vec(ctx, at::kInt, S, table, "decode_slot_map: ctx");
   check_vec(active, at::kBool, S, table, "decode_slot_map: active");
@@ -121,7 +122,8 @@ void kv4_append_(const Tensor& k, const Tensor& v, const Tensor& slots, Tensor p
   const int64_t T = k.size(0), nkv = k.size(1), hd = k.size(2);
   const int64_t bs = kv4_block(pages, hd, "kv4_append_");
   TORCH_CHECK_VALUE(pages.size(1) == nkv, "kv4_append_: the pool holds ", pages.size(1), " heads, k has ", nkv);
-  TORCH_CHECK(v.device() == k.device() && pages.device() == k.device() && T <= INT_MAX, "kv4_append_: k, v and the pages on one device");
+  TORCH_CHECK(v.device() == k.device() && pages.device() == k.device(), "kv4_append_: k, v and the pages on one device");
+  TORCH_CHECK(T <= (1 << 30), "kv4_append_: at most 2^30 tokens, got ", T);
   check_vec(slots, at::kLong, T, k, "kv4_append_: slots");
   if (T == 0 || nkv == 0 || pages.size(0) == 0) return;
   for (const Tensor* t : {&k, &v})
@@ -137,6 +139,7 @@ void kv4_append_(const Tensor& k, const Tensor& v, const Tensor& slots, Tensor p
 std::tuple<Tensor, Tensor> kv4_gather(const Tensor& pages, const Tensor& slots, int64_t hd, at::ScalarType dtype) {
   const int64_t bs = kv4_block(pages, hd, "kv4_gather"), T = length(slots), nkv = pages.size(1);
   TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kHalf, "kv4_gather: bf16 or fp16");
+  TORCH_CHECK(T <= (1 << 30), "kv4_gather: at most 2^30 tokens, got ", T);
   check_vec(slots, at::kLong, T, pages, "kv4_gather: slots");
   const c10::cuda::CUDAGuard guard(pages.device());
   Tensor k = at::empty({T, nkv, hd}, pages.options().dtype(dtype)), v = at::empty_like(k);
@@ -202,14 +205,18 @@ VbScores scores_of(const Tensor& x, const Tensor& ids, double temperature, int64
   TORCH_CHECK_VALUE(temperature > 0, what, ": temperature must be positive, got ", temperature);
   TORCH_CHECK_VALUE(valid >= 0 && valid <= x.size(1), what, ": valid_vocab must lie in 0 .. ", x.size(1), ", got ", valid);
   a.type = type_of(x, true, what);
-  TORCH_CHECK(x.size(1) < INT_MAX && x.size(0) <= INT_MAX && (x.stride(1) == 1 || x.size(1) == 1) && ids.device() == x.device() && ids.is_contiguous(), what,
+  TORCH_CHECK((x.stride(1) == 1 || x.size(1) == 1) && ids.device() == x.device() && ids.is_contiguous(), what,
               ": logits and ids on one device, with contiguous rows");
   a.x = x.data_ptr(); a.ldx = x.size(0) <= 1 ? 0 : x.stride(0); a.T = (int)x.size(0); a.V = (int)(valid ? valid : x.size(1));
   a.inv_temp = (float)(1.0 / temperature);
   a.ids = lptr(ids); a.K = ids.dim() == 1 ? 1 : (int)ids.size(1);
   return a;
 }
-Tensor by_rows(const Tensor& x) { return x.dim() == 2 && x.stride(1) != 1 && x.size(1) > 1 ? x.contiguous() : x; }
+// Rows with contiguous columns. Rows and columns are counted in 31 bits, by steps of up to some thousand.
+Tensor by_rows(const Tensor& x) {
+  TORCH_CHECK(x.dim() != 2 || std::max(x.size(0), x.size(1)) <= (1LL << 31) - (1 << 14), "logits of ", x.sizes(), ": at most 2^31 - 2^14 rows and columns");
+  return x.dim() == 2 && x.stride(1) != 1 && x.size(1) > 1 ? x.contiguous() : x;
+}
 
 // `stat`, where the gradient is to follow: [rows, 4] fp32, what it wants of the rows.
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> scores(const Tensor& logits, const Tensor& given, int64_t top, double temperature, int64_t valid, float* stat) {
