@@ -113,3 +113,26 @@ def test_contexts_that_one_warp_works_on_alone(nh, nkv, hd, n, dtype):
     off = max(beside_rounding(o, want) for o in out[:: B // 12])
     print(f"beside rounding {off:.2e}")
     assert off <= BOUND[dtype]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("size", [2.0**18, 2.0**24, 2.0**30, 2.0**40])
+def test_scores_whose_steps_are_larger_than_weights_are_apart(size, dtype):
+    """Scores up to `size`, where fp32 numbers are up to 2^-6 .. 2^16 apart: one token is all of its row's output, however coarse the distances to it are."""
+    nh, nkv, hd, bs, n = 8, 2, 64, 64, 1000
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    pages = pool_of(-(-n // bs), nkv, hd, bs, gen)
+    table = torch.arange(len(pages), device="cuda", dtype=torch.int32).view(1, -1).expand(60, -1).contiguous()
+    q = torch.randn(nh, hd, device="cuda", generator=gen).to(dtype)
+    k, v = rows_of(pages, hd, bs)
+    s = torch.einsum("hgd,htd->hgt", q.double().view(nkv, -1, hd), k[:, :n])
+    scale = size / float(s.abs().max())
+    first, second = (s * scale).topk(2, -1).values.unbind(-1)
+    sure = (first - second > 2.0**-9 * size).flatten()           # what bf16's roundings leave in doubt is left out
+    assert sure.sum() >= 2 and float((first - second).min()) > 100
+    want = torch.gather(v[:, :n], 1, s.argmax(-1)[..., None].expand(-1, -1, hd)).reshape(nh, hd)
+    out = F.paged_decode_attention_kv4(q.expand(60, -1, -1).contiguous(), pages, table, torch.full((60,), n, dtype=torch.int32, device="cuda"), scale=scale)
+    assert out.isfinite().all()
+    # the value itself: two fp16 numbers of at most 11 bits and a sum for bf16, and the output's rounding
+    near = (out.double() - want).abs() <= (2.0**-10 * 5 + 2.0**-8 * want.abs() if dtype == torch.bfloat16 else 2.0**-11 * want.abs() + 2.0**-16)
+    assert near[:, sure].all()

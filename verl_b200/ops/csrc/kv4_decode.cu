@@ -477,8 +477,9 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
             top[h] *= sc[t][h];  // the factor is not negative: its sign is the query's
           }
           const uint32_t column = 0x11111111u << c;  // the lanes of this thread's heads
-          const uint32_t near0 = __ballot_sync(0xffffffffu, top[0] >= m[t][0] + KD_LOW), near1 = __ballot_sync(0xffffffffu, top[1] >= m[t][1] + KD_LOW);
-          const bool high = top[0] > m[t][0] + KD_HIGH || top[1] > m[t][1] + KD_HIGH, low = (near0 & column) == 0u || (near1 & column) == 0u;
+          // distances, which are exact where they are small, however large the scores are
+          const uint32_t near0 = __ballot_sync(0xffffffffu, top[0] - m[t][0] >= KD_LOW), near1 = __ballot_sync(0xffffffffu, top[1] - m[t][1] >= KD_LOW);
+          const bool high = top[0] - m[t][0] > KD_HIGH || top[1] - m[t][1] > KD_HIGH, low = (near0 & column) == 0u || (near1 & column) == 0u;
           if (__any_sync(0xffffffffu, high || low)) {
             float alpha[2];
 #pragma unroll
@@ -490,10 +491,11 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
                 big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, step));
               }
               const int room = KD_ROOM + 127 - static_cast<int>(__float_as_uint(big) >> 23);
-              if (mx > to + KD_HIGH)
-                to = mx - KD_BELOW;
-              else if (mx < to + KD_LOW && mx > -INFINITY && room > 0)
-                to = fmaxf(mx - KD_BELOW, to - static_cast<float>(room));
+              const float below = mx - (mx - KD_BELOW) <= KD_HIGH ? mx - KD_BELOW : mx;  // the score itself where steps are larger
+              if (mx - to > KD_HIGH)
+                to = below;
+              else if (mx - to < KD_LOW && mx > -INFINITY && room > 0)
+                to = fmaxf(below, to - static_cast<float>(room));
               alpha[h] = to == m[t][h] ? 1.f : fast_exp2(m[t][h] - to);
               m[t][h] = to;
               l[t][h] *= alpha[h];
@@ -506,14 +508,25 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
               o[t][i][2] *= alpha[0]; o[t][i][3] *= alpha[1];
             }
           }
+          // Scores of 2^22 and more are rounded as the reference was: half a step of theirs is no exponent of 2 any more
+          const bool far = __any_sync(0xffffffffu, fmaxf(fabsf(m[t][0]), fabsf(m[t][1])) >= 0x1p22f);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float mu = m[t][h] == -INFINITY ? 0.f : m[t][h];
+            float by = sc[t][h];
+            if (far) {
+#pragma unroll
+              for (int i = 0; i < KD_TILES; ++i) {
+                st[t][i][h] = __fmul_rn(st[t][i][h], by);
+                st[t][i][2 + h] = __fmul_rn(st[t][i][2 + h], by);
+              }
+              by = 1.f;
+            }
             float sum = 0.f;  // of the piece first: beside a sum that is far larger its parts would be lost
 #pragma unroll
             for (int i = 0; i < KD_TILES; ++i) {
-              st[t][i][h] = fast_exp2(fmaf(st[t][i][h], sc[t][h], -mu));
-              st[t][i][2 + h] = fast_exp2(fmaf(st[t][i][2 + h], sc[t][h], -mu));
+              st[t][i][h] = fast_exp2(fmaf(st[t][i][h], by, -mu));
+              st[t][i][2 + h] = fast_exp2(fmaf(st[t][i][2 + h], by, -mu));
               sum += st[t][i][h] + st[t][i][2 + h];
             }
             l[t][h] += sum;
