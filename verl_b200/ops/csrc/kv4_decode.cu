@@ -26,10 +26,10 @@
 // code 8, because the sum of codes and that of least values would each be hundreds of times their difference over a long context, and matrix
 // instructions add up by cutting off. That takes two and three matrix instructions for one, and 1.75 times the time where instructions count.
 //
-// 320 sequences of 28 heads over 4 KV heads of 128 channels, 2560 tokens on average: 130 us for 525 MB with the join (0.62 of the copy rate; fp16 200),
-// 5 of them for the reference that follows the scores and the sums that are folded. Neither HBM (57 %) nor the schedulers (0.53 instructions a cycle) are
-// full: three warps to a scheduler, each of which goes through keys, softmax and values one behind the other, do not cover what they wait for. One
-// sequence of 131072 tokens, 8 KV heads: 49 us for 168 MB (fp16 72), 8 of them the join's. Four of 160 tokens: 12 us, two launches.
+// 320 sequences of 28 heads over 4 KV heads of 128 channels, 2560 tokens on average: 119 us for 525 MB with the join (0.68 of the copy rate; fp16 207),
+// 4 of them for the reference that follows the scores. Neither HBM (57 %) nor the schedulers (0.51 instructions a cycle) are full: three warps to a
+// scheduler, each of which goes through keys, softmax and values one behind the other, do not cover what they wait for. One sequence of 131072 tokens,
+// 8 KV heads: 50 us for 168 MB (fp16 74), 8 of them the join's. Four of 160 tokens: 12 us, two launches.
 #include <math.h>
 
 #include <type_traits>
@@ -57,7 +57,7 @@ constexpr int KD_MIN_PIECES = 1;                 // shortest run of a warp
 // that only rises). The sums may then grow to 2^60, which fp32 holds. Weights below 2^-32 of the largest one of their own piece are lost.
 constexpr float KD_BELOW = 8.f, KD_HIGH = 14.f, KD_LOW = -4.f;
 constexpr int KD_ROOM = 60;
-constexpr int KD_FOLD = 32;                      // pieces after which a warp's sums of products go to shared memory
+constexpr int KD_FOLD = 64;                      // pieces after which a warp's sums of products go to shared memory
 
 __device__ int g_kv4_status[4];
 
@@ -174,7 +174,7 @@ __device__ __forceinline__ uint32_t pack2_rest(float lo, float hi, uint32_t roun
   return pack2(lo - __low2float(h), hi - __high2float(h));
 }
 
-template <int HD, int NT>
+template <int HD, int NT, bool FOLD>
 struct KDSmem {
   static constexpr int CODES = KD_PIECE * HD / 2;             // of keys, or of values
   static constexpr int PARAMS = KD_PIECE * (HD / KV4_GROUP) * 4;
@@ -182,7 +182,7 @@ struct KDSmem {
   static constexpr int STAGE = 2 * CODES + 2 * PARAMS;        // of a warp, a multiple of 128 bytes
   static constexpr int SUMS = NT * (HD / 16 + 2) * 512;       // of a warp: four numbers a thread and sum, and the references that they are under
   static constexpr int OFF_SUMS = KD_WARPS * STAGE;
-  static constexpr int OFF_BAR = OFF_SUMS + KD_WARPS * SUMS;
+  static constexpr int OFF_BAR = OFF_SUMS + (FOLD ? KD_WARPS * SUMS : 0);
   static constexpr int TOTAL = OFF_BAR + KD_WARPS * 2 * 8;
 };
 
@@ -237,10 +237,10 @@ __device__ __forceinline__ bool kd_wait(uint64_t* full, uint32_t parity) {
   return true;
 }
 
-template <int HD, int NT, typename T>
+template <int HD, int NT, bool FOLD, typename T>
 __global__ void __launch_bounds__(KD_THREADS, kd_ctas(HD, NT))
 kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
-  using L = KDSmem<HD, NT>;
+  using L = KDSmem<HD, NT, FOLD>;
   constexpr bool FINE = std::is_same<T, __half>::value;  // numbers, queries and weights without a rounding that an output of 11 bits would show
   using Sc = std::conditional_t<FINE, FineScales, Scales>;
   constexpr int PARTS = FINE ? 2 : 1;
@@ -374,8 +374,8 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
     }
     // Matrix instructions add up by cutting off, always towards zero: over thousands of tokens that is far more than what is left where values of either
     // sign cancel (131072 tokens a warp: outputs off by 1.6e-2 of their norm in bf16 and 2.8e-3 in fp16 beside their own rounding). So sums of KD_FOLD
-    // pieces are added up here, rounded to nearest: 2.5e-4 and 3e-6; with 8 pieces 2.1e-4 and 4e-6, in the same time. Every thread
-    // has a place of its own in shared memory. `keep`: what is there is taken along; `back`: it comes back into the registers.
+    // pieces are added up here, rounded to nearest: 3.6e-4 and 5e-6 (of 32: 2.5e-4, 3e-6). Every thread has a place of its own in shared memory. `keep`: what is there is taken
+    // along; `back`: it comes back into the registers.
     const auto fold = [&](bool keep, bool back) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
@@ -406,7 +406,7 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
     };
     for (; u < seg_end; ++u, ++round) {
       const int next = u + 1, done = u - seg;
-      if (done > 0 && done % KD_FOLD == 0) fold(done > KD_FOLD, false);
+      if (FOLD && done > 0 && done % KD_FOLD == 0) fold(done > KD_FOLD, false);
       if (looked == 2) {
         looked = 0;
         if (next < u1) look_all(next);
@@ -609,7 +609,7 @@ kv4_decode_kernel(const VbKv4Decode p, int block_shift, int* status) {
       ++looked;
     }
 
-    if (seg_end - seg > KD_FOLD) fold(true, true);
+    if (FOLD && seg_end - seg > KD_FOLD) fold(true, true);
     // ---- end of a segment. O^T[channel r VPR + 2 i, head] = 16 o + z, and the channel behind it o' - o + z
     const bool whole = seg == g.base && seg_end == g.end;
     float* part = p.part + (2LL * run + (seg == u0 ? 0 : 1)) * G * (HD + 4);
@@ -744,10 +744,10 @@ kv4_plan_kernel(const VbKv4Decode p) {
   }
 }
 
-template <int HD, int NT, typename T>
+template <int HD, int NT, bool FOLD, typename T>
 static cudaError_t kd_launch(const VbKv4Decode& p, int* status, cudaStream_t s) {
-  auto kern = kv4_decode_kernel<HD, NT, T>;
-  constexpr int smem = KDSmem<HD, NT>::TOTAL;
+  auto kern = kv4_decode_kernel<HD, NT, FOLD, T>;
+  constexpr int smem = KDSmem<HD, NT, FOLD>::TOTAL;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   const int ctas = num_sms() * kd_ctas(HD, NT);
@@ -770,11 +770,20 @@ static cudaError_t kd_launch(const VbKv4Decode& p, int* status, cudaStream_t s) 
   return cudaLaunchKernelEx(&cfg, kv4_join_kernel<HD, T>, p, runs, heads);
 }
 
+// The kernel without folding where no warp can have more than KD_FOLD pieces of a (sequence, head), which the size of the table says: 320 sequences of
+// up to 4096 tokens take 119 us (fp16 207), and 125 (213) with the other one, which folds nothing there either but has other registers.
+template <int HD, int NT, typename T>
+static cudaError_t kd_fold(const VbKv4Decode& p, int* status, cudaStream_t s) {
+  const long long most = (static_cast<long long>(p.width) * p.block_size + KD_PIECE - 1) / KD_PIECE, runs = num_sms() * kd_ctas(HD, NT) * KD_WARPS;
+  const long long run = (most * p.B * p.nkv + runs - 1) / runs;
+  return min(most, run) > KD_FOLD ? kd_launch<HD, NT, true, T>(p, status, s) : kd_launch<HD, NT, false, T>(p, status, s);
+}
+
 template <typename T>
 static cudaError_t kd_dispatch(const VbKv4Decode& p, int* status, cudaStream_t s) {
   const bool wide = p.nh / p.nkv > 8;
-  if (p.hd == 128) return wide ? kd_launch<128, 2, T>(p, status, s) : kd_launch<128, 1, T>(p, status, s);
-  return wide ? kd_launch<64, 2, T>(p, status, s) : kd_launch<64, 1, T>(p, status, s);
+  if (p.hd == 128) return wide ? kd_fold<128, 2, T>(p, status, s) : kd_fold<128, 1, T>(p, status, s);
+  return wide ? kd_fold<64, 2, T>(p, status, s) : kd_fold<64, 1, T>(p, status, s);
 }
 
 }  // namespace vb
