@@ -8,7 +8,7 @@
 //
 // Both kernels move bytes: 8 channels of a token a thread (16 bytes of input, 4 of codes), four threads a group, the group's extremes by two shuffles.
 // 16384 tokens of 8 heads of 128 channels: append 39 us for 88 MB (2.3 TB/s), gather 23 us for 88 MB (3.8 TB/s), both bound by the instructions
-// that they issue (about 200 and 110 for the 8 channels of a thread, a slot's address and a group's parameters among them; 0.74 and 0.7 a cycle and
+// that they issue (about 200 and 110 for the 8 channels of a thread, a slot's address and a group's parameters among them; 0.74 and 0.66 a cycle and
 // scheduler). With a block for every few tokens append took 53 us and gather 30: each thread works out its place by divisions. A decode step's few tokens
 // cost a launch, 6 us.
 #include "kv4_common.cuh"

@@ -119,7 +119,7 @@ constexpr int SM_THREADS = 256;
 constexpr int SM_TOKENS = 4;  // consecutive tokens of a thread: 16 and 32 bytes of output
 constexpr int SM_OWN_SUMS = 8192;  // sequences whose sums fit the shared memory that every launch has
 constexpr int SM_TURNS = 4;   // times that a block goes on: its sums over the batch are made once for 4096 tokens
-// 512 sequences of 2.3 million tokens: 15 us for 28 MB (1.9 TB/s; 4.5 us at the copy rate) in 568 blocks. A block's time is a chain: two sums over the
+// 512 sequences of 2.3 million tokens: 13 us for 28 MB (2.1 TB/s; 4.5 us at the copy rate) in 568 blocks. A block's time is a chain: two sums over the
 // batch, the search for its sequences, row and start, page, stores. Look-ups token by token, of which a warp nearly always needs some, took 17 us.
 
 // cu[i + 1]: the tokens up to and with sequence i, no more than `total` of them.

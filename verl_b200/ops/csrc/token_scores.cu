@@ -19,7 +19,7 @@
 // logarithm of the sum that the forward pass left, not from their sum, the log-sum-exp.
 //
 // Measured, rows of 152064: 2048 of bf16 without alternatives 104 us (6.0 TB/s, 0.93 of the copy rate), with 64 of them 135 us, with 128 161 us; the same in
-// fp32 219 us with 64 (0.88); their gradient, which reads once and writes once, 205 us in bf16 (0.94). One row of 151936: 12 us. What bounds the bf16
+// fp32 221 us with 64 (0.87); their gradient, which reads once and writes once, 209 us in bf16 (0.92). One row of 151936: 12 us. What bounds the bf16
 // forward is HBM beside its exponentials (70 us at the 16 a cycle that an SM has), and with alternatives the end of a row (15000 cycles of 75000:
 // the bound 2300, the groups 2300, their values from memory 6600, ranks 4200), a chain that an SM's three other blocks do not cover: blocks that
 // start a part of a row apart take as long. 256 threads and four blocks an SM: with fewer blocks less covers that end, with more the registers do not
